@@ -318,6 +318,71 @@ int w4a16_gemm_prenorm(const void* x, const void* row_stats, const void* norm_we
                        int N, int K, int group_size, void* stream, unsigned flags);
 
 /*
+ * The paged 4-bit key/value cache ("kv4").  No counterpart in the reference, which keeps keys and values in fp16 and grows them with
+ * torch.cat (modeling_opt_ours.py:249-250).  A token's row of one head is quantised by groups of g dims: m = the group's minimum
+ * (fp16), s = fp16((maximum - minimum) / 15), codes n = rint((x - m) / s) in 0..15; it stands for m + n s.  A group that holds an
+ * infinity or a NaN reads back as NaN.
+ *   pool    uint8 [layers][pages][kv_heads][page_size / 16][tile bytes], 16-byte aligned; `pool` of the calls on one layer is that
+ *           layer's part.  A tile holds 16 tokens of one head: K codes, K (s, m), V codes, V (s, m) (w4a16_kv4_tile_bytes bytes;
+ *           the order of codes inside a row is that of csrc/w4a16_kv4.cuh).  Fresh pools must be zeroed or at least hold no token
+ *           that is read before it was written.
+ *   table   int32 [rows][width]: page numbers of each row's tokens 0 .. page_size-1, page_size .. ; -1 where it has none
+ *   pos     int32 [batch]: position of the row's first new token; negative: the batch row holds no sequence, nothing of it is read
+ *           and its outputs stay as they were
+ *   counts  int32 [batch] or NULL: new tokens of the row, at most `seq` (NULL: seq); outputs of the others stay as they were
+ * head_dim 64 or 128, g 32, 64 or 128 and at most head_dim, page_size a power of two from 16 to 1024, heads a multiple of kv_heads
+ * (query head h reads key/value head h / (heads / kv_heads)), width * page_size < 2^30.  Positions, page and row numbers are read
+ * on the device, so that a captured graph can be replayed: one out of range raises the device error word and is left out - 3: a
+ * position outside the table or the rotary tables (that token or query is skipped), 4: a page number outside the pool (its tokens
+ * are neither written nor attended to), 5: fewer free pages than asked for, 6: a row number outside the table, a fork into a row
+ * in use, a broken reference count.  Nothing is allocated; calls that write the same pages must be ordered by the caller.
+ */
+size_t w4a16_kv4_tile_bytes(int head_dim, int group);      /* 0: no such format */
+/* Keys (with rotary embedding where tables are given) and values of `seq` tokens a row, quantised into their pages.
+ *   qkv     fp16 [batch][seq] rows of qkv_stride elements, a multiple of 8: q (heads*head_dim) | k (kv_heads*head_dim) | v; 16-byte
+ *           aligned.  q is not read.
+ *   rope_cos, rope_sin  fp16 [rope_rows][head_dim] tables over all positions ("rotate half"), or both NULL; keys are rotated in
+ *           fp32 and rounded to fp16 before they are quantised */
+int w4a16_kv4_append(const void* qkv, void* pool, const void* table, const void* pos, const void* counts, const void* rope_cos,
+                     const void* rope_sin, int batch, int seq, int heads, int kv_heads, int head_dim, int group, int page_size,
+                     int pages, int width, long long qkv_stride, int rope_rows, void* stream);
+/* k, v fp16 [batch][kv_heads][seq][head_dim]: the values of tokens pos .. pos + count - 1, zeros where a row has no such token. */
+int w4a16_kv4_read(const void* pool, const void* table, const void* pos, const void* counts, void* k, void* v, int batch, int seq,
+                   int kv_heads, int head_dim, int group, int page_size, int pages, int width, void* stream);
+/* One new token per row: its key and value are appended and attention runs over positions 0 .. pos.  qkv [batch] rows as above,
+ * out fp16 [batch][heads*head_dim].  q is rotated and rounded to fp16; scores, softmax and sums are fp32. */
+int w4a16_kv4_decode_attention(const void* qkv, void* pool, const void* table, const void* pos, const void* rope_cos,
+                               const void* rope_sin, void* out, int batch, int heads, int kv_heads, int head_dim, int group,
+                               int page_size, int pages, int width, long long qkv_stride, int rope_rows, float scale, void* stream);
+/* Causal attention of a chunk: query i of a row (position pos + i) over positions 0 .. pos + i, all of which the cache holds (append
+ * first).  qkv rows need hold the queries only (qkv_stride >= heads*head_dim); out fp16 [batch][seq][heads*head_dim]. */
+int w4a16_kv4_attention(const void* qkv, const void* pool, const void* table, const void* pos, const void* counts,
+                        const void* rope_cos, const void* rope_sin, void* out, int batch, int seq, int heads, int kv_heads,
+                        int head_dim, int group, int page_size, int pages, int width, long long qkv_stride, int rope_rows,
+                        float scale, void* stream);
+/* Pages.  lens int32 [rows] are the tokens of each row, refs int32 [pages] the number of rows that hold each page; a page is free
+ * when nobody holds it.  Free pages are dealt lowest number first, to rows (forks) in order; from the first that cannot be served
+ * on nobody gets pages.  Two calls on the same table must not overlap.
+ *   reserve  room for counts[r] more tokens of row r: pos[r] = lens[r], lens[r] += counts[r] and the pages that this needs; pos[r] = -1
+ *            and nothing else where counts[r] <= 0 or the row cannot be served.  rows <= 8192
+ *   fork     row dst[i] (empty) continues row src[i]: whole pages are shared, the last, partly filled one is copied (all layers,
+ *            filled tiles), so that pages more than one row holds are never written.  Sources are taken as before the call.
+ *            A pair that names a row out of range, a row in use or an earlier pair's destination is refused.  n <= 8192
+ *   free     the rows give their pages back and are empty afterwards; naming a row twice is the same as once
+ *   compact  the pages in use become the first ones: those above move to the free ones below, both in order, and the table and
+ *            refs follow.  Contents above are left behind. */
+int w4a16_kv4_reserve(void* table, void* lens, void* refs, const void* counts, void* pos, int rows, int width, int pages,
+                      int page_size, void* stream);
+int w4a16_kv4_free(void* table, void* lens, void* refs, const void* which, int n, int rows, int width, int pages, void* stream);
+size_t w4a16_kv4_fork_workspace(int n, int rows);           /* bytes, 4-byte aligned; like all workspaces not shared by calls in flight */
+int w4a16_kv4_fork(void* pool, void* table, void* lens, void* refs, const void* src, const void* dst, void* workspace,
+                   size_t workspace_bytes, int n, int rows, int width, int layers, int pages, int kv_heads, int head_dim, int group,
+                   int page_size, void* stream);
+size_t w4a16_kv4_compact_workspace(int pages);
+int w4a16_kv4_compact(void* pool, void* table, void* refs, void* workspace, size_t workspace_bytes, int rows, int width, int layers,
+                      int pages, int kv_heads, int head_dim, int group, int page_size, void* stream);
+
+/*
  * No counterpart in the reference.  The tcgen05 GEMM with K split in two, for callers that cannot
  * allocate device memory (inside stream capture, inside a host runtime that owns the allocator, or
  * with a memory budget pinned at start-up): the fp32 partial tiles, the arrival counters and the

@@ -1,0 +1,141 @@
+// The paged 4-bit key/value cache: format, addressing and what its kernels share.
+//
+// Every token's key and value row of one head is quantised by groups of G dims: m = min (fp16, exact), s = fp16((max - min) / 15),
+// code n = rint((x - m) / s) in 0..15 (ties to even); the row stands for m + n s.  A group that holds an infinity or a NaN gets
+// s = NaN, so that it reads back as NaN instead of as some finite values.
+//
+// 16 tokens of one head are a tile, contiguous and a multiple of 64 bytes:
+//     K codes [16][D/2] | K (s, m) half2 [16][D/G] | V codes [16][D/2] | V (s, m) half2 [16][D/G]
+// and a page is [kv heads][page size / 16] tiles, so that one head's part of a page is one contiguous run for the copy engine.
+//
+// Order inside a code row: what a lane of an mma.m16n8k16 fragment needs is adjacent.
+//   K (A operand, rows = tokens, k = dims): word w of 8 dims (8w .. 8w+7, nibble i = dim 8w + i) stands at word
+//     (w % 4) * (D/32) + w / 4: lane c = w % 4 of a row reads its D/32 words in one load.
+//   V (A operand, rows = dims, k = tokens): half-word h of 4 dims (4h .. 4h+3) stands at half-word (h % 8) * (D/32) + h / 8: lane
+//     r = h % 8 reads its D/32 half-words of a token in one load.  At D = 128 the 32-byte halves of rows with bit 1 set are
+//     exchanged, which keeps the four rows that a quarter of a warp reads together on different shared-memory banks.
+#pragma once
+
+#include "w4a16_common.cuh"
+
+namespace w4a16 {
+namespace kv4 {
+
+constexpr int kTile = 16;                         // tokens of a tile
+
+// values of the device error word (0: none; 1 to 3 are the other kernels')
+constexpr int kErrPosition = 3;                   // a position outside the table or the rotary tables
+constexpr int kErrPage = 4;                       // a page number outside the pool where a page is needed
+constexpr int kErrNoPages = 5;                    // fewer free pages than were asked for
+constexpr int kErrRow = 6;                        // a row number outside the table, a fork into a row in use, a broken reference count
+
+__host__ __device__ constexpr int tile_bytes(int D, int G) { return 16 * D + 128 * D / G; }
+
+template <int D, int G>
+struct Fmt {
+    static constexpr int J = D / 32;                          // words of a lane per key row, half-words per value row
+    static constexpr int NW = D / 8;                          // words of a code row
+    static constexpr int NG = D / G;                          // groups of a row
+    static constexpr int kKeyPar = kTile * D / 2;             // byte offsets inside a tile
+    static constexpr int kVal = kKeyPar + kTile * NG * 4;
+    static constexpr int kValPar = kVal + kTile * D / 2;
+    static constexpr int kBytes = kValPar + kTile * NG * 4;
+    __device__ static constexpr int key_word(int row, int w) { return row * (D / 2) + 4 * ((w % 4) * J + w / 4); }
+    __device__ static constexpr int val_half(int row, int h)
+    {
+        const int at = 2 * ((h % 8) * J + h / 8);
+        return kVal + row * (D / 2) + (D == 128 ? at ^ (((row >> 1) & 1) << 5) : at);
+    }
+    __device__ static constexpr int key_par(int row, int g) { return kKeyPar + (row * NG + g) * 4; }
+    __device__ static constexpr int val_par(int row, int g) { return kValPar + (row * NG + g) * 4; }
+};
+static_assert(Fmt<128, 64>::kBytes == tile_bytes(128, 64) && Fmt<64, 32>::kBytes == tile_bytes(64, 32), "tile size");
+
+// One layer's pages and the table that says which of them a row of the batch holds.
+struct Cache {
+    unsigned char* pool;             // [pages][kv heads][page size / 16][tile bytes]
+    const int* table;                // [batch][width] page numbers
+    int pages, width, page_shift;    // page size = 1 << page_shift tokens
+    int kv_heads;
+    __device__ __forceinline__ int capacity() const { return width << page_shift; }
+    // the tile with token t of (row, head); null when the table holds no page of the pool there
+    __device__ __forceinline__ unsigned char* tile(int row, int head, int t, int bytes) const
+    {
+        const int page = table[(size_t)row * width + (t >> page_shift)];
+        if ((unsigned)page >= (unsigned)pages) return nullptr;
+        const int per = 1 << (page_shift - 4);                                  // tiles of one head in a page
+        return pool + (((size_t)page * kv_heads + head) * per + ((t >> 4) & (per - 1))) * (size_t)bytes;
+    }
+};
+
+// Eight dims of a row from a quantisation group spread over `lanes` adjacent lanes: (s, m) of the group and the eight codes.
+// Every step is one IEEE fp32 operation, so the codes are the same integers that elementary tensor operations give.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], int lanes, __half2& par)
+{
+    float lo = x[0], hi = x[0];
+    bool odd = !(fabsf(x[0]) <= 65504.f);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+        odd |= !(fabsf(x[i]) <= 65504.f);
+    }
+    int any = odd;
+    for (int o = 1; o < lanes; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        any |= __shfl_xor_sync(0xffffffffu, any, o);
+    }
+    const __half sh = any ? __ushort_as_half(0x7fff) : __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+    const float s = __half2float(sh);
+    par = __halves2half2(sh, __float2half_rn(lo));
+    uint32_t word = 0;
+    if (s > 0.f) {                                                              // not at s = 0 (all values m) and NaN
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            word |= (uint32_t)fminf(rintf(__fdiv_rn(__fsub_rn(x[i], lo), s)), 15.f) << (4 * i);
+    }
+    return word;
+}
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
+{
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(h[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+    }
+}
+
+// Word w (dims 8w .. 8w+7) of a head row at `src` with the rotary embedding of position t ("rotate half"), rounded to fp16 as the
+// fp16 cache holds keys; fp32 products and sum, each rounded.
+template <int D>
+__device__ __forceinline__ void load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t, float (&x)[8])
+{
+    unpack8(*reinterpret_cast<const uint4*>(src + 8 * w), x);
+    if (!cos) return;
+    float y[8], c[8], s[8];
+    unpack8(*reinterpret_cast<const uint4*>(src + 8 * (w ^ (D / 16))), y);
+    unpack8(*reinterpret_cast<const uint4*>(cos + (size_t)t * D + 8 * w), c);
+    unpack8(*reinterpret_cast<const uint4*>(sin + (size_t)t * D + 8 * w), s);
+    const float sign = w < D / 16 ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = __half2float(__float2half_rn(__fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(sign * y[i], s[i]))));
+}
+
+// Arguments every entry point with a pool checks alike; fills c.
+int check_cache(Cache& c, const void* pool, const void* table, int pages, int width, int page_size, int kv_heads, int head_dim, int group);
+
+// Calls f(Fmt<D, G>) for the head size and group that were checked before.
+template <class F>
+int with_format(int D, int G, F f)
+{
+    if (D == 128) return G == 32 ? f(Fmt<128, 32>{}) : G == 64 ? f(Fmt<128, 64>{}) : f(Fmt<128, 128>{});
+    return G == 32 ? f(Fmt<64, 32>{}) : f(Fmt<64, 64>{});
+}
+
+}  // namespace kv4
+}  // namespace w4a16

@@ -1,0 +1,612 @@
+// The paged 4-bit key/value cache: quantise-and-append, read back, and the operations on its pages.
+#include "w4a16_kv4.cuh"
+
+namespace w4a16 {
+namespace kv4 {
+
+int check_cache(Cache& c, const void* pool, const void* table, int pages, int width, int page_size, int kv_heads, int head_dim, int group)
+{
+    if (!pool || !table) return W4A16_ERR_NULL_POINTER;
+    if (group != 32 && group != 64 && group != 128) return W4A16_ERR_GROUP_SIZE;
+    if ((head_dim != 64 && head_dim != 128) || group > head_dim) return W4A16_ERR_BAD_SHAPE;
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) || pages <= 0 || width <= 0 || kv_heads <= 0)
+        return W4A16_ERR_BAD_SHAPE;
+    if ((long long)width * page_size >= (1ll << 30)) return W4A16_ERR_TOO_LARGE;     // positions are 32-bit
+    if (((uintptr_t)pool & 15) || ((uintptr_t)table & 3)) return W4A16_ERR_MISALIGNED;
+    c.pool = (unsigned char*)pool;
+    c.table = (const int*)table;
+    c.pages = pages; c.width = width; c.kv_heads = kv_heads;
+    c.page_shift = 0;
+    while ((1 << c.page_shift) < page_size) ++c.page_shift;
+    return W4A16_OK;
+}
+
+namespace {
+
+struct AppendArgs {
+    Cache c;
+    const __half* qkv;
+    const int* pos;
+    const int* counts;            // null: seq tokens in every row
+    const __half* cos;
+    const __half* sin;
+    int* error;
+    int seq, rope_rows;
+    int key_at, val_at;           // first element of the keys and of the values in a token's row
+    long long stride;
+    long long units;              // batch * kv heads * seq
+};
+
+// A (token, head) unit is 2 D/8 lanes: the first half take the key row's words of 8 dims, the others the value row's.  Tokens run
+// fastest, so that the 16 rows of a tile are written close together.  Bound: memory (reads 4 D bytes, writes tile bytes / 16).
+template <class F, int D>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
+{
+    constexpr int kUnit = 2 * F::NW, kPer = 256 / kUnit;
+    const long long u = (long long)blockIdx.x * kPer + threadIdx.x / kUnit;
+    const int l = threadIdx.x % kUnit, w = l % F::NW;
+    const bool value = l >= F::NW;
+    bool live = u < a.units;
+    int s = 0, head = 0, b = 0, t = 0;
+    if (live) {
+        s = (int)(u % a.seq);
+        const long long bh = u / a.seq;
+        head = (int)(bh % a.c.kv_heads);
+        b = (int)(bh / a.c.kv_heads);
+        const int p = a.pos[b];
+        live = p >= 0 && (!a.counts || s < a.counts[b]);
+        if (live && (p > a.c.capacity() || p + s >= a.c.capacity() || (a.cos && p + s >= a.rope_rows))) {
+            live = false;
+            atomicExch(a.error, kErrPosition);
+        }
+        t = p + s;
+    }
+    unsigned char* tile = nullptr;
+    if (live) {
+        tile = a.c.tile(b, head, t, F::kBytes);
+        if (!tile) atomicExch(a.error, kErrPage);
+    }
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (tile) {
+        const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + (value ? a.val_at : a.key_at) + head * D;
+        load_rotated<D>(row, w, value ? nullptr : a.cos, a.sin, t, x);
+    }
+    constexpr int kLanes = D / F::NG / 8;                                       // lanes of a group
+    __half2 par;
+    const uint32_t word = quantize8(x, kLanes, par);                            // (all lanes: shuffles)
+    if (!tile) return;
+    const int r = t & 15;
+    if (!value) {
+        *reinterpret_cast<uint32_t*>(tile + F::key_word(r, w)) = word;
+    } else {
+        *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w)) = (uint16_t)word;
+        *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w + 1)) = (uint16_t)(word >> 16);
+    }
+    if (w % kLanes == 0) *reinterpret_cast<__half2*>(tile + (value ? F::val_par(r, w / kLanes) : F::key_par(r, w / kLanes))) = par;
+}
+
+struct ReadArgs {
+    Cache c;
+    const int* pos;
+    const int* counts;
+    __half* k;
+    __half* v;
+    int* error;
+    int seq;
+    long long units;
+};
+
+// The same units as append_kernel; out [batch][kv heads][seq][D], zeros where a row has no such token.
+template <class F, int D>
+__global__ void __launch_bounds__(256) read_kernel(const ReadArgs a)
+{
+    constexpr int kUnit = 2 * F::NW, kPer = 256 / kUnit;
+    const long long u = (long long)blockIdx.x * kPer + threadIdx.x / kUnit;
+    const int l = threadIdx.x % kUnit, w = l % F::NW;
+    const bool value = l >= F::NW;
+    if (u >= a.units) return;
+    const int s = (int)(u % a.seq);
+    const long long bh = u / a.seq;
+    const int head = (int)(bh % a.c.kv_heads), b = (int)(bh / a.c.kv_heads);
+    const int p = a.pos[b];
+    const unsigned char* tile = nullptr;
+    if (p >= 0 && (!a.counts || s < a.counts[b])) {
+        if (p > a.c.capacity() || p + s >= a.c.capacity()) {
+            atomicExch(a.error, kErrPosition);
+        } else {
+            tile = a.c.tile(b, head, p + s, F::kBytes);
+            if (!tile) atomicExch(a.error, kErrPage);
+        }
+    }
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (tile) {
+        const int r = (p + s) & 15, g = w * 8 * F::NG / D;
+        uint32_t word;
+        if (!value) {
+            word = *reinterpret_cast<const uint32_t*>(tile + F::key_word(r, w));
+        } else {
+            word = *reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w)) |
+                   (uint32_t)*reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w + 1)) << 16;
+        }
+        const float2 par = __half22float2(*reinterpret_cast<const __half2*>(tile + (value ? F::val_par(r, g) : F::key_par(r, g))));
+        __half2* o = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            o[e] = __floats2half2_rn(fmaf((float)((word >> (8 * e)) & 15), par.x, par.y), fmaf((float)((word >> (8 * e + 4)) & 15), par.x, par.y));
+    }
+    *reinterpret_cast<uint4*>((value ? a.v : a.k) + u * D + 8 * w) = out;
+}
+
+// ---- pages -------------------------------------------------------------------------------------------------------------------
+// refs[p]: rows that hold page p; free pages are the ones nobody holds and are dealt lowest number first, to rows (or forks) in
+// order.  All bookkeeping of a call is one block of 1024 threads: a few thousand integers, bound by latency.
+
+constexpr int kPageThreads = 1024;
+constexpr int kMaxRows = 8192;                    // rows of a reserve, pairs of a fork: their demand is kept in shared memory
+
+// inclusive sum over the block; total in `total`.  Ends with a barrier.
+__device__ __forceinline__ int block_sum(int v, int* warp_s, int& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+    }
+    if (lane == 31) warp_s[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        int s = warp_s[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int n = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += n;
+        }
+        warp_s[lane] = s;
+    }
+    __syncthreads();
+    const int before = warp ? warp_s[warp - 1] : 0;
+    total = warp_s[31];
+    __syncthreads();
+    return v + before;
+}
+
+// running[i] = demand of entries 0 .. i; returns the whole demand
+__device__ int sum_demand(int* running, int n, int* warp_s)
+{
+    int base = 0, total;
+    for (int i0 = 0; i0 < n; i0 += kPageThreads) {
+        const int i = i0 + threadIdx.x;
+        const int v = block_sum(i < n ? running[i] : 0, warp_s, total);
+        if (i < n) running[i] = base + v;
+        base += total;
+    }
+    __syncthreads();
+    return base;
+}
+
+__device__ int count_free(const int* refs, int pages, int* warp_s)
+{
+    int mine = 0, total;
+    for (int p = threadIdx.x; p < pages; p += kPageThreads) mine += refs[p] == 0;
+    block_sum(mine, warp_s, total);
+    return total;
+}
+
+// Deals the lowest `wanted` free pages: give(k, page) for k = 0, 1, ... in the order of the page numbers.
+template <class Give>
+__device__ void deal_free(const int* refs, int pages, int wanted, int* warp_s, Give give)
+{
+    int base = 0, total;
+    for (int p0 = 0; p0 < pages && base < wanted; p0 += kPageThreads) {
+        const int p = p0 + threadIdx.x;
+        const int free = p < pages && refs[p] == 0;
+        const int k = base + block_sum(free, warp_s, total) - 1;
+        if (free && k < wanted) give(k, p);
+        base += total;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ int first_above(const int* running, int n, int k)    // the entry that the k-th page belongs to
+{
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (running[mid] > k) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPageThreads) reserve_kernel(int* table, int* lens, int* refs, const int* counts, int* pos, int rows,
+                                                               int width, int pages, int page_shift, int* error)
+{
+    extern __shared__ int running[];
+    __shared__ int warp_s[32];
+    const int P = 1 << page_shift;
+    const long long capacity = (long long)width << page_shift;
+    for (int r = threadIdx.x; r < rows; r += kPageThreads) {
+        const int c = counts[r], n = lens[r];
+        int need = 0;
+        bool ok = c > 0;
+        if (ok && (n < 0 || (long long)n + c > capacity)) {
+            ok = false;
+            atomicExch(error, kErrPosition);
+        }
+        if (ok) need = (int)(((long long)n + c + P - 1) >> page_shift) - ((n + P - 1) >> page_shift);
+        pos[r] = ok ? n : -1;
+        running[r] = need;
+    }
+    __syncthreads();
+    const int wanted = sum_demand(running, rows, warp_s);
+    int fits = rows;                                                            // rows below this one get what they asked for
+    if (wanted > 0) {
+        const int free = count_free(refs, pages, warp_s);
+        if (free < wanted) {
+            fits = first_above(running, rows, free);                            // running[fits] > free: the first row that does not fit
+            if (threadIdx.x == 0) atomicExch(error, kErrNoPages);
+        }
+        const int deal = fits < rows ? (fits ? running[fits - 1] : 0) : wanted;
+        deal_free(refs, pages, deal, warp_s, [&](int k, int p) {
+            const int r = first_above(running, rows, k), i = k - (r ? running[r - 1] : 0);
+            table[(size_t)r * width + ((lens[r] + P - 1) >> page_shift) + i] = p;
+        });
+        // (reference counts are changed only after the last block of them has been read)
+        for (int r = threadIdx.x; r < fits; r += kPageThreads) {
+            const int n = running[r] - (r ? running[r - 1] : 0);
+            for (int i = 0; i < n; ++i) refs[table[(size_t)r * width + ((lens[r] + P - 1) >> page_shift) + i]] = 1;
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < rows; r += kPageThreads) {
+        if (pos[r] < 0) continue;
+        if (r >= fits && running[r] > (r ? running[r - 1] : 0)) pos[r] = -1;     // asked for pages and got none: as it was
+        else lens[r] += counts[r];
+    }
+}
+
+// Each (entry, column) hands its page back once, however often a row is named.
+__global__ void __launch_bounds__(256) free_kernel(int* table, int* lens, int* refs, const int* rows, int n_rows, int width, int pages, int* error)
+{
+    const int r = rows[blockIdx.x];
+    if ((unsigned)r >= (unsigned)n_rows) {
+        if (threadIdx.x == 0) atomicExch(error, kErrRow);
+        return;
+    }
+    for (int i = threadIdx.x; i < width; i += blockDim.x) {
+        const int p = atomicExch(table + (size_t)r * width + i, -1);
+        if (p < 0) continue;
+        if (p >= pages) {
+            atomicExch(error, kErrPage);
+        } else if (atomicSub(refs + p, 1) <= 0) {
+            atomicAdd(refs + p, 1);
+            atomicExch(error, kErrRow);
+        }
+    }
+    if (threadIdx.x == 0) lens[r] = 0;
+}
+
+struct ForkArgs {
+    int* table;
+    int* lens;
+    int* refs;
+    const int* src;
+    const int* dst;
+    int* moves;                   // [n][4]: source page, new page, tiles, unused; source page -1: nothing to copy
+    int* mark;                    // [rows]: the first pair that names a row as destination
+    int* error;
+    int n, rows, width, pages, page_shift;
+};
+
+__global__ void __launch_bounds__(kPageThreads) fork_kernel(const ForkArgs a)
+{
+    extern __shared__ int running[];
+    __shared__ int warp_s[32];
+    const int P = 1 << a.page_shift, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r = threadIdx.x; r < a.rows; r += kPageThreads) a.mark[r] = 0x7fffffff;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n; i += kPageThreads)
+        if ((unsigned)a.dst[i] < (unsigned)a.rows) atomicMin(a.mark + a.dst[i], i);
+    __syncthreads();
+    // a warp takes a pair: is it sound, and does it need a page?  (moves: source page or -1, length or -1 where it is refused)
+    for (int i = warp; i < a.n; i += kPageThreads / 32) {
+        const int s = a.src[i], d = a.dst[i];
+        int why = 0, n = 0;
+        if ((unsigned)s >= (unsigned)a.rows || (unsigned)d >= (unsigned)a.rows || a.mark[d] != i || a.lens[d] != 0) why = kErrRow;
+        if (!why) {
+            n = a.lens[s];
+            if (n < 0 || n > a.width << a.page_shift) why = kErrPosition;
+        }
+        if (!why) {
+            bool bad = false;
+            for (int col = lane; col < (n + P - 1) >> a.page_shift; col += 32)
+                bad |= (unsigned)a.table[(size_t)s * a.width + col] >= (unsigned)a.pages;
+            if (__any_sync(0xffffffffu, bad)) why = kErrPage;
+            bool used = false;
+            for (int col = lane; col < a.width; col += 32) used |= a.table[(size_t)d * a.width + col] >= 0;
+            if (__any_sync(0xffffffffu, used)) why = kErrRow;
+        }
+        if (lane == 0) {
+            if (why) atomicExch(a.error, why);
+            const int part = why ? 0 : n & (P - 1);
+            running[i] = part > 0;
+            a.moves[4 * i] = part ? a.table[(size_t)s * a.width + (n >> a.page_shift)] : -1;
+            a.moves[4 * i + 1] = -1;
+            a.moves[4 * i + 2] = (part + 15) >> 4;
+            a.moves[4 * i + 3] = why ? -1 : n;
+        }
+    }
+    __syncthreads();
+    const int wanted = sum_demand(running, a.n, warp_s);
+    int fits = a.n;
+    if (wanted > 0) {
+        const int free = count_free(a.refs, a.pages, warp_s);
+        if (free < wanted) {
+            fits = first_above(running, a.n, free);
+            if (threadIdx.x == 0) atomicExch(a.error, kErrNoPages);
+        }
+        const int deal = fits < a.n ? (fits ? running[fits - 1] : 0) : wanted;
+        deal_free(a.refs, a.pages, deal, warp_s, [&](int k, int p) { a.moves[4 * first_above(running, a.n, k) + 1] = p; });
+    }
+    for (int i = warp; i < a.n; i += kPageThreads / 32) {
+        const int n = a.moves[4 * i + 3], page = a.moves[4 * i + 1];
+        const bool part = a.moves[4 * i] >= 0;
+        __syncwarp();
+        if (n <= 0 || (part && page < 0)) {                                      // refused, empty, or no page left for it
+            if (lane == 0) a.moves[4 * i] = -1;
+            continue;
+        }
+        const int s = a.src[i], d = a.dst[i], full = n >> a.page_shift;
+        for (int col = lane; col < full; col += 32) {
+            const int p = a.table[(size_t)s * a.width + col];
+            a.table[(size_t)d * a.width + col] = p;
+            atomicAdd(a.refs + p, 1);
+        }
+        if (lane == 0) {
+            if (part) {
+                a.table[(size_t)d * a.width + full] = page;
+                a.refs[page] = 1;
+            }
+            a.lens[d] = n;
+        }
+    }
+}
+
+// The filled tiles of a forked row's last page, in every layer and head: grid (layers x heads, pairs).
+__global__ void __launch_bounds__(256) fork_copy_kernel(unsigned char* pool, const int* moves, int kv_heads, long long layer_bytes,
+                                                        int head_bytes, int tile_bytes)
+{
+    const int* m = moves + 4 * blockIdx.y;
+    if (m[0] < 0) return;
+    const int layer = blockIdx.x / kv_heads, head = blockIdx.x % kv_heads;
+    unsigned char* base = pool + layer * layer_bytes;
+    const uint4* from = reinterpret_cast<const uint4*>(base + ((long long)m[0] * kv_heads + head) * head_bytes);
+    uint4* to = reinterpret_cast<uint4*>(base + ((long long)m[1] * kv_heads + head) * head_bytes);
+    const int n = m[2] * tile_bytes / 16;
+    for (int i = threadIdx.x; i < n; i += 256) to[i] = from[i];
+}
+
+// moves[0] = how many; then pairs (from, to); to_id [pages] = where a page's contents are afterwards
+__global__ void __launch_bounds__(kPageThreads) compact_kernel(int* refs, int pages, int* moves, int* to_id, int* error)
+{
+    __shared__ int warp_s[32];
+    const int free = count_free(refs, pages, warp_s), used = pages - free;
+    int base = 0, total;
+    for (int p0 = 0; p0 < pages; p0 += kPageThreads) {
+        const int p = p0 + threadIdx.x;
+        if (p < pages) {
+            to_id[p] = p;
+            if (refs[p] < 0) atomicExch(error, kErrRow);
+        }
+    }
+    deal_free(refs, pages, free, warp_s, [&](int k, int p) { if (p < used) moves[2 + 2 * k + 1] = p; });
+    for (int p0 = used / kPageThreads * kPageThreads; p0 < pages; p0 += kPageThreads) {
+        const int p = p0 + threadIdx.x;
+        const int high = p >= used && p < pages && refs[p] != 0;
+        const int k = base + block_sum(high, warp_s, total) - 1;
+        if (high) moves[2 + 2 * k] = p;
+        base += total;
+    }
+    if (threadIdx.x == 0) moves[0] = base;
+    __syncthreads();
+    for (int k = threadIdx.x; k < base; k += kPageThreads) {
+        const int from = moves[2 + 2 * k], to = moves[2 + 2 * k + 1];
+        refs[to] = refs[from];
+        refs[from] = 0;
+        to_id[from] = to;
+    }
+}
+
+// Moves the pages (all layers) and renames them in the table.  Sources and destinations are different pages.
+__global__ void __launch_bounds__(256) compact_copy_kernel(unsigned char* pool, int* table, const int* moves, const int* to_id, int layers,
+                                                           int pages, long long entries, long long layer_bytes, long long page_bytes)
+{
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < entries; i += (long long)gridDim.x * 256) {
+        const int p = table[i];
+        if ((unsigned)p < (unsigned)pages) table[i] = to_id[p];
+    }
+    const long long jobs = (long long)moves[0] * layers;
+    constexpr int kChunk = 16384;                                               // bytes a block copies at a time
+    const long long per = (page_bytes + kChunk - 1) / kChunk;
+    for (long long j = blockIdx.x; j < jobs * per; j += gridDim.x) {
+        const long long job = j / per, at = (j % per) * kChunk;
+        const int k = (int)(job / layers), layer = (int)(job % layers);
+        unsigned char* base = pool + layer * layer_bytes + at;
+        const uint4* from = reinterpret_cast<const uint4*>(base + moves[2 + 2 * k] * page_bytes);
+        uint4* to = reinterpret_cast<uint4*>(base + moves[2 + 2 * k + 1] * page_bytes);
+        const int n = (int)((page_bytes - at < kChunk ? page_bytes - at : kChunk) / 16);
+        for (int i = threadIdx.x; i < n; i += 256) to[i] = from[i];
+    }
+}
+
+int last_launch(unsigned n = 1)
+{
+    count_launch(n);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? W4A16_OK : record_cuda_error(e);
+}
+
+}  // namespace
+}  // namespace kv4
+}  // namespace w4a16
+
+using namespace w4a16;
+using namespace w4a16::kv4;
+
+extern "C" size_t w4a16_kv4_tile_bytes(int head_dim, int group)
+{
+    if ((head_dim != 64 && head_dim != 128) || (group != 32 && group != 64 && group != 128) || group > head_dim) return 0;
+    return (size_t)tile_bytes(head_dim, group);
+}
+
+extern "C" int w4a16_kv4_append(const void* qkv, void* pool, const void* table, const void* pos, const void* counts, const void* rope_cos,
+                                const void* rope_sin, int batch, int seq, int heads, int kv_heads, int head_dim, int group, int page_size,
+                                int pages, int width, long long qkv_stride, int rope_rows, void* stream)
+{
+    AppendArgs a;
+    if (!qkv || !pos || ((rope_cos == nullptr) != (rope_sin == nullptr))) return W4A16_ERR_NULL_POINTER;
+    int s = check_cache(a.c, pool, table, pages, width, page_size, kv_heads, head_dim, group);
+    if (s != W4A16_OK) return s;
+    if (batch < 0 || seq < 0 || heads <= 0 || heads % kv_heads || qkv_stride < (heads + 2ll * kv_heads) * head_dim || (qkv_stride % 8) ||
+        (rope_cos && rope_rows <= 0))
+        return W4A16_ERR_BAD_SHAPE;
+    if (((uintptr_t)qkv | (uintptr_t)rope_cos | (uintptr_t)rope_sin) & 15 || ((uintptr_t)pos | (uintptr_t)counts) & 3) return W4A16_ERR_MISALIGNED;
+    if ((heads + 2ll * kv_heads) * head_dim >= (1ll << 30) || seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
+    a.units = (long long)batch * seq * kv_heads;
+    if (a.units == 0) return W4A16_OK;
+    const long long blocks = (a.units * 2 * (head_dim / 8) + 255) / 256;
+    if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
+    a.qkv = (const __half*)qkv; a.pos = (const int*)pos; a.counts = (const int*)counts;
+    a.cos = (const __half*)rope_cos; a.sin = (const __half*)rope_sin;
+    a.seq = seq; a.rope_rows = rope_rows; a.stride = qkv_stride;
+    a.key_at = heads * head_dim; a.val_at = (heads + kv_heads) * head_dim;
+    a.error = device_error_word();
+    if (!a.error) return W4A16_ERR_CUDA;
+    return with_format(head_dim, group, [&](auto f) {
+        using F = decltype(f);
+        append_kernel<F, F::NW * 8><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+        return last_launch();
+    });
+}
+
+extern "C" int w4a16_kv4_read(const void* pool, const void* table, const void* pos, const void* counts, void* k, void* v, int batch, int seq,
+                              int kv_heads, int head_dim, int group, int page_size, int pages, int width, void* stream)
+{
+    ReadArgs a;
+    if (!pos || !k || !v) return W4A16_ERR_NULL_POINTER;
+    int s = check_cache(a.c, pool, table, pages, width, page_size, kv_heads, head_dim, group);
+    if (s != W4A16_OK) return s;
+    if (batch < 0 || seq < 0) return W4A16_ERR_BAD_SHAPE;
+    if (((uintptr_t)k | (uintptr_t)v) & 15 || ((uintptr_t)pos | (uintptr_t)counts) & 3) return W4A16_ERR_MISALIGNED;
+    if (seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
+    a.units = (long long)batch * seq * kv_heads;
+    if (a.units == 0) return W4A16_OK;
+    const long long blocks = (a.units * 2 * (head_dim / 8) + 255) / 256;
+    if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
+    a.pos = (const int*)pos; a.counts = (const int*)counts; a.k = (__half*)k; a.v = (__half*)v; a.seq = seq;
+    a.error = device_error_word();
+    if (!a.error) return W4A16_ERR_CUDA;
+    return with_format(head_dim, group, [&](auto f) {
+        using F = decltype(f);
+        read_kernel<F, F::NW * 8><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+        return last_launch();
+    });
+}
+
+namespace {
+int check_pages(const void* table, const void* refs, int rows, int width, int pages, int page_size)
+{
+    if (!table || !refs) return W4A16_ERR_NULL_POINTER;
+    if (rows <= 0 || width <= 0 || pages <= 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return W4A16_ERR_BAD_SHAPE;
+    if ((long long)width * page_size >= (1ll << 30)) return W4A16_ERR_TOO_LARGE;
+    if (((uintptr_t)table | (uintptr_t)refs) & 3) return W4A16_ERR_MISALIGNED;
+    return W4A16_OK;
+}
+int log2_of(int v)
+{
+    int s = 0;
+    while ((1 << s) < v) ++s;
+    return s;
+}
+}  // namespace
+
+extern "C" int w4a16_kv4_reserve(void* table, void* lens, void* refs, const void* counts, void* pos, int rows, int width, int pages,
+                                 int page_size, void* stream)
+{
+    int s = check_pages(table, refs, rows, width, pages, page_size);
+    if (s != W4A16_OK) return s;
+    if (!lens || !counts || !pos) return W4A16_ERR_NULL_POINTER;
+    if (((uintptr_t)lens | (uintptr_t)counts | (uintptr_t)pos) & 3) return W4A16_ERR_MISALIGNED;
+    if (rows > kMaxRows) return W4A16_ERR_TOO_LARGE;
+    int* err = device_error_word();
+    if (!err) return W4A16_ERR_CUDA;
+    reserve_kernel<<<1, kPageThreads, rows * sizeof(int), (cudaStream_t)stream>>>((int*)table, (int*)lens, (int*)refs, (const int*)counts,
+                                                                                (int*)pos, rows, width, pages, log2_of(page_size), err);
+    return last_launch();
+}
+
+extern "C" int w4a16_kv4_free(void* table, void* lens, void* refs, const void* which, int n, int rows, int width, int pages, void* stream)
+{
+    int s = check_pages(table, refs, rows, width, pages, 16);
+    if (s != W4A16_OK) return s;
+    if (!lens || (n > 0 && !which)) return W4A16_ERR_NULL_POINTER;
+    if (n < 0) return W4A16_ERR_BAD_SHAPE;
+    if (((uintptr_t)lens | (uintptr_t)which) & 3) return W4A16_ERR_MISALIGNED;
+    if (n == 0) return W4A16_OK;
+    int* err = device_error_word();
+    if (!err) return W4A16_ERR_CUDA;
+    free_kernel<<<n, 256, 0, (cudaStream_t)stream>>>((int*)table, (int*)lens, (int*)refs, (const int*)which, rows, width, pages, err);
+    return last_launch();
+}
+
+extern "C" size_t w4a16_kv4_fork_workspace(int n, int rows) { return n <= 0 || rows <= 0 ? 0 : ((size_t)4 * n + rows) * sizeof(int); }
+
+extern "C" int w4a16_kv4_fork(void* pool, void* table, void* lens, void* refs, const void* src, const void* dst, void* workspace,
+                              size_t workspace_bytes, int n, int rows, int width, int layers, int pages, int kv_heads, int head_dim, int group,
+                              int page_size, void* stream)
+{
+    if (!lens || (n > 0 && (!src || !dst)) || !refs) return W4A16_ERR_NULL_POINTER;
+    Cache c;
+    int s = check_cache(c, pool, table, pages, width, page_size, kv_heads, head_dim, group);
+    if (s != W4A16_OK) return s;
+    if (n < 0 || rows <= 0 || layers <= 0) return W4A16_ERR_BAD_SHAPE;
+    if (((uintptr_t)lens | (uintptr_t)refs | (uintptr_t)src | (uintptr_t)dst | (uintptr_t)workspace) & 3) return W4A16_ERR_MISALIGNED;
+    if (n > kMaxRows || (long long)layers * kv_heads >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
+    if (n == 0) return W4A16_OK;
+    if (!workspace || workspace_bytes < w4a16_kv4_fork_workspace(n, rows)) return W4A16_ERR_WORKSPACE;
+    ForkArgs a;
+    a.table = (int*)table; a.lens = (int*)lens; a.refs = (int*)refs; a.src = (const int*)src; a.dst = (const int*)dst;
+    a.moves = (int*)workspace; a.mark = a.moves + 4 * n;
+    a.error = device_error_word();
+    if (!a.error) return W4A16_ERR_CUDA;
+    a.n = n; a.rows = rows; a.width = width; a.pages = pages; a.page_shift = c.page_shift;
+    fork_kernel<<<1, kPageThreads, n * sizeof(int), (cudaStream_t)stream>>>(a);
+    const int T = tile_bytes(head_dim, group), head_bytes = T * (page_size / 16);
+    fork_copy_kernel<<<dim3((unsigned)(layers * kv_heads), (unsigned)n), 256, 0, (cudaStream_t)stream>>>(
+        (unsigned char*)pool, a.moves, kv_heads, (long long)pages * kv_heads * head_bytes, head_bytes, T);
+    return last_launch(2);
+}
+
+extern "C" size_t w4a16_kv4_compact_workspace(int pages) { return pages <= 0 ? 0 : ((size_t)3 * pages + 2) * sizeof(int); }
+
+extern "C" int w4a16_kv4_compact(void* pool, void* table, void* refs, void* workspace, size_t workspace_bytes, int rows, int width, int layers,
+                                 int pages, int kv_heads, int head_dim, int group, int page_size, void* stream)
+{
+    if (!refs) return W4A16_ERR_NULL_POINTER;
+    Cache c;
+    int s = check_cache(c, pool, table, pages, width, page_size, kv_heads, head_dim, group);
+    if (s != W4A16_OK) return s;
+    if (rows <= 0 || layers <= 0) return W4A16_ERR_BAD_SHAPE;
+    if (((uintptr_t)refs | (uintptr_t)workspace) & 3) return W4A16_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < w4a16_kv4_compact_workspace(pages)) return W4A16_ERR_WORKSPACE;
+    int* err = device_error_word();
+    if (!err) return W4A16_ERR_CUDA;
+    int* moves = (int*)workspace;
+    int* to_id = moves + 2 + 2 * (size_t)pages;
+    compact_kernel<<<1, kPageThreads, 0, (cudaStream_t)stream>>>((int*)refs, pages, moves, to_id, err);
+    const long long page_bytes = (long long)kv_heads * tile_bytes(head_dim, group) * (page_size / 16);
+    compact_copy_kernel<<<(unsigned)(device_sm_count() * 8), 256, 0, (cudaStream_t)stream>>>(
+        (unsigned char*)pool, (int*)table, moves, to_id, layers, pages, (long long)rows * width, pages * page_bytes, page_bytes);
+    return last_launch(2);
+}

@@ -22,6 +22,8 @@ import torch
 __all__ = [
     "gemm_awq_ut", "transpose_merge_zeros_scales", "convert_ours_to_awq", "convert_awq_to_lmdeploy",
     "dequant", "quantize_pack", "gemm_awq_bias", "library_path", "load_library", "launch_count",
+    "kv4_pool", "kv4_append", "kv4_read", "kv4_decode_attention", "kv4_attention",
+    "kv4_reserve", "kv4_fork", "kv4_free", "kv4_compact",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -85,6 +87,17 @@ C_ABI = {
     "w4a16_device_error_clear": (_ci, []),
     "w4a16_exchange_reset": (_ci, [_vp]),
     "w4a16_tune_exchange_wait": (None, [ctypes.c_uint]),
+    "w4a16_kv4_tile_bytes": (_sz, [_ci, _ci]),
+    "w4a16_kv4_append": (_ci, [_vp] * 7 + [_ci] * 9 + [ctypes.c_longlong, _ci, _vp]),
+    "w4a16_kv4_read": (_ci, [_vp] * 6 + [_ci] * 8 + [_vp]),
+    "w4a16_kv4_decode_attention": (_ci, [_vp] * 7 + [_ci] * 8 + [ctypes.c_longlong, _ci, ctypes.c_float, _vp]),
+    "w4a16_kv4_attention": (_ci, [_vp] * 8 + [_ci] * 9 + [ctypes.c_longlong, _ci, ctypes.c_float, _vp]),
+    "w4a16_kv4_reserve": (_ci, [_vp] * 5 + [_ci] * 4 + [_vp]),
+    "w4a16_kv4_free": (_ci, [_vp] * 4 + [_ci] * 4 + [_vp]),
+    "w4a16_kv4_fork_workspace": (_sz, [_ci, _ci]),
+    "w4a16_kv4_fork": (_ci, [_vp] * 7 + [_sz] + [_ci] * 9 + [_vp]),
+    "w4a16_kv4_compact_workspace": (_sz, [_ci]),
+    "w4a16_kv4_compact": (_ci, [_vp] * 4 + [_sz] + [_ci] * 8 + [_vp]),
 }
 
 
@@ -540,3 +553,7 @@ def dequant(W, W_zeros_scales, N: int, K: int, group_size: int):
                                           int(group_size), _stream(W))
     _check(st, "dequant")
     return out
+
+
+from .kv4 import (kv4_append, kv4_attention, kv4_compact, kv4_decode_attention, kv4_fork, kv4_free, kv4_pool,  # noqa: E402
+                  kv4_read, kv4_reserve)

@@ -1,0 +1,253 @@
+"""The paged 4-bit key/value cache of `quant`: quantise-and-append, attention, and the operations on its pages.
+
+A pool is uint8 [layers, pages, kv_heads, page_size / 16, tile bytes] (kv4_pool); the calls on one layer take `pool[layer]`.  A table
+is int32 [rows, width] of page numbers (-1: none), refs int32 [pages] the number of rows that hold each page, lens int32 [rows] the
+tokens of each row.  All of them live on the device and are updated in place, so that a captured token step can be replayed.
+Format, limits and the device error word's values: include/w4a16_b200.h.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _check, _check_tensor, _need, _stream, load_library
+
+# tile bytes -> (head_dim, group): 16 head_dim + 128 head_dim / group are different for all formats
+_FORMATS = {16 * d + 128 * d // g: (d, g) for d in (64, 128) for g in (32, 64, 128) if g <= d}
+
+
+def kv4_pool(layers: int, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, group: int = 64, device="cuda"):
+    """A zeroed pool for `pages` pages of `page_size` tokens in each of `layers` layers."""
+    layers, pages, kv_heads, page_size = int(layers), int(pages), int(kv_heads), int(page_size)
+    tile = 16 * int(head_dim) + 128 * int(head_dim) // max(int(group), 1)
+    _need(int(group) in (32, 64, 128), "unsupported group size")
+    _need(_FORMATS.get(tile) == (int(head_dim), int(group)), "head_dim must be 64 or 128, group at most head_dim")
+    _need(16 <= page_size <= 1024 and page_size & (page_size - 1) == 0, "page_size must be a power of two from 16 to 1024")
+    _need(layers > 0 and pages > 0 and kv_heads > 0, "layers, pages and kv_heads must be positive")
+    return torch.zeros((layers, pages, kv_heads, page_size // 16, tile), dtype=torch.uint8, device=device)
+
+
+def _ints(t, name, device, dims=1, numel=None):
+    _check_tensor(t, name, dtype=torch.int32, dims=dims)
+    _need(t.get_device() == device, "all tensors must be on the same device")
+    _need(numel is None or t.numel() == numel, f"Tensor {name} must have {numel} elements")
+
+
+def _pool_shape(pool, layers=False):
+    """(pages, kv_heads, page_size, head_dim, group) of a layer's pool, or of a whole one with the layers in front."""
+    _check_tensor(pool, "pool", dtype=torch.uint8, dims=5 if layers else 4)
+    shape = tuple(pool.shape)
+    fmt = _FORMATS.get(shape[-1])
+    _need(fmt is not None, "pool must be [pages, kv_heads, page_size / 16, tile bytes] of a kv4 format")
+    pages, kv, per = shape[-4:-1]
+    _need(pages > 0 and kv > 0 and per > 0, "pool must not be empty")
+    out = (pages, kv, 16 * per, *fmt)
+    return (shape[0], *out) if layers else out
+
+
+def _rope_args(rope, D, device):
+    if rope is None:
+        return None, None, 0
+    cos, sin = rope
+    _check_tensor(cos, "rope cos", dtype=torch.float16, dims=2)
+    _check_tensor(sin, "rope sin", dtype=torch.float16, dims=2)
+    _need(cos.shape[1] == D and sin.shape == cos.shape and cos.get_device() == sin.get_device() == device,
+          "rope tables must be [positions, head_dim] on the same device")
+    return cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+
+
+class _on:
+    """The device guard of a call, where the tensors are not on the current device."""
+
+    def __init__(self, device):
+        self.guard = None if torch.cuda.current_device() == device else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def kv4_append(qkv, pool, table, pos, heads: int, rope=None, counts=None):
+    """Keys and values of qkv fp16 [B, S, >= (heads + 2 kv_heads) * head_dim] into the pages of positions pos[b] ..: quantised to 4
+    bits, keys rotated by `rope` = (cos, sin) fp16 [positions, head_dim] first.  pool: one layer's [pages, kv_heads, page_size / 16,
+    tile bytes], updated in place; table int32 [B, width]; pos int32 [B], negative for a batch row without a sequence; counts int32 [B]
+    tokens a row has of the S (None: all)."""
+    _check_tensor(qkv, "qkv", dtype=torch.float16, dims=3)
+    pages, kv, page, D, g = _pool_shape(pool)
+    dev, (B, S, N), heads = qkv.get_device(), qkv.shape, int(heads)
+    _need(pool.get_device() == dev, "all tensors must be on the same device")
+    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
+    _need(N >= (heads + 2 * kv) * D, "qkv must be [B, S, >= (heads + 2 kv_heads) * head_dim]")
+    _ints(table, "table", dev, 2)
+    _need(table.shape[0] == B, "table must have a row for every batch row")
+    _ints(pos, "pos", dev, numel=B)
+    if counts is not None:
+        _ints(counts, "counts", dev, numel=B)
+    cos, sin, rope_rows = _rope_args(rope, D, dev)
+    if B == 0 or S == 0:
+        return
+    lib = load_library()
+    with _on(dev):
+        st = lib.w4a16_kv4_append(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
+                                  None if counts is None else counts.data_ptr(), cos, sin, B, S, heads, kv, D, g, page, pages,
+                                  table.shape[1], N, rope_rows, _stream(qkv))
+    _check(st, "kv4_append")
+
+
+def kv4_read(pool, table, pos, count: int, counts=None):
+    """(k, v) fp16 [B, kv_heads, count, head_dim]: what the cache holds for positions pos[b] .. pos[b] + count - 1 (counts int32 [B]: only
+    that many of them), zeros where the row has no sequence (pos < 0)."""
+    pages, kv, page, D, g = _pool_shape(pool)
+    dev, count = pool.get_device(), int(count)
+    _ints(table, "table", dev, 2)
+    B = table.shape[0]
+    _ints(pos, "pos", dev, numel=B)
+    if counts is not None:
+        _ints(counts, "counts", dev, numel=B)
+    _need(count >= 0, "count must not be negative")
+    k = torch.empty((B, kv, count, D), dtype=torch.float16, device=pool.device)
+    v = torch.empty_like(k)
+    if B == 0 or count == 0:
+        return k, v
+    lib = load_library()
+    with _on(dev):
+        st = lib.w4a16_kv4_read(pool.data_ptr(), table.data_ptr(), pos.data_ptr(), None if counts is None else counts.data_ptr(),
+                                k.data_ptr(), v.data_ptr(), B, count, kv, D, g, page, pages, table.shape[1], _stream(pool))
+    _check(st, "kv4_read")
+    return k, v
+
+
+def kv4_decode_attention(qkv, pool, table, pos, heads: int, rope=None, scale=None, out=None):
+    """One token step: the new token of every row (qkv fp16 [B, >= (heads + 2 kv_heads) * head_dim], position pos[b]) is appended to the
+    4-bit cache and attends to positions 0 .. pos[b].  Returns fp16 [B, heads * head_dim]; rows with pos < 0 keep what `out` held
+    (without `out`: zeros).  Other arguments as for kv4_append; scale defaults to head_dim ** -0.5."""
+    _check_tensor(qkv, "qkv", dtype=torch.float16, dims=2)
+    pages, kv, page, D, g = _pool_shape(pool)
+    dev, (B, N), heads = qkv.get_device(), qkv.shape, int(heads)
+    _need(pool.get_device() == dev, "all tensors must be on the same device")
+    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
+    _need(N >= (heads + 2 * kv) * D, "qkv must be [B, >= (heads + 2 kv_heads) * head_dim]")
+    _ints(table, "table", dev, 2)
+    _need(table.shape[0] == B, "table must have a row for every batch row")
+    _ints(pos, "pos", dev, numel=B)
+    cos, sin, rope_rows = _rope_args(rope, D, dev)
+    out = _output(out, (B, heads * D), qkv)
+    if B == 0:
+        return out
+    lib = load_library()
+    with _on(dev):
+        st = lib.w4a16_kv4_decode_attention(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(), cos, sin, out.data_ptr(),
+                                            B, heads, kv, D, g, page, pages, table.shape[1], N, rope_rows,
+                                            float(D ** -0.5 if scale is None else scale), _stream(qkv))
+    _check(st, "kv4_decode_attention")
+    return out
+
+
+def _output(out, shape, like):
+    if out is None:
+        return torch.zeros(shape, dtype=torch.float16, device=like.device)
+    _check_tensor(out, "out", dtype=torch.float16)
+    _need(tuple(out.shape) == shape and out.device == like.device, f"Tensor out must have shape {list(shape)}")
+    return out
+
+
+def kv4_attention(qkv, pool, table, pos, heads: int, rope=None, scale=None, counts=None, out=None):
+    """Causal attention of a chunk of queries over the 4-bit cache, which already holds their own keys and values (kv4_append): query i
+    of row b stands at position pos[b] + i and attends to positions 0 .. pos[b] + i.  qkv fp16 [B, S, >= heads * head_dim], queries in
+    front.  Returns fp16 [B, S, heads * head_dim]; queries past counts[b] and rows with pos < 0 keep what `out` held (without `out`:
+    zeros)."""
+    _check_tensor(qkv, "qkv", dtype=torch.float16, dims=3)
+    pages, kv, page, D, g = _pool_shape(pool)
+    dev, (B, S, N), heads = qkv.get_device(), qkv.shape, int(heads)
+    _need(pool.get_device() == dev, "all tensors must be on the same device")
+    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
+    _need(N >= heads * D, "qkv must be [B, S, >= heads * head_dim]")
+    _ints(table, "table", dev, 2)
+    _need(table.shape[0] == B, "table must have a row for every batch row")
+    _ints(pos, "pos", dev, numel=B)
+    if counts is not None:
+        _ints(counts, "counts", dev, numel=B)
+    cos, sin, rope_rows = _rope_args(rope, D, dev)
+    out = _output(out, (B, S, heads * D), qkv)
+    if B == 0 or S == 0:
+        return out
+    lib = load_library()
+    with _on(dev):
+        st = lib.w4a16_kv4_attention(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
+                                     None if counts is None else counts.data_ptr(), cos, sin, out.data_ptr(), B, S, heads, kv, D, g, page,
+                                     pages, table.shape[1], N, rope_rows, float(D ** -0.5 if scale is None else scale), _stream(qkv))
+    _check(st, "kv4_attention")
+    return out
+
+
+def _bookkeeping(table, refs, lens):
+    _check_tensor(table, "table", dtype=torch.int32, dims=2)
+    dev = table.get_device()
+    _need(table.numel() > 0, "table must not be empty")
+    _ints(refs, "refs", dev)
+    if lens is not None:
+        _ints(lens, "lens", dev, numel=table.shape[0])
+    return dev
+
+
+def kv4_reserve(table, lens, refs, counts, page_size: int):
+    """Room for counts[r] (int32 [rows]) more tokens of every row: lens grow by them and the table gets the pages they need, lowest free
+    numbers first.  Returns pos int32 [rows]: where the new tokens start, -1 for rows that asked for none or could not be served."""
+    dev = _bookkeeping(table, refs, lens)
+    rows, width = table.shape
+    _ints(counts, "counts", dev, numel=rows)
+    pos = torch.empty_like(lens)
+    lib = load_library()
+    with _on(dev):
+        st = lib.w4a16_kv4_reserve(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), counts.data_ptr(), pos.data_ptr(), rows, width,
+                                   refs.numel(), int(page_size), _stream(table))
+    _check(st, "kv4_reserve")
+    return pos
+
+
+def kv4_free(table, lens, refs, rows):
+    """The rows (int32 [n]) give their pages back and are empty afterwards."""
+    dev = _bookkeeping(table, refs, lens)
+    _ints(rows, "rows", dev)
+    lib = load_library()
+    with _on(dev):
+        st = lib.w4a16_kv4_free(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), rows.data_ptr(), rows.numel(), table.shape[0],
+                                table.shape[1], refs.numel(), _stream(table))
+    _check(st, "kv4_free")
+
+
+def kv4_fork(pool, table, lens, refs, src, dst):
+    """Row dst[i] (empty) continues row src[i] (int32 [n] both): whole pages are shared, the last, partly filled one is copied in every
+    layer.  pool: the whole [layers, pages, kv_heads, page_size / 16, tile bytes]."""
+    layers, pages, kv, page, D, g = _pool_shape(pool, layers=True)
+    dev = _bookkeeping(table, refs, lens)
+    _need(pool.get_device() == dev and layers > 0, "all tensors must be on the same device")
+    _need(refs.numel() == pages, "refs must have an element for every page of the pool")
+    _ints(src, "src", dev)
+    _ints(dst, "dst", dev, numel=src.numel())
+    lib = load_library()
+    n, (rows, width) = src.numel(), table.shape
+    if n == 0:
+        return
+    ws = torch.empty(lib.w4a16_kv4_fork_workspace(n, rows), dtype=torch.uint8, device=pool.device)
+    with _on(dev):
+        st = lib.w4a16_kv4_fork(pool.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(),
+                                ws.data_ptr(), ws.numel(), n, rows, width, layers, pages, kv, D, g, page, _stream(pool))
+    _check(st, "kv4_fork")
+
+
+def kv4_compact(pool, table, refs):
+    """The pages in use become the pool's first ones (their contents move in every layer, table and refs follow)."""
+    layers, pages, kv, page, D, g = _pool_shape(pool, layers=True)
+    dev = _bookkeeping(table, refs, None)
+    _need(pool.get_device() == dev and layers > 0, "all tensors must be on the same device")
+    _need(refs.numel() == pages, "refs must have an element for every page of the pool")
+    lib = load_library()
+    ws = torch.empty(lib.w4a16_kv4_compact_workspace(pages), dtype=torch.uint8, device=pool.device)
+    with _on(dev):
+        st = lib.w4a16_kv4_compact(pool.data_ptr(), table.data_ptr(), refs.data_ptr(), ws.data_ptr(), ws.numel(), table.shape[0],
+                                   table.shape[1], layers, pages, kv, D, g, page, _stream(pool))
+    _check(st, "kv4_compact")
