@@ -137,18 +137,3 @@ extern "C" int w4a16_kv4_attention(const void* qkv, const void* pool, const void
     if (batch == 0 || seq == 0) return W4A16_OK;
     return launch_simple(a, batch, head_dim, group, (cudaStream_t)stream);
 }
-
-extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const void* table, const void* pos, const void* rope_cos,
-                                          const void* rope_sin, void* out, int batch, int heads, int kv_heads, int head_dim, int group,
-                                          int page_size, int pages, int width, long long qkv_stride, int rope_rows, float scale, void* stream)
-{
-    AttnArgs a;
-    int s = check_attention(a, qkv, pool, table, pos, nullptr, rope_cos, rope_sin, out, batch, 1, heads, kv_heads, head_dim, group, page_size,
-                            pages, width, qkv_stride, rope_rows, scale, (heads + 2ll * kv_heads) * head_dim);
-    if (s != W4A16_OK) return s;
-    if (batch == 0) return W4A16_OK;
-    s = w4a16_kv4_append(qkv, pool, table, pos, nullptr, rope_cos, rope_sin, batch, 1, heads, kv_heads, head_dim, group, page_size, pages,
-                         width, qkv_stride, rope_rows, stream);
-    if (s != W4A16_OK) return s;
-    return launch_simple(a, batch, head_dim, group, (cudaStream_t)stream);
-}

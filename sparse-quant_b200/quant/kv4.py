@@ -139,8 +139,10 @@ def kv4_decode_attention(qkv, pool, table, pos, heads: int, rope=None, scale=Non
         return out
     lib = load_library()
     with _on(dev):
+        ws_bytes = lib.w4a16_kv4_decode_workspace(B, heads, kv, D, page, table.shape[1])
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device) if ws_bytes else None
         st = lib.w4a16_kv4_decode_attention(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(), cos, sin, out.data_ptr(),
-                                            B, heads, kv, D, g, page, pages, table.shape[1], N, rope_rows,
+                                            None if ws is None else ws.data_ptr(), ws_bytes, B, heads, kv, D, g, page, pages, table.shape[1], N, rope_rows,
                                             float(D ** -0.5 if scale is None else scale), _stream(qkv))
     _check(st, "kv4_decode_attention")
     return out

@@ -184,6 +184,59 @@ def test_decode_attention(D, G, heads, kv):
                 assert (np.abs(got[b, h] - ref) <= tol).all(), (b, h, float(np.abs(got[b, h] - ref).max()), float(tol.max()))
 
 
+@pytest.mark.parametrize("splits", [1, 2, 4, 8, 9, 37])
+def test_decode_attention_split_over_ctas(splits):
+    """A row's tiles split over a cluster or over the grid, also over more CTAs than it has tiles."""
+    import quant
+    lib = quant.load_library()
+    try:
+        lib.w4a16_tune_kv4(splits)
+        for D, G, heads, kv, lens in ((128, 64, 4, 2, [0, 15, 16, 129, 700]), (64, 32, 20, 2, [333, 0, 1]), (128, 128, 1, 1, [1100])):
+            c = Case(lens, kv, heads, D, G, 32, seed=splits, rope=True, dead=(1,) if len(lens) == 3 else ())
+            d = c.device()
+            for again in range(2):
+                out = quant.kv4_decode_attention(d["qkv"][:, 0], d["pool"], d["table"], d["pos"], heads, rope=d["rope"])
+                if not again:
+                    c.append()
+                assert np.array_equal(_bytes(d["pool"]), c.pages.pool)
+                got = out.double().cpu().numpy().reshape(c.B, heads, D)
+                for b in range(c.B):
+                    for h in range(heads):
+                        if c.lens[b] < 0:
+                            assert not got[b, h].any()
+                            continue
+                        ref, tol = c.attend(b, 0, h, chunk=False)
+                        assert (np.abs(got[b, h] - ref) <= tol).all(), (b, h, float(np.abs(got[b, h] - ref).max()), float(tol.max()))
+    finally:
+        lib.w4a16_tune_kv4(0)
+
+
+def test_decode_attention_keeps_nan():
+    """A query, a key or a value that is not finite makes the outputs NaN that depend on it, and no others."""
+    import quant
+    for what in ("q", "k", "v", "old"):
+        c = Case([37, 50], 2, 4, 128, 64, 16, seed=2)
+        x, D = c.qkv, 128
+        if what == "old":
+            for h in range(2):
+                c.pages.store(0, h, 5, np.ones(D, np.float16), np.where(np.arange(D) == 70, np.inf, 1).astype(np.float16))
+        else:
+            at = {"q": 1, "k": 4, "v": 6}[what] * D                     # query head 1, key head 0, value head 0
+            x[0, 0, at + 3] = float("nan") if what != "v" else float("inf")
+        d = c.device()
+        got = quant.kv4_decode_attention(d["qkv"][:, 0], d["pool"], d["table"], d["pos"], 4).view(2, 4, D).isnan().cpu()
+        want = torch.zeros_like(got)
+        if what == "q":
+            want[0, 1] = True
+        elif what == "k":
+            want[0, :2] = True
+        elif what == "v":
+            want[0, :2, :64] = True                                     # the group of dims that the infinity stands in
+        else:
+            want[0, :, 64:] = True
+        assert torch.equal(got, want), what
+
+
 def test_decode_attention_leaves_rows_without_a_sequence():
     import quant
     c = Case([40, 3, 7], 2, 4, 64, 32, 16, dead=(1,))

@@ -36,9 +36,9 @@ def test_status_codes_of_cache_calls():
     def read(pool=p, table=p, pos=p, k=p, v=p, batch=1, seq=1, kv=2, D=128, g=64, page=16, pages=4, width=2):
         return lib.w4a16_kv4_read(pool, table, pos, None, k, v, batch, seq, kv, D, g, page, pages, width, None)
 
-    def decode(qkv=p, pool=p, table=p, pos=p, cos=None, sin=None, out=p, batch=1, heads=4, kv=2, D=128, g=64, page=16, pages=4, width=2,
+    def decode(qkv=p, pool=p, table=p, pos=p, cos=None, sin=None, out=p, ws=None, ws_bytes=0, batch=1, heads=4, kv=2, D=128, g=64, page=16, pages=4, width=2,
                stride=8 * 128, rope_rows=0):
-        return lib.w4a16_kv4_decode_attention(qkv, pool, table, pos, cos, sin, out, batch, heads, kv, D, g, page, pages, width, stride,
+        return lib.w4a16_kv4_decode_attention(qkv, pool, table, pos, cos, sin, out, ws, ws_bytes, batch, heads, kv, D, g, page, pages, width, stride,
                                               rope_rows, 0.1, None)
 
     def chunk(qkv=p, pool=p, table=p, pos=p, cos=None, sin=None, out=p, batch=1, seq=1, heads=4, kv=2, D=128, g=64, page=16, pages=4,
@@ -61,6 +61,10 @@ def test_status_codes_of_cache_calls():
         assert call(batch=0) == 0                                              # nothing to do
     assert read(k=None) == 1 and read(v=p + 2) == 4
     assert decode(out=None) == 1 and chunk(out=p + 2) == 4
+    # one row over a wide table is split over more CTAs than a cluster holds: it needs a workspace
+    need = lib.w4a16_kv4_decode_workspace(1, 4, 2, 128, 16, 10000)
+    assert need > 0 and lib.w4a16_kv4_decode_workspace(64, 32, 32, 128, 16, 10000) == 0
+    assert decode(width=10000) == 5 and decode(width=10000, ws=p, ws_bytes=need - 1) == 5 and decode(width=10000, ws=p + 2, ws_bytes=need) == 4
     assert append(seq=0) == 0 and read(seq=0) == 0 and chunk(seq=0) == 0
     assert append(seq=-1) == 2 and read(seq=-1) == 2 and chunk(seq=-1) == 2
     del keep
