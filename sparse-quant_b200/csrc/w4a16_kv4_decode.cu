@@ -10,28 +10,30 @@
 // (token, group), 2^-11 of it, scaled by a power of two that follows the largest step seen, so that values near fp16's smallest keep
 // their precision.  Scores, maxima, sums and the minima's part of the output are fp32.
 //
-// A warp owns tiles of 16 tokens of one (row, key/value head), with a ring of tiles of its own in shared memory, filled by the copy
-// engine (a tile is one contiguous run, also where pages are small), and a softmax of its own: running maximum and sum, rescaled
-// only when a score exceeds the maximum by 2^8.  Queries that share the key/value head are the 8 columns of mma.m16n8k16:
+// Work is dealt in chunks of 32 tokens of one (row, key/value head, 8 query heads) - a unit.  All units of all rows stand in one line,
+// and every warp of the GPU takes an equal stretch of it (four CTAs of four warps an SM), so that rows of any lengths fill the
+// machine.  A stretch is cut into segments at the ends of units; a segment that is not a whole unit leaves (reference, sum, output) in a
+// workspace, which join_kernel puts together.  Where a CTA's four stretches lie in one unit its warps meet in shared memory first.  Short
+// rows are dealt by units instead, a CTA each, and need no second launch.  A warp streams its chunks through a ring
+// of its own in shared memory (16-byte asynchronous copies; two adjacent tiles are one run, from pages of 32 tokens on), across segments.
+// (Copies by one lane in bulk cost three times the instructions here: the loop is bound by what the warps can issue.)
+//
+// Queries that share the key/value head are the 8 columns of mma.m16n8k16:
 //     scores  A = keys (16 tokens x 16 dims), B = queries;   output  A = values^T (16 dims x 16 tokens), B = weights
-// and the accumulator of the first is the layout the second needs after an 8x8 transpose (movmatrix).  Warps, and the S CTAs that
-// split a row's tiles, meet in shared memory, through the cluster's for S <= 8, or through a workspace and a second launch.
-#include <cooperative_groups.h>
-
+// and the accumulator of the first is the layout the second needs after an 8x8 transpose (movmatrix).  Weights are 2^(score - ref)
+// with ref = maximum + log2 of the largest step, moved only when a score exceeds the maximum by 2^8 or a step the largest by 2^5.
 #include "w4a16_kv4.cuh"
-#include "w4a16_sm100.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace w4a16 {
 namespace kv4 {
 namespace {
 
-using namespace sm100;
-
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kCols = 8;                          // query heads of one pass
-constexpr uint64_t kWaitNs = 400000000ull;        // a copy that has not arrived by then never will: error word 1
+constexpr int kChunk = 2 * kTile;                 // tokens
+constexpr int kStart = 2;                         // what a segment costs besides its chunks (queries, result), in chunks
+constexpr int kLeast = 4;                         // a warp's share of the line at least, in chunks
+constexpr int kSmem4 = 57344;                     // shared memory of a CTA with which four fit an SM
 
 struct DecodeArgs {
     Cache c;
@@ -41,11 +43,13 @@ struct DecodeArgs {
     const __half* cos;
     const __half* sin;
     int* error;
-    float* part;                  // split over the grid: [batch][heads][splits][D + 2]
-    int heads, share;             // share: query heads of a key/value head
-    int blocks;                   // passes of 8 query heads over a key/value head
-    int splits, rope_rows;
-    long long stride;
+    int4* split_units;         // [warps]: (row, unit, warps that have a part of it, 0) of the unit that starts in the warp's stretch and ends behind it
+    float* part;                  // [warps][2][columns][D + 4]: of the unit that starts before the stretch, and of the one that ends behind it
+    int batch, heads, share;      // share: query heads of a key/value head
+    int blocks, units;            // passes of 8 query heads over a key/value head; kv heads * blocks: units of a row
+    int cols;                     // min(8, share)
+    int rope_rows, stages;
+    long long stride, page_bytes;
     float scale_log2;             // scale * log2(e)
 };
 
@@ -67,479 +71,716 @@ __device__ __forceinline__ uint32_t pack2(float a, float b)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }        // -126 <= e <= 127
+__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23) - 127; }     // of a positive normal number
+template <int N>
+__device__ __forceinline__ void load_params(const unsigned char* at, __half2 (&p)[N])
+{
+    if constexpr (N == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(at);
+    else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(at);
+    else p[0] = *reinterpret_cast<const __half2*>(at);
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from)
+{
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // which token of a tile stands in row i (of 8) of a fragment; rows 8 to 15 are the tokens 8 further on.  The order spreads the rows
 // that one load instruction touches over the shared-memory banks, for keys (two or four rows at a time) and values (every other).
 __device__ __forceinline__ int token_of(int i) { return i ^ ((i >> 2) & 1); }
 
+// Chunks of batch row b, 0 where it has no sequence or a position that cannot be served.
+__device__ __forceinline__ int chunks_of(const DecodeArgs& a, int b)
+{
+    const int p = a.pos[b];
+    return p < 0 || p >= a.c.capacity() || (a.cos && p >= a.rope_rows) ? 0 : p / kChunk + 1;
+}
+
+// The line as a warp sees it.  A unit of n chunks is kStart + n long; chunk k stands at kStart + k of it.
+struct Rows {
+    long long v0;                 // lengths of rows 0 .. lane (inclusive sums of the first 32)
+    long long total;              // of all rows
+    int lane;
+    __device__ __forceinline__ long long upto(const DecodeArgs& a, int b0) const        // inclusive sums of rows b0 .. b0 + 31
+    {
+        const int b = b0 + lane, n = b < a.batch ? chunks_of(a, b) : 0;
+        long long v = n ? (long long)(n + kStart) * a.units : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        return v;
+    }
+    __device__ __forceinline__ explicit Rows(const DecodeArgs& a) : lane(threadIdx.x & 31)
+    {
+        v0 = upto(a, 0);
+        total = __shfl_sync(0xffffffffu, v0, 31);
+        for (int b0 = 32; b0 < a.batch; b0 += 32) total += __shfl_sync(0xffffffffu, upto(a, b0), 31);
+    }
+    // the row that place `find` < total of the line belongs to, and what stands before that row
+    __device__ __forceinline__ int row_of(const DecodeArgs& a, long long find, long long& before) const
+    {
+        before = 0;
+        for (int b0 = 0;; b0 += 32) {
+            const long long v = b0 ? upto(a, b0) : v0;
+            const unsigned beyond = __ballot_sync(0xffffffffu, before + v > find);
+            if (beyond) {
+                const int l = __ffs(beyond) - 1;
+                if (l) before += __shfl_sync(0xffffffffu, v, l - 1);
+                return b0 + l;
+            }
+            before += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+};
+
+// A stretch of the line, and the segment of it that is being worked on.
+struct Line {
+    int b, unit;                  // row, key/value head * blocks + pass of query heads
+    int lo, hi, n;                // the segment's chunks of the unit's n; may be none
+    long long left;               // of the stretch, behind the segment
+    __device__ __forceinline__ void take(int from)                                      // `from` of the unit's length on
+    {
+        const long long to = from + left < n + kStart ? from + left : n + kStart;
+        left -= to - from;
+        lo = from > kStart ? from - kStart : 0;
+        hi = to > kStart ? (int)to - kStart : 0;
+    }
+    __device__ __forceinline__ bool next(const DecodeArgs& a)
+    {
+        if (left <= 0) return false;
+        if (++unit == a.units) {
+            unit = 0;
+            do ++b; while ((n = chunks_of(a, b)) == 0);                          // (left > 0: there is one)
+        }
+        take(0);
+        return true;
+    }
+};
+
 template <class F, int D>
-struct Smem {
-    static constexpr int kStages = F::kBytes > 2304 ? 5 : F::kBytes > 1280 ? 6 : 10;      // four CTAs an SM
-    alignas(128) unsigned char ring[kWarps][kStages][F::kBytes];
-    uint64_t full[kWarps][kStages];
-    float m[kWarps + 1][kCols], l[kWarps + 1][kCols];                                      // [kWarps]: of the whole CTA
-    int abort_flag[kWarps];
+struct Layout {                   // shared memory of a warp: ring, then queries
+    static constexpr int kQPitch = F::NW + 4;                                   // words of 16 bytes a query head: rows 64 bytes apart modulo the banks
+    static constexpr int kHead = kQPitch * 16 + (F::NG + 1) * 4 + (16 - (F::NG + 1) * 4 % 16) % 16;
+    static constexpr int kStage = 2 * F::kBytes;
+    static constexpr int kPitch = D + 4;                                        // floats of an output row where warps meet
+    static __host__ __device__ constexpr int warp_bytes(int stages, int cols) { return (stages * kStage + cols * kHead + 63) / 64 * 64; }
 };
 
 template <class F, int D>
 __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
 {
-    constexpr int J = F::J, NG = F::NG, kStages = Smem<F, D>::kStages, kPitch = D + 4;
-    static_assert(sizeof(float) * kCols * kPitch <= sizeof(Smem<F, D>::ring[0]), "a warp's output takes the place of its ring");
+    using L = Layout<F, D>;
+    constexpr int J = F::J, NG = F::NG, kBytes = F::kBytes, kPitch = L::kPitch;
     extern __shared__ __align__(128) unsigned char raw[];
-    Smem<F, D>& sm = *reinterpret_cast<Smem<F, D>*>(raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c4 = lane & 3;
-    const int split = blockIdx.x, kvh = blockIdx.y / a.blocks, hb = blockIdx.y % a.blocks, b = blockIdx.z;
+    unsigned char* ring = raw + warp * L::warp_bytes(a.stages, a.cols);
+    uint4* q_s = reinterpret_cast<uint4*>(ring + a.stages * L::kStage);
+    float* qsum_s = reinterpret_cast<float*>(q_s + a.cols * L::kQPitch);        // [columns][NG], then unit [columns]
+    float* unit_s = qsum_s + a.cols * NG;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (lane < kStages) mbar_init(smem_u32(&sm.full[warp][lane]), 1);
-    if (lane == 0) sm.abort_flag[warp] = 0;
-    mbar_fence_init();
-    __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int pos = a.pos[b];
-    if (pos < 0) return;                                                        // (uniform over the cluster: nobody waits)
-    if (pos >= a.c.capacity() || (a.cos && pos >= a.rope_rows)) {
-        if (threadIdx.x == 0) atomicExch(a.error, kErrPosition);
-        return;
-    }
-    const int tiles = (pos >> 4) + 1;
-    const int lo = (int)((long long)tiles * split / a.splits), hi = (int)((long long)tiles * (split + 1) / a.splits);
-    const int mine = hi - lo > warp ? (hi - lo - warp + kWarps - 1) / kWarps : 0;  // tiles lo + warp, lo + warp + kWarps, ...
 
-    // ---- the ring: page numbers 32 tiles at a time, one batch ahead
-    const int* table = a.c.table + (size_t)b * a.c.width;
-    const int tshift = a.c.page_shift - 4;
-    auto page_of = [&](int i) {
-        const int t = lo + warp + i * kWarps;
-        return t < hi ? table[t >> tshift] : -1;
-    };
-    int ids0 = page_of(lane), ids1 = mine > 32 ? page_of(32 + lane) : -1, batch = 0;
-    auto id_at = [&](int i) { return __shfl_sync(0xffffffffu, (i >> 5) == batch ? ids0 : ids1, i & 31); };
-    auto tile_at = [&](int i, int page) {
-        const int t = lo + warp + i * kWarps;
-        return a.c.pool + ((((size_t)page * a.c.kv_heads + kvh) << tshift) + (t & ((1 << tshift) - 1))) * (size_t)F::kBytes;
-    };
-    auto fetch = [&](int i) {
-        const int page = id_at(i);
-        if (lane == 0 && (unsigned)page < (unsigned)a.c.pages) {
-            const uint32_t bar = smem_u32(&sm.full[warp][i % kStages]);
-            mbar_arrive_expect_tx(bar, F::kBytes);
-            bulk_load(smem_u32(sm.ring[warp][i % kStages]), tile_at(i, page), F::kBytes, bar);
-        } else if (lane == 0) {
-            mbar_arrive(smem_u32(&sm.full[warp][i % kStages]));                 // no page: the phase passes, the tile is left out
+    // ---- this warp's stretch of the line
+    Line line;
+    bool together;                                                              // the CTA's warps work on one unit and meet at its end
+    const long long me = (long long)blockIdx.x * kWarps + warp;
+    int4 split_unit = make_int4(0, 0, 0, 0);                                    // the one that starts in this stretch and ends behind it
+    long long total = 0, warps = 0;
+    if (!a.part) {
+        together = true;
+        line.b = blockIdx.x / a.units;
+        line.unit = blockIdx.x % a.units;
+        line.n = chunks_of(a, line.b);
+        if (line.n == 0) {
+            if (threadIdx.x == 0 && line.unit == 0 && a.pos[line.b] >= 0) atomicExch(a.error, kErrPosition);
+            return;
         }
-    };
-    for (int i = 0; i < kStages && i < mine; ++i) fetch(i);
-
-    // ---- queries: column n = lane / 4, dims 32 j + 8 c .. + 7 (the key word the same lane reads)
-    uint32_t qf[J][4];                                                          // low nibbles' dims (0,4)(2,6), high nibbles' (1,5)(3,7) / 16
-    float qsum[NG][2], unit[2];
-    {
-        const int h = hb * kCols + row;
-        float q[J][8], top = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[j][i] = 0.f;
-            if (h < a.share) load_rotated<D>(a.qkv + b * a.stride + (kvh * a.share + h) * D, 4 * j + c4, a.cos, a.sin, pos, q[j]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[j][i]));
+        line.left = 0;
+        line.lo = line.n * warp / kWarps;
+        line.hi = line.n * (warp + 1) / kWarps;
+    } else {
+        if (blockIdx.x == 0)                                                    // whoever cannot be served is told of once
+            for (int b = threadIdx.x; b < a.batch; b += kThreads)
+                if (a.pos[b] >= 0 && chunks_of(a, b) == 0) atomicExch(a.error, kErrPosition);
+        const Rows rows(a);
+        total = rows.total;
+        warps = min((long long)gridDim.x * kWarps, max((total + kLeast - 1) / kLeast, 1ll));
+        if (me >= warps || total == 0) {
+            if (lane == 0) a.split_units[me] = split_unit;
+            if (me - warp >= warps || total == 0) return;                       // the whole CTA
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // largest element into [2^14, 2^15): then a sixteenth of an element is exact down to 2^-39 of the largest
-        const int e = top > 0.f ? max(14 - ((__float_as_int(top) >> 23) - 127), -2) : 0;      // (-2: infinities)
-        const float up = pow2(e);
-        float sums[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) sums[g] = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[j][i] *= up;
-                sums[32 * j * NG / D] += q[j][i];
-            }
-            qf[j][0] = pack2(q[j][0], q[j][4]);
-            qf[j][1] = pack2(q[j][2], q[j][6]);
-            qf[j][2] = pack2(q[j][1] * 0.0625f, q[j][5] * 0.0625f);
-            qf[j][3] = pack2(q[j][3] * 0.0625f, q[j][7] * 0.0625f);
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
-            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
-            sums[g] *= 5.9604644775390625e-08f;                                 // 2^-24, as the codes' products carry it
-#pragma unroll
-            for (int k = 0; k < 2; ++k) qsum[g][k] = __shfl_sync(0xffffffffu, sums[g], 4 * (2 * c4 + k));
-        }
-        const float mul = a.scale_log2 * pow2(24 - e);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) unit[k] = __shfl_sync(0xffffffffu, mul, 4 * (2 * c4 + k));
+        long long before;
+        const long long from = total * min(me, warps - 1) / warps, to = me < warps ? total * (me + 1) / warps : from;
+        line.b = rows.row_of(a, from, before);
+        line.n = chunks_of(a, line.b);
+        const int len = line.n + kStart;
+        line.unit = (int)((from - before) / len);
+        line.left = to - from;
+        // does the CTA's stretch end in the unit that it starts in?
+        const long long cta_from = total * (me - warp) / warps, cta_to = total * min(me - warp + kWarps, warps) / warps;
+        const long long unit_at = before + (long long)line.unit * len;
+        together = cta_from >= unit_at && cta_to <= unit_at + len;
+        together = __syncthreads_and(together);
+        line.take((int)(from - unit_at));
     }
 
-    float acc[J][2][4];                                                         // [32 dims][pair of dims of a half-word][fragment]
-    float off[NG][2];                                                           // the minima's part
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-    float vinv = 16777216.f;                                                    // power of two: steps times it are at most 32
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][e][i] = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) off[g][0] = off[g][1] = 0.f;
-
-    const int t0 = token_of(row);
-    bool gave_up = false;
-    int issued = mine < kStages ? mine : kStages;
-    for (int i = 0; i < mine && i < issued; ++i) {
-        if ((i >> 5) != batch) {
-            ids0 = ids1;
-            ++batch;
-            ids1 = page_of(32 * (batch + 1) + lane);
+    // ---- the warp's ring: a cursor that runs ahead of the work, over this and the following segments
+    const int tshift = a.c.page_shift - 4, per1 = (1 << tshift) - 1;
+    const uint32_t ring_s = smem_u32(ring) + lane * 16;
+    Line ahead = line;
+    const int* ids = nullptr;                                                   // the cursor's row of the table
+    const unsigned char* head = nullptr;                                        // its head's part of page 0
+    int at = line.lo, id0 = -1;                                                 // its chunk, and the page of the chunk's first tile
+    bool more = true;
+    uint32_t there_q = 0;                                                       // two bits for every chunk on its way: which tiles there are
+    auto enter = [&]() {
+        ids = a.c.table + (size_t)ahead.b * a.c.width;
+        head = a.c.pool + ((size_t)(ahead.unit / a.blocks) << tshift) * kBytes + lane * 16;
+    };
+    auto look = [&]() {                                                         // the cursor's chunk, if there is one, is looked up
+        while (at >= ahead.hi) {
+            if (!(more = ahead.next(a))) return;
+            at = ahead.lo;
+            enter();
         }
-        const int page = id_at(i);
-        unsigned char* tile = sm.ring[warp][i % kStages];
-        if (!mbar_wait(smem_u32(&sm.full[warp][i % kStages]), (i / kStages) & 1, &sm.abort_flag[warp], kWaitNs)) gave_up = true;
-        gave_up = __any_sync(0xffffffffu, gave_up);
-        const bool there = (unsigned)page < (unsigned)a.c.pages;
-        if (!there && lane == 0) atomicExch(a.error, kErrPage);
-        if (there && !gave_up) {
-            const bool last = lo + warp + i * kWarps == tiles - 1;
-            if (last) {
-                // the new token's row: quantised here, into this tile and (by the first pass) into the cache
-                const bool value = (lane / F::NW) & 1;
-                const int w = lane % F::NW, r = pos & 15;
-                constexpr int kLanes = D / NG / 8;
-                float x[8];
-                load_rotated<D>(a.qkv + b * a.stride + (a.heads + (value ? a.c.kv_heads : 0) + kvh) * D, w, value ? nullptr : a.cos, a.sin, pos, x);
-                __half2 par;
-                const uint32_t word = quantize8(x, kLanes, par);
-                auto put = [&](unsigned char* to) {
-                    if (!value) {
-                        *reinterpret_cast<uint32_t*>(to + F::key_word(r, w)) = word;
-                    } else {
-                        *reinterpret_cast<uint16_t*>(to + F::val_half(r, 2 * w)) = (uint16_t)word;
-                        *reinterpret_cast<uint16_t*>(to + F::val_half(r, 2 * w + 1)) = (uint16_t)(word >> 16);
-                    }
-                    if (w % kLanes == 0) *reinterpret_cast<__half2*>(to + (value ? F::val_par(r, w / kLanes) : F::key_par(r, w / kLanes))) = par;
-                };
-                if (lane < 2 * F::NW) {
-                    put(tile);
-                    if (hb == 0) put(tile_at(i, page));
+        id0 = ids[(2 * at) >> tshift];
+    };
+    auto fetch = [&](int stage) {
+        uint32_t there = 0;
+        if (more) {
+            const uint32_t to = ring_s + stage * L::kStage;
+            const bool ok0 = (unsigned)id0 < (unsigned)a.c.pages;
+            const unsigned char* from = head + id0 * a.page_bytes;
+            if (tshift > 0) {                                                   // both tiles in one page
+                if (ok0) {
+                    from += ((2 * at) & per1) * kBytes;
+#pragma unroll
+                    for (int i = 0; i < (2 * kBytes + 511) / 512; ++i)
+                        if ((i + 1) * 512 <= 2 * kBytes || i * 512 + lane * 16 < 2 * kBytes) copy16(to + i * 512, from + i * 512);
+                    there = 3;
                 }
-                __syncwarp();
+            } else {
+                const int id1 = 2 * at + 1 < a.c.width ? ids[2 * at + 1] : -1;
+                const bool ok1 = (unsigned)id1 < (unsigned)a.c.pages;
+                const unsigned char* second = head + id1 * a.page_bytes;
+#pragma unroll
+                for (int i = 0; i < (kBytes + 511) / 512; ++i) {
+                    const bool in = (i + 1) * 512 <= kBytes || i * 512 + lane * 16 < kBytes;
+                    if (ok0 && in) copy16(to + i * 512, from + i * 512);
+                    if (ok1 && in) copy16(to + kBytes + i * 512, second + i * 512);
+                }
+                there = ok0 | ok1 << 1;
             }
-            // scores: fragment rows are the tokens t0 and t0 + 8, columns the heads 2 c and 2 c + 1
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            {
-                uint32_t ka[J], kb[J];
-                if constexpr (J == 4) {
-                    *reinterpret_cast<uint4*>(ka) = *reinterpret_cast<const uint4*>(tile + t0 * (D / 2) + 16 * c4);
-                    *reinterpret_cast<uint4*>(kb) = *reinterpret_cast<const uint4*>(tile + (t0 + 8) * (D / 2) + 16 * c4);
-                } else {
-                    *reinterpret_cast<uint2*>(ka) = *reinterpret_cast<const uint2*>(tile + t0 * (D / 2) + 8 * c4);
-                    *reinterpret_cast<uint2*>(kb) = *reinterpret_cast<const uint2*>(tile + (t0 + 8) * (D / 2) + 8 * c4);
+            ++at;
+            look();
+        }
+        there_q |= there << (2 * a.stages);                                     // (shifted down by two when the next chunk is taken)
+        copies_issued();
+    };
+    enter();
+    look();
+    for (int i = 0; i < a.stages; ++i) {
+        there_q >>= 2;
+        fetch(i);
+    }
+    there_q >>= 2;
+
+    const int t0 = token_of(row), kcol = min(row, a.cols - 1);                  // columns that no head stands in repeat the last one
+    int stage = 0;
+    for (;;) {
+        const int b = line.b, kvh = line.unit / a.blocks, hb = line.unit % a.blocks, pos = a.pos[b];
+        const int cols = min(kCols, a.share - hb * kCols), head0 = kvh * a.share + hb * kCols;
+        if (line.lo < line.hi) {
+            // ---- queries to shared memory, as B fragments: head n, word w of 8 dims -> low nibbles' dims (0,4)(2,6), high nibbles'
+            // (1,5)(3,7) / 16, of q times the power of two that brings its largest element into [2^14, 2^15): a sixteenth is then
+            // exact down to 2^-39 of the largest
+            for (int i0 = 0; i0 < a.cols * F::NW; i0 += 32) {
+                const bool in = i0 + lane < a.cols * F::NW;
+                const int n = min(i0 + lane, a.cols * F::NW - 1) / F::NW, w = (i0 + lane) % F::NW;
+                constexpr int kLanes = D / NG / 8;
+                float q[8], top = 0.f, sum = 0.f;
+                load_rotated<D>(a.qkv + b * a.stride + (head0 + min(n, cols - 1)) * D, w, a.cos, a.sin, pos, q);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(q[k]));
+#pragma unroll
+                for (int o = 1; o < F::NW; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const int e = top > 0.f ? max(14 - exponent(top), -2) : 0;      // (-2: infinities)
+                // (the scale's sign goes into the queries, so that `unit` is positive; a scale of zero makes them zero)
+                const float up = a.scale_log2 == 0.f ? 0.f : a.scale_log2 < 0.f ? -pow2(e) : pow2(e);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += q[k] *= up;
+                if (in) q_s[n * L::kQPitch + w] = make_uint4(pack2(q[0], q[4]), pack2(q[2], q[6]), pack2(q[1] * 0.0625f, q[5] * 0.0625f),
+                                                             pack2(q[3] * 0.0625f, q[7] * 0.0625f));
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (in && w % kLanes == 0) qsum_s[n * NG + w / kLanes] = sum * 5.9604644775390625e-08f;   // 2^-24, as the codes' products carry it
+                if (in && w == 0) unit_s[n] = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2) * pow2(24 - e);
+            }
+            __syncwarp();
+        }
+        float qsum[NG][2], unit[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int n = min(2 * c4 + k, a.cols - 1);
+            unit[k] = unit_s[n];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qsum[g][k] = qsum_s[n * NG + g];
+        }
+        float acc[J][2][4];                                                     // [32 dims][pair of dims of a half-word][fragment]
+        float off[NG][2];                                                       // the minima's part
+        float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+        int elog = -24;                                                         // steps are below 2^(elog + 5)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][e][i] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) off[g][0] = off[g][1] = 0.f;
+
+        for (int t = line.lo; t < line.hi; ++t) {
+            unsigned char* chunk = ring + stage * L::kStage;
+            if (a.stages == 3) copies_wait<2>();
+            else copies_wait<1>();
+            __syncwarp();
+            const int there = there_q & 3;
+            const int left = pos + 1 - t * kChunk;                              // tokens from the chunk's first on
+            int count0 = kTile, count1 = kTile;
+            if (there != 3 || left <= kChunk) {
+                count0 = there & 1 ? min(left, kTile) : 0;
+                count1 = there & 2 ? min(left - kTile, kTile) : 0;
+                if (lane == 0 && (!(there & 1) || (left > kTile && !(there & 2)))) atomicExch(a.error, kErrPage);
+                const int behind = left > kTile;                                // the new token's tile, where the chunk has it
+                if (left <= kChunk && (behind ? count1 : count0) > 0) {
+                    // the new token's row: quantised here, into this chunk and (by the first pass) into the cache
+                    const bool value = (lane / F::NW) & 1;
+                    const int w = lane % F::NW, r = pos & 15;
+                    constexpr int kLanes = D / NG / 8;
+                    float x[8];
+                    load_rotated<D>(a.qkv + b * a.stride + (a.heads + (value ? a.c.kv_heads : 0) + kvh) * D, w, value ? nullptr : a.cos, a.sin, pos, x);
+                    __half2 par;
+                    const uint32_t word = quantize8(x, kLanes, par);
+                    auto put = [&](unsigned char* to) {
+                        if (!value) {
+                            *reinterpret_cast<uint32_t*>(to + F::key_word(r, w)) = word;
+                        } else {
+                            *reinterpret_cast<uint16_t*>(to + F::val_half(r, 2 * w)) = (uint16_t)word;
+                            *reinterpret_cast<uint16_t*>(to + F::val_half(r, 2 * w + 1)) = (uint16_t)(word >> 16);
+                        }
+                        if (w % kLanes == 0) *reinterpret_cast<__half2*>(to + (value ? F::val_par(r, w / kLanes) : F::key_par(r, w / kLanes))) = par;
+                    };
+                    if (lane < 2 * F::NW) {
+                        put(chunk + behind * kBytes);
+                        if (hb == 0) put(a.c.tile(b, kvh, pos, kBytes));
+                    }
+                    __syncwarp();
+                }
+            }
+            if (count0 > 0 || count1 > 0) {
+                // scores: fragment rows are the tokens t0 and t0 + 8 of a tile, columns the heads 2 c and 2 c + 1
+                float x[2][4];
+                uint32_t ka[2][J], kb[2][J];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const unsigned char* tile = chunk + u * kBytes;
+                    if constexpr (J == 4) {
+                        *reinterpret_cast<uint4*>(ka[u]) = *reinterpret_cast<const uint4*>(tile + t0 * (D / 2) + 16 * c4);
+                        *reinterpret_cast<uint4*>(kb[u]) = *reinterpret_cast<const uint4*>(tile + (t0 + 8) * (D / 2) + 16 * c4);
+                    } else {
+                        *reinterpret_cast<uint2*>(ka[u]) = *reinterpret_cast<const uint2*>(tile + t0 * (D / 2) + 8 * c4);
+                        *reinterpret_cast<uint2*>(kb[u]) = *reinterpret_cast<const uint2*>(tile + (t0 + 8) * (D / 2) + 8 * c4);
+                    }
                 }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                    float s4[2][4];
 #pragma unroll
                     for (int j = g * J / NG; j < (g + 1) * J / NG; ++j) {
-                        uint32_t ha[4], hc[4];
-                        unpack_s4x8_denorm(ka[j], ha);
-                        unpack_s4x8_denorm(kb[j], hc);
-                        const uint32_t lowf[4] = {ha[0], hc[0], ha[2], hc[2]}, highf[4] = {ha[1], hc[1], ha[3], hc[3]};
-                        mma_m16n8k16(s4, lowf, qf[j][0], qf[j][1]);
-                        mma_m16n8k16(s4, highf, qf[j][2], qf[j][3]);
+                        const uint4 qf = q_s[kcol * L::kQPitch + 4 * j + c4];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            uint32_t ha[4], hc[4];
+                            unpack_s4x8_denorm(ka[u][j], ha);
+                            unpack_s4x8_denorm(kb[u][j], hc);
+                            const uint32_t lowf[4] = {ha[0], hc[0], ha[2], hc[2]}, highf[4] = {ha[1], hc[1], ha[3], hc[3]};
+                            if (j == g * J / NG) mma_m16n8k16_zc(s4[u], lowf, qf.x, qf.y);
+                            else mma_m16n8k16(s4[u], lowf, qf.x, qf.y);
+                            mma_m16n8k16(s4[u], highf, qf.z, qf.w);
+                        }
                     }
-                    const float2 pa = __half22float2(*reinterpret_cast<const __half2*>(tile + F::key_par(t0, g)));
-                    const float2 pb = __half22float2(*reinterpret_cast<const __half2*>(tile + F::key_par(t0 + 8, g)));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(chunk + u * kBytes + F::key_par(t0, g)));
+                        const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(chunk + u * kBytes + F::key_par(t0 + 8, g)));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            x[u][k] = fmaf(fa.x, s4[u][k], g ? fmaf(fa.y, qsum[g][k], x[u][k]) : fa.y * qsum[g][k]);
+                            x[u][2 + k] = fmaf(fb.x, s4[u][2 + k], g ? fmaf(fb.y, qsum[g][k], x[u][2 + k]) : fb.y * qsum[g][k]);
+                        }
+                    }
+                }
+                __half2 va[2][NG], vb[2][NG];                                   // (step, minimum) of the two tokens' values
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    load_params<NG>(chunk + u * kBytes + F::val_par(t0, 0), va[u]);
+                    load_params<NG>(chunk + u * kBytes + F::val_par(t0 + 8, 0), vb[u]);
+                }
+                if (count0 < kTile || count1 < kTile) {                         // tokens behind the new one, pages that are none
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int count = u ? count1 : count0;
+                        if (t0 >= count) {
+                            x[u][0] = x[u][1] = -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) va[u][g] = __half2half2(__ushort_as_half(0));
+                        }
+                        if (t0 + 8 >= count) {
+                            x[u][2] = x[u][3] = -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) vb[u][g] = __half2half2(__ushort_as_half(0));
+                        }
+                    }
+                }
+                __half2 big = __hmax2(va[0][0], vb[0][0]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+                        if (u || g) big = __hmax2(big, __hmax2(va[u][g], vb[u][g]));
+                float smax = __low2float(big);
+                const float m0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])) * unit[0];
+                const float m1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3])) * unit[1];
+                const float room = 8.f - (float)elog;
+                if (__any_sync(0xffffffffu, m0 - ref[0] > room || m1 - ref[1] > room || smax > pow2(elog + 5))) {
+                    float n0 = fmaxf(m0, ref[0] - (float)elog), n1 = fmaxf(m1, ref[1] - (float)elog);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+                        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+                        smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
+                    }
+                    if (smax > pow2(elog + 5)) elog = exponent(fminf(smax, 65504.f));
+                    const float r0 = n0 + (float)elog, r1 = n1 + (float)elog;
+                    const float keep[2] = {ref[0] == -INFINITY ? 0.f : ex2(ref[0] - r0), ref[1] == -INFINITY ? 0.f : ex2(ref[1] - r1)};
+                    ref[0] = r0;
+                    ref[1] = r1;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        x[k] = fmaf(pa.x, s4[k], fmaf(pa.y, qsum[g][k], x[k]));
-                        x[2 + k] = fmaf(pb.x, s4[2 + k], fmaf(pb.y, qsum[g][k], x[2 + k]));
+                        sum[k] *= keep[k];
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) off[g][k] *= keep[k];
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                acc[j][e][k] *= keep[k];
+                                acc[j][e][2 + k] *= keep[k];
+                            }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const unsigned char* tile = chunk + u * kBytes;
+                    float p[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(x[u][k], unit[k & 1], -ref[k & 1]));
+                    sum[0] += p[0] + p[2];
+                    sum[1] += p[1] + p[3];
+                    uint32_t wf[NG][2];                                         // B fragments: tokens 2c, 2c+1 (+ 8) of column lane / 4
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float2 fa = __half22float2(va[u][g]), fb = __half22float2(vb[u][g]);
+                        wf[g][0] = transpose8x8(pack2(p[0] * fa.x, p[1] * fa.x));
+                        wf[g][1] = transpose8x8(pack2(p[2] * fb.x, p[3] * fb.x));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) off[g][k] = fmaf(p[k], fa.y, fmaf(p[2 + k], fb.y, off[g][k]));
+                    }
+                    // output: fragment rows are dims 32 j + 4 row + 2 e and the next one
+                    uint32_t v[4][J / 2];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int tk = token_of(2 * c4 + (k & 1)) + 8 * (k >> 1);
+                        const unsigned char* vat = tile + F::kVal + tk * (D / 2) + (D == 128 ? (8 * row) ^ (((tk >> 1) & 1) << 5) : 4 * row);
+                        if constexpr (J == 4) *reinterpret_cast<uint2*>(v[k]) = *reinterpret_cast<const uint2*>(vat);
+                        else v[k][0] = *reinterpret_cast<const uint32_t*>(vat);
+                    }
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const uint32_t u0 = __byte_perm(v[0][j / 2], v[1][j / 2], j & 1 ? 0x7632 : 0x5410);
+                        const uint32_t u1 = __byte_perm(v[2][j / 2], v[3][j / 2], j & 1 ? 0x7632 : 0x5410);
+                        uint32_t h0[4], h1[4];
+                        unpack_s4x8_denorm(u0, h0);
+                        unpack_s4x8_denorm(u1, h1);
+                        const uint32_t f0[4] = {h0[0], h0[1], h1[0], h1[1]}, f1[4] = {h0[2], h0[3], h1[2], h1[3]};
+                        constexpr int per = D / NG;
+                        mma_m16n8k16(acc[j][0], f0, wf[32 * j / per][0], wf[32 * j / per][1]);
+                        mma_m16n8k16(acc[j][1], f1, wf[32 * j / per][0], wf[32 * j / per][1]);
                     }
                 }
             }
-            float2 va[NG], vb[NG];                                              // (step, minimum) of the two tokens' values
-            float smax = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                va[g] = __half22float2(*reinterpret_cast<const __half2*>(tile + F::val_par(t0, g)));
-                vb[g] = __half22float2(*reinterpret_cast<const __half2*>(tile + F::val_par(t0 + 8, g)));
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                x[k] *= unit[k];
-                x[2 + k] *= unit[k];
-            }
-            if (last) {                                                         // tokens behind the new one: whatever the page holds there
-                const int left = pos & 15;
-                if (t0 > left) {
-                    x[0] = x[1] = -INFINITY;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) va[g] = make_float2(0.f, 0.f);
-                }
-                if (t0 + 8 > left) {
-                    x[2] = x[3] = -INFINITY;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) vb[g] = make_float2(0.f, 0.f);
-                }
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) smax = fmaxf(smax, fmaxf(va[g].x, vb[g].x));
-            const float m0 = fmaxf(x[0], x[2]), m1 = fmaxf(x[1], x[3]);
-            if (__any_sync(0xffffffffu, m0 > top[0] + 8.f || m1 > top[1] + 8.f || smax * vinv > 32.f)) {
-                float n0 = fmaxf(m0, top[0]), n1 = fmaxf(m1, top[1]);
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-                    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
-                    smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
-                }
-                // steps up to the largest fp16, 2^16, down to 2^-24
-                const float vnew = smax * vinv > 32.f ? pow2(-((__float_as_int(fminf(smax, 65504.f)) >> 23) - 127)) : vinv;
-                const float keep[2] = {top[0] == -INFINITY ? 0.f : ex2(top[0] - n0), top[1] == -INFINITY ? 0.f : ex2(top[1] - n1)};
-                const float turn = vnew / vinv;
-                top[0] = n0;
-                top[1] = n1;
-                vinv = vnew;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    sum[k] *= keep[k];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) off[g][k] *= keep[k];
-#pragma unroll
-                    for (int j = 0; j < J; ++j)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            acc[j][e][k] *= keep[k] * turn;
-                            acc[j][e][2 + k] *= keep[k] * turn;
-                        }
-                }
-            }
-            const float p[4] = {ex2(x[0] - top[0]), ex2(x[1] - top[1]), ex2(x[2] - top[0]), ex2(x[3] - top[1])};
-            sum[0] += p[0] + p[2];
-            sum[1] += p[1] + p[3];
-            uint32_t wf[NG][2];                                                 // B fragments: tokens 2c, 2c+1 (+ 8) of column lane / 4
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const float sa = va[g].x * vinv, sb = vb[g].x * vinv;
-                wf[g][0] = transpose8x8(pack2(p[0] * sa, p[1] * sa));
-                wf[g][1] = transpose8x8(pack2(p[2] * sb, p[3] * sb));
-#pragma unroll
-                for (int k = 0; k < 2; ++k) off[g][k] = fmaf(p[k], va[g].y, fmaf(p[2 + k], vb[g].y, off[g][k]));
-            }
-            // output: fragment rows are dims 32 j + 4 row + 2 e and the next one
-            uint32_t v[4][J / 2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = token_of(2 * c4 + (k & 1)) + 8 * (k >> 1);
-                const unsigned char* at = tile + F::kVal + t * (D / 2) + (D == 128 ? (8 * row) ^ (((t >> 1) & 1) << 5) : 4 * row);
-                if constexpr (J == 4) *reinterpret_cast<uint2*>(v[k]) = *reinterpret_cast<const uint2*>(at);
-                else v[k][0] = *reinterpret_cast<const uint32_t*>(at);
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const uint32_t u0 = __byte_perm(v[0][j / 2], v[1][j / 2], j & 1 ? 0x7632 : 0x5410);
-                const uint32_t u1 = __byte_perm(v[2][j / 2], v[3][j / 2], j & 1 ? 0x7632 : 0x5410);
-                uint32_t h0[4], h1[4];
-                unpack_s4x8_denorm(u0, h0);
-                unpack_s4x8_denorm(u1, h1);
-                const uint32_t f0[4] = {h0[0], h0[1], h1[0], h1[1]}, f1[4] = {h0[2], h0[3], h1[2], h1[3]};
-                constexpr int per = D / NG;
-                mma_m16n8k16(acc[j][0], f0, wf[32 * j / per][0], wf[32 * j / per][1]);
-                mma_m16n8k16(acc[j][1], f1, wf[32 * j / per][0], wf[32 * j / per][1]);
-            }
+            __syncwarp();                                                       // everybody has read the chunk
+            fetch(stage);
+            there_q >>= 2;
+            if (++stage == a.stages) stage = 0;
         }
-        __syncwarp();                                                           // everybody has read the tile
-        if (!gave_up && issued < mine) {
-            fetch(issued);
-            ++issued;
-        }
-    }
-    if (gave_up && lane == 0) atomicExch(a.error, 1);
 
-    // ---- the warp's result takes the place of its ring: [column][D], maxima and sums beside it
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) off[g][k] += __shfl_xor_sync(0xffffffffu, off[g][k], o);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        if (sum[k] != sum[k]) top[k] = sum[k];                                  // NaN scores: not to be taken for "no tiles"
-    __syncwarp();
-    float* o_s = reinterpret_cast<float*>(sm.ring[warp]);
-    const float back = 1.f / vinv;                                              // (exact: a power of two)
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float* at = o_s + (2 * c4 + k) * kPitch + 32 * j + 4 * row + 2 * e;
-                at[0] = fmaf(acc[j][e][k] * kDenormScaleLo, back, off[32 * j * NG / D][k]);
-                at[1] = fmaf(acc[j][e][2 + k] * kDenormScaleHi, back, off[32 * j * NG / D][k]);
-            }
-    if (row == 0) {
+        // ---- the segment's result: dims 32 j + 4 row .. + 3 of columns 2 c and 2 c + 1
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            sm.m[warp][2 * c4 + k] = top[k];
-            sm.l[warp][2 * c4 + k] = sum[k];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) off[g][k] += __shfl_xor_sync(0xffffffffu, off[g][k], o);
+            }
+            if (sum[k] != sum[k]) ref[k] = sum[k];                              // NaN scores: not to be taken for "no chunks"
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float o = off[32 * j * NG / D][k];
+                acc[j][0][k] = fmaf(acc[j][0][k], kDenormScaleLo, o);
+                acc[j][0][2 + k] = fmaf(acc[j][0][2 + k], kDenormScaleHi, o);
+                acc[j][1][k] = fmaf(acc[j][1][k], kDenormScaleLo, o);
+                acc[j][1][2 + k] = fmaf(acc[j][1][2 + k], kDenormScaleHi, o);
+            }
         }
-    }
-    __syncthreads();
-    const int cols = min(kCols, a.share - hb * kCols);
-    if (threadIdx.x < kCols) {
-        float m = -INFINITY, l = 0.f;
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm.m[w][threadIdx.x]);
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = sm.m[w][threadIdx.x] == -INFINITY ? 0.f : ex2(sm.m[w][threadIdx.x] - m);
-            l = fmaf(sm.l[w][threadIdx.x], f, l);
-            sm.m[w][threadIdx.x] = f;                                           // from here on: the warp's factor
+        const bool starts = line.lo == 0 && line.hi > 0, whole = starts && line.hi == line.n;
+        // the warps that a unit starting here is dealt to, this one first: its last chunk stands n - hi behind the segment's end
+        auto dealt = [&]() {
+            const long long end = total * (me + 1) / warps - line.left + line.n - line.hi;
+            return make_int4(b, line.unit, (int)((end * warps - 1) / total - me) + 1, 0);
+        };
+        if (!together) {
+            if (line.lo < line.hi) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (2 * c4 + k >= cols) continue;
+                    if (whole) {
+                        const float l = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+                        __half* to = a.out + ((size_t)b * a.heads + head0 + 2 * c4 + k) * D + 4 * row;
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+                            *reinterpret_cast<uint2*>(to + 32 * j) = make_uint2(pack2(acc[j][0][k] * l, acc[j][0][2 + k] * l), pack2(acc[j][1][k] * l, acc[j][1][2 + k] * l));
+                    } else {
+                        float* to = a.part + ((me * 2 + starts) * a.cols + 2 * c4 + k) * (D + 4);
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+                            *reinterpret_cast<float4*>(to + 32 * j + 4 * row) = make_float4(acc[j][0][k], acc[j][0][2 + k], acc[j][1][k], acc[j][1][2 + k]);
+                        if (row == 0) *reinterpret_cast<float2*>(to + D) = make_float2(ref[k], sum[k]);
+                    }
+                }
+                if (starts && !whole) split_unit = dealt();
+            }
+            if (line.next(a)) continue;
+            if (lane == 0) a.split_units[me] = split_unit;
+            return;
         }
-        sm.m[kWarps][threadIdx.x] = m;
-        sm.l[kWarps][threadIdx.x] = l;
-    }
-    __syncthreads();
-    auto merged = [&](int col, int d) {
-        float v = 0.f;
+
+        // ---- together: the four warps' results meet where the rings were
+        copies_wait<0>();
+        __syncthreads();
+        float* meet = reinterpret_cast<float*>(raw);                            // [warps][columns][kPitch], reference and sum behind the dims
+        int* ends = reinterpret_cast<int*>(meet + kWarps * a.cols * kPitch);    // [warps]: chunks of the unit up to the warp's, -1: none of its own
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (2 * c4 + k >= cols) continue;
+            float* to = meet + (warp * a.cols + 2 * c4 + k) * kPitch;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                *reinterpret_cast<float4*>(to + 32 * j + 4 * row) = make_float4(acc[j][0][k], acc[j][0][2 + k], acc[j][1][k], acc[j][1][2 + k]);
+            if (row == 0) *reinterpret_cast<float2*>(to + D) = make_float2(ref[k], sum[k]);
+        }
+        if (lane == 0) {
+            ends[warp] = line.lo < line.hi ? line.hi : -1;
+            ends[kWarps + warp] = starts;
+        }
+        __syncthreads();
+        int last = -1, starter = -1;                                            // end of the CTA's chunks; the warp that has chunk 0
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = sm.m[w][col];
-            if (f != 0.f) v = fmaf(reinterpret_cast<const float*>(sm.ring[w])[col * kPitch + d], f, v);
+            last = max(last, ends[w]);
+            if (ends[kWarps + w]) starter = w;
         }
-        return v;
-    };
-    const int head0 = kvh * a.share + hb * kCols;
-    if (a.splits == 1) {
+        if (a.part && lane == 0) a.split_units[me] = starter == warp && last < line.n ? dealt() : make_int4(0, 0, 0, 0);
+        if (last < 0) return;
+        // the part goes to the slot of one warp that has a share, the others' say that they hold nothing
+        const bool all = starter >= 0 && last == line.n;
+        const int holder = starter >= 0 ? starter : blockIdx.x % (a.part ? (int)min((long long)kWarps, warps - (me - warp)) : kWarps);
         for (int i = threadIdx.x; i < cols * D; i += kThreads) {
-            const float l = sm.l[kWarps][i / D];
-            a.out[((size_t)b * a.heads + head0) * D + i] = __float2half_rn(l == 0.f ? 0.f : merged(i / D, i % D) / l);
-        }
-        return;
-    }
-    if (a.part) {                                                               // joined by join_kernel
-        for (int i = threadIdx.x; i < cols * D; i += kThreads)
-            a.part[(((size_t)b * a.heads + head0 + i / D) * a.splits + split) * (D + 2) + i % D] = merged(i / D, i % D);
-        if (threadIdx.x < cols) {
-            float* at = a.part + (((size_t)b * a.heads + head0 + threadIdx.x) * a.splits + split) * (D + 2) + D;
-            at[0] = sm.m[kWarps][threadIdx.x];
-            at[1] = sm.l[kWarps][threadIdx.x];
-        }
-        return;
-    }
-    // the cluster: every CTA leaves its merged output in place of warp 0's, and joins its share of the elements
-    {
-        float* o0 = reinterpret_cast<float*>(sm.ring[0]);
-        for (int i = threadIdx.x; i < cols * D; i += kThreads) o0[(i / D) * kPitch + i % D] = merged(i / D, i % D);
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        for (int i = threadIdx.x + split * kThreads; i < cols * D; i += kThreads * a.splits) {
-            const int col = i / D;
-            float m = -INFINITY, num = 0.f, den = 0.f;
-            for (int r = 0; r < a.splits; ++r) m = fmaxf(m, *cluster.map_shared_rank(&sm.m[kWarps][col], r));
-            for (int r = 0; r < a.splits; ++r) {
-                const float mr = *cluster.map_shared_rank(&sm.m[kWarps][col], r);
-                if (mr == -INFINITY) continue;                                  // no tiles of its own
-                const float f = ex2(mr - m);
-                num = fmaf(*cluster.map_shared_rank(o0 + col * kPitch + i % D, r), f, num);
-                den = fmaf(*cluster.map_shared_rank(&sm.l[kWarps][col], r), f, den);
+            const int col = i / D, d = i % D;
+            float m = -INFINITY, l = 0.f, v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, meet[(w * a.cols + col) * kPitch + D]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float* from = meet + (w * a.cols + col) * kPitch;
+                if (from[D] == -INFINITY) continue;                             // no chunk of its own
+                const float f = ex2(from[D] - m);
+                l = fmaf(from[D + 1], f, l);
+                v = fmaf(from[d], f, v);
             }
-            a.out[((size_t)b * a.heads + head0) * D + i] = __float2half_rn(den == 0.f ? 0.f : num / den);
+            if (all) {
+                a.out[((size_t)b * a.heads + head0) * D + i] = __float2half_rn(l == 0.f ? 0.f : v / l);
+            } else {
+                float* to = a.part + ((((long long)blockIdx.x * kWarps + holder) * 2 + (starter >= 0)) * a.cols + col) * (D + 4);
+                to[d] = v;
+                if (d < kWarps) {
+                    if (d == holder) *reinterpret_cast<float2*>(to + D) = make_float2(l != l ? l : m, l);
+                    else a.part[((((long long)blockIdx.x * kWarps + d) * 2) * a.cols + col) * (D + 4) + D] = -INFINITY;
+                }
+            }
         }
-        cluster.sync();                                                         // others may still be reading this CTA's
+        return;
     }
 }
 
-// Joins the partial outputs of a row's splits: grid (heads, batch), a thread per dim.
+// Puts the parts of split units together: a warp for every warp of the grid before, a column each (blockIdx.y); units of more than 16 parts
+// are joined by the whole block afterwards, so that a long row alone does not wait for one part after the other.
 template <int D>
-__global__ void __launch_bounds__(D) join_kernel(const DecodeArgs a)
+__global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a, int warps)
 {
-    const int head = blockIdx.x, b = blockIdx.y, pos = a.pos[b];
-    if (pos < 0 || pos >= a.c.capacity() || (a.cos && pos >= a.rope_rows)) return;
-    const float* part = a.part + ((size_t)b * a.heads + head) * a.splits * (D + 2);
-    float m = -INFINITY, num = 0.f, den = 0.f;
-    for (int r = 0; r < a.splits; ++r) m = fmaxf(m, part[r * (D + 2) + D]);
-    for (int r = 0; r < a.splits; ++r) {
-        const float mr = part[r * (D + 2) + D];
-        if (mr == -INFINITY) continue;
-        const float f = ex2(mr - m);
-        num = fmaf(part[r * (D + 2) + threadIdx.x], f, num);
-        den = fmaf(part[r * (D + 2) + D + 1], f, den);
+    constexpr int kDims = D / 4, kSub = 256 / kDims, kFew = 16;
+    __shared__ int4 many[8];
+    __shared__ float4 num_s[kSub][kDims];
+    __shared__ float top_s[8], den_s[kSub];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int me = blockIdx.x * 8 + warp;
+    int4 u = me < warps ? a.split_units[me] : make_int4(0, 0, 0, 0);
+    if (u.y % a.blocks * kCols + col >= a.share) u.z = 0;                       // a pass of fewer heads
+    auto part = [&](int first, int i) { return a.part + (((first + (long long)i) * 2 + (i == 0)) * a.cols + col) * (D + 4); };
+    auto out = [&](const int4& u) {
+        return a.out + ((size_t)u.x * a.heads + u.y / a.blocks * a.share + u.y % a.blocks * kCols + col) * D;
+    };
+    if (lane == 0) many[warp] = make_int4(u.x, u.y, u.z > kFew ? u.z : 0, me);
+    if (u.z > 0 && u.z <= kFew) {
+        const float2 ml = lane < u.z ? *reinterpret_cast<const float2*>(part(me, lane) + D) : make_float2(-INFINITY, 0.f);
+        float m = ml.x, l = 0.f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = __shfl_sync(0xffffffffu, m, 0);
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);                // (NaN stays)
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < u.z; ++i) {
+            const float fi = __shfl_sync(0xffffffffu, f, i), li = __shfl_sync(0xffffffffu, ml.y, i);
+            if (fi == 0.f) continue;                                            // holds nothing, or vanishes beside the others
+            l = fmaf(li, fi, l);
+            if (lane < kDims) {
+                const float4 x = *reinterpret_cast<const float4*>(part(me, i) + 4 * lane);
+                v = make_float4(fmaf(x.x, fi, v.x), fmaf(x.y, fi, v.y), fmaf(x.z, fi, v.z), fmaf(x.w, fi, v.w));
+            }
+        }
+        const float r = l == 0.f ? 0.f : 1.f / l;
+        if (lane < kDims) *reinterpret_cast<uint2*>(out(u) + 4 * lane) = make_uint2(pack2(v.x * r, v.y * r), pack2(v.z * r, v.w * r));
     }
-    a.out[((size_t)b * a.heads + head) * D + threadIdx.x] = __float2half_rn(den == 0.f ? 0.f : num / den);
+    __syncthreads();
+    for (int k = 0; k < 8; ++k) {
+        const int4 w = many[k];
+        if (w.z == 0) continue;                                                 // (uniform)
+        float m = -INFINITY;
+        for (int i = threadIdx.x; i < w.z; i += 256) m = fmaxf(m, part(w.w, i)[D]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) top_s[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, top_s[i]);
+        const int sub = threadIdx.x / kDims, d4 = threadIdx.x % kDims;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+        // (whole groups of 8 parts in flight; their references first, so that parts that hold nothing are not fetched)
+        for (int i0 = sub; i0 < w.z; i0 += 8 * kSub) {
+            float2 ml[8];
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                ml[i] = i0 + i * kSub < w.z ? *reinterpret_cast<const float2*>(part(w.w, i0 + i * kSub) + D) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (ml[i].x != -INFINITY) x[i] = *reinterpret_cast<const float4*>(part(w.w, i0 + i * kSub) + 4 * d4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (ml[i].x == -INFINITY) continue;
+                const float f = ex2(ml[i].x - m);
+                l = fmaf(ml[i].y, f, l);
+                v = make_float4(fmaf(x[i].x, f, v.x), fmaf(x[i].y, f, v.y), fmaf(x[i].z, f, v.z), fmaf(x[i].w, f, v.w));
+            }
+        }
+        num_s[sub][d4] = v;
+        if (d4 == 0) den_s[sub] = l;
+        __syncthreads();
+        if (threadIdx.x < D) {
+            float x = 0.f, den = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSub; ++i) {
+                x += reinterpret_cast<const float*>(num_s[i])[threadIdx.x];
+                den += den_s[i];
+            }
+            out(w)[threadIdx.x] = __float2half_rn(den == 0.f ? 0.f : x / den);
+        }
+        __syncthreads();
+    }
 }
 
-int g_force_split = 0;
+int g_force_ctas = 0;
 
 }  // namespace
 
-// CTAs that share a row's tiles.  Up to 8 meet in a cluster, more go through the workspace.
-int decode_splits(int batch, int heads, int kv_heads, int page_size, int width)
+// CTAs of a call that share the line, 0 where each takes a whole unit.  The line costs about 8 us more (finding the place, the second
+// launch); a CTA with a unit of its own takes a round of its four warps for every four chunks.  The host knows how long rows can be
+// from the table's width alone.  Measured, by units / by the line: 1 row of 77 tokens 6.3 / 12.9 us, 8 rows of 520 tokens, 32 heads
+// 14 / 20 us, 32 rows of 1030 51 / 50 us, 24 rows of 1 to 6000 tokens, 8 heads of 64 50 / 21 us.
+int decode_ctas(int batch, int units, int page_size, int width)
 {
-    if (g_force_split) return g_force_split;
-    const int share = heads / kv_heads, blocks = (share + kCols - 1) / kCols;
-    const long long units = (long long)batch * kv_heads * blocks, slots = 4ll * device_sm_count();
-    const long long tiles = (long long)width * page_size / kTile;              // of the longest row the table can hold
-    int s = 1;
-    while (s < 8 && units * s * 2 <= slots && tiles >= 2ll * kWarps * s * 2) s *= 2;
-    if (s == 8 && units * 16 <= slots && tiles >= 16ll * kWarps * 8) {
-        s = (int)(slots / units);
-        while (s > 16 && tiles < (long long)s * kWarps * 4) --s;
-        if (s > 128) s = 128;
-    }
-    return s;
+    if (g_force_ctas) return g_force_ctas < 0 ? 0 : g_force_ctas;
+    const long long slots = 4ll * device_sm_count(), longest = (long long)width * page_size / kChunk;
+    const long long waves = ((long long)batch * units + slots - 1) / slots;
+    return longest * waves <= 40 ? 0 : (int)slots;
 }
 
 template <class F, int D>
-static int launch_decode_as(const DecodeArgs& a, int batch, cudaStream_t st)
+static int launch_decode_as(DecodeArgs& a, int ctas, cudaStream_t st)
 {
-    using S = Smem<F, D>;
+    using L = Layout<F, D>;
     static int configured[64] = {0};   // benign race: the attribute call is idempotent
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(decode_kernel<F, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(S));
+        e = cudaFuncSetAttribute(decode_kernel<F, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem4);
         if (e != cudaSuccess) return record_cuda_error(e);
         if (dev < 64) configured[dev] = 1;
     }
+    static_assert(kWarps * L::warp_bytes(2, kCols) <= kSmem4, "two stages fit");
+    static_assert(kWarps * kCols * L::kPitch * 4 + 2 * kWarps * 4 <= kWarps * L::warp_bytes(2, kCols) &&
+                  kWarps * L::kPitch * 4 + 2 * kWarps * 4 <= kWarps * L::warp_bytes(2, 1), "the warps' results fit where the rings were");
+    a.stages = kWarps * L::warp_bytes(3, a.cols) <= kSmem4 ? 3 : 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.splits, a.c.kv_heads * a.blocks, batch);
+    cfg.gridDim = dim3(ctas ? ctas : a.units * a.batch);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(S);
+    cfg.dynamicSmemBytes = kWarps * L::warp_bytes(a.stages, a.cols);
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (a.splits > 1 && !a.part) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = a.splits;
-        attr[n].val.clusterDim.y = 1;
-        attr[n++].val.clusterDim.z = 1;
-    }
-    if (aux_programmatic_launch()) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = n;
-    e = cudaLaunchKernelEx(&cfg, decode_kernel<F, D>, a);
+    cfg.numAttrs = aux_programmatic_launch() ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, decode_kernel<F, D>, (const DecodeArgs)a);
     if (e != cudaSuccess) return record_cuda_error(e);
     count_launch();
-    if (a.part) {
-        join_kernel<D><<<dim3(a.heads, batch), D, 0, st>>>(a);
-        count_launch();
-        e = cudaGetLastError();
+    if (ctas) {
+        cfg.gridDim = dim3((ctas * kWarps + 7) / 8, a.cols);
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        cfg.numAttrs = 1;                                                       // resident when the last chunks are done
+        e = cudaLaunchKernelEx(&cfg, join_kernel<D>, (const DecodeArgs)a, ctas * kWarps);
         if (e != cudaSuccess) return record_cuda_error(e);
+        count_launch();
     }
     return W4A16_OK;
 }
@@ -550,18 +791,14 @@ static int launch_decode_as(const DecodeArgs& a, int batch, cudaStream_t st)
 using namespace w4a16;
 using namespace w4a16::kv4;
 
-// Tuning hook for tests and benchmarks: CTAs per (row, head), 0 = automatic.  Not part of the drop-in surface.
-extern "C" void w4a16_tune_kv4(int splits)
-{
-    const bool ok = splits == 1 || splits == 2 || splits == 4 || splits == 8 || (splits > 8 && splits <= 128);
-    w4a16::kv4::g_force_split = ok ? splits : 0;
-}
+// Tuning hook for tests and benchmarks: CTAs of a call, 0 = automatic, negative: one per unit.  Not part of the drop-in surface.
+extern "C" void w4a16_tune_kv4(int ctas) { w4a16::kv4::g_force_ctas = ctas > 4096 ? 4096 : ctas; }
 
 extern "C" size_t w4a16_kv4_decode_workspace(int batch, int heads, int kv_heads, int head_dim, int page_size, int width)
 {
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || page_size <= 0 || width <= 0) return 0;
-    const int s = decode_splits(batch, heads, kv_heads, page_size, width);
-    return s <= 8 ? 0 : (size_t)batch * heads * s * (head_dim + 2) * sizeof(float);
+    const int share = heads / kv_heads, cols = share < kCols ? share : kCols;
+    return (size_t)decode_ctas(batch, kv_heads * ((share + kCols - 1) / kCols), page_size, width) * kWarps * (sizeof(int4) + 2 * cols * (head_dim + 4) * sizeof(float));
 }
 
 extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const void* table, const void* pos, const void* rope_cos,
@@ -576,27 +813,32 @@ extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const voi
     if (batch < 0 || heads <= 0 || heads % kv_heads || qkv_stride < (heads + 2ll * kv_heads) * head_dim || (qkv_stride % 8) ||
         (rope_cos && rope_rows <= 0))
         return W4A16_ERR_BAD_SHAPE;
-    if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)rope_cos | (uintptr_t)rope_sin) & 15 || ((uintptr_t)pos | (uintptr_t)workspace) & 3)
+    if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)rope_cos | (uintptr_t)rope_sin) & 15 || (uintptr_t)pos & 3 || (uintptr_t)workspace & 15)
         return W4A16_ERR_MISALIGNED;
     if ((heads + 2ll * kv_heads) * head_dim >= (1ll << 30) || batch > 65535) return W4A16_ERR_TOO_LARGE;
     a.share = heads / kv_heads;
     a.blocks = (a.share + kCols - 1) / kCols;
-    if ((long long)kv_heads * a.blocks > 65535) return W4A16_ERR_TOO_LARGE;
+    a.cols = a.share < kCols ? a.share : kCols;
+    a.units = kv_heads * a.blocks;
+    if ((long long)a.units * batch >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
     if (batch == 0) return W4A16_OK;
-    a.splits = decode_splits(batch, heads, kv_heads, page_size, width);
+    const int ctas = decode_ctas(batch, a.units, page_size, width);
     a.part = nullptr;
-    if (a.splits > 8) {
+    a.split_units = nullptr;
+    if (ctas) {
         if (!workspace || workspace_bytes < w4a16_kv4_decode_workspace(batch, heads, kv_heads, head_dim, page_size, width)) return W4A16_ERR_WORKSPACE;
-        a.part = (float*)workspace;
+        a.split_units = (int4*)workspace;
+        a.part = (float*)(a.split_units + (size_t)ctas * kWarps);
     }
     a.qkv = (const __half*)qkv; a.out = (__half*)out; a.pos = (const int*)pos;
     a.cos = (const __half*)rope_cos; a.sin = (const __half*)rope_sin;
-    a.heads = heads; a.rope_rows = rope_rows; a.stride = qkv_stride;
+    a.batch = batch; a.heads = heads; a.rope_rows = rope_rows; a.stride = qkv_stride;
+    a.page_bytes = (long long)kv_heads * (page_size / kTile) * tile_bytes(head_dim, group);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.error = device_error_word();
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        return launch_decode_as<F, F::NW * 8>(a, batch, (cudaStream_t)stream);
+        return launch_decode_as<F, F::NW * 8>(a, ctas, (cudaStream_t)stream);
     });
 }

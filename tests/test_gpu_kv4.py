@@ -184,15 +184,15 @@ def test_decode_attention(D, G, heads, kv):
                 assert (np.abs(got[b, h] - ref) <= tol).all(), (b, h, float(np.abs(got[b, h] - ref).max()), float(tol.max()))
 
 
-@pytest.mark.parametrize("splits", [1, 2, 4, 8, 9, 37])
-def test_decode_attention_split_over_ctas(splits):
-    """A row's tiles split over a cluster or over the grid, also over more CTAs than it has tiles."""
+@pytest.mark.parametrize("ctas", [-1, 1, 2, 3, 7, 64, 1000])
+def test_decode_attention_dealt_to_ctas(ctas):
+    """The work dealt to one CTA, to a few whose stretches begin and end inside rows, to more than there are chunks, or by units."""
     import quant
     lib = quant.load_library()
     try:
-        lib.w4a16_tune_kv4(splits)
+        lib.w4a16_tune_kv4(ctas)
         for D, G, heads, kv, lens in ((128, 64, 4, 2, [0, 15, 16, 129, 700]), (64, 32, 20, 2, [333, 0, 1]), (128, 128, 1, 1, [1100])):
-            c = Case(lens, kv, heads, D, G, 32, seed=splits, rope=True, dead=(1,) if len(lens) == 3 else ())
+            c = Case(lens, kv, heads, D, G, 32, seed=abs(ctas), rope=True, dead=(1,) if len(lens) == 3 else ())
             d = c.device()
             for again in range(2):
                 out = quant.kv4_decode_attention(d["qkv"][:, 0], d["pool"], d["table"], d["pos"], heads, rope=d["rope"])
@@ -209,6 +209,24 @@ def test_decode_attention_split_over_ctas(splits):
                         assert (np.abs(got[b, h] - ref) <= tol).all(), (b, h, float(np.abs(got[b, h] - ref).max()), float(tol.max()))
     finally:
         lib.w4a16_tune_kv4(0)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.0])
+def test_decode_attention_scale(scale):
+    import quant
+    c = Case([70, 5], 2, 4, 64, 32, 16, seed=1)
+    d = c.device()
+    out = quant.kv4_decode_attention(d["qkv"][:, 0], d["pool"], d["table"], d["pos"], 4, scale=scale).double().cpu().numpy().reshape(2, 4, 64)
+    c.append()
+    for b in range(2):
+        for h in range(4):
+            ref, tol = c.attend(b, 0, h, chunk=False, scale=scale)
+            assert (np.abs(out[b, h] - ref) <= tol).all()
+    got = quant.kv4_attention(d["qkv"], d["pool"], d["table"], d["pos"], 4, scale=scale).double().cpu().numpy().reshape(2, 4, 64)
+    for b in range(2):
+        for h in range(4):
+            ref, tol = c.attend(b, 0, h, chunk=True, scale=scale)
+            assert (np.abs(got[b, h] - ref) <= tol).all()
 
 
 def test_decode_attention_keeps_nan():
