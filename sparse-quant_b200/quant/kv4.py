@@ -70,53 +70,95 @@ class _on:
             self.guard.__exit__(*exc)
 
 
+def _is(t, dtype, dims: int, device: int) -> bool:
+    """A contiguous CUDA tensor of this type, dimension number and device."""
+    return isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == dims and t.get_device() == device and t.is_contiguous()
+
+
+def _call_shape(x, x_dims, pool, table, pos, counts, rope, heads, row_parts):
+    """(B, S, N, device, pages, kv_heads, page_size, head_dim, group, heads, table width, cos, sin, rope rows) of a call on a layer's pool, all arguments
+    checked: x fp16 [B, (S,) N] with N at least heads + row_parts kv_heads head rows, or None (kv4_read).  One pass over the checks where
+    they hold - an eager call is host time -, the checks one by one, each with its message, where one does not."""
+    ref = pool if x is None else x
+    dev = ref.get_device() if isinstance(ref, torch.Tensor) and ref.is_cuda else -1
+    fmt = _FORMATS.get(pool.shape[-1]) if dev >= 0 and _is(pool, torch.uint8, 4, dev) and pool.numel() else None
+    if fmt is not None and _is(table, torch.int32, 2, dev) and _is(pos, torch.int32, 1, dev) and (x is None or _is(x, torch.float16, x_dims, dev)):
+        D, g = fmt
+        pages, kv, per, _ = pool.shape
+        B, width = table.shape
+        N = 0 if x is None else x.shape[-1]
+        heads = kv if x is None else int(heads)
+        ok = pos.shape[0] == B and heads > 0 and heads % kv == 0 and (x is None or x.shape[0] == B and N >= (heads + row_parts * kv) * D) and \
+            (counts is None or _is(counts, torch.int32, 1, dev) and counts.shape[0] == B)
+        if ok and rope is not None:
+            cos, sin = rope
+            ok = _is(cos, torch.float16, 2, dev) and _is(sin, torch.float16, 2, dev) and cos.shape == sin.shape and cos.shape[1] == D
+        if ok:
+            S = x.shape[1] if x_dims == 3 else 1
+            if rope is None:
+                return B, S, N, dev, pages, kv, 16 * per, D, g, heads, width, None, None, 0
+            return B, S, N, dev, pages, kv, 16 * per, D, g, heads, width, cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    if x is not None:
+        _check_tensor(x, "qkv", dtype=torch.float16, dims=x_dims)
+    pages, kv, page, D, g = _pool_shape(pool)
+    dev = pool.get_device()
+    _need(x is None or x.get_device() == dev, "all tensors must be on the same device")
+    heads = kv if x is None else int(heads)
+    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
+    _need(x is None or x.shape[-1] >= (heads + row_parts * kv) * D, f"qkv must have rows of at least (heads + {row_parts} kv_heads) * head_dim elements")
+    _ints(table, "table", dev, 2)
+    _need(x is None or table.shape[0] == x.shape[0], "table must have a row for every batch row")
+    _ints(pos, "pos", dev, numel=table.shape[0])
+    if counts is not None:
+        _ints(counts, "counts", dev, numel=table.shape[0])
+    return (table.shape[0], x.shape[1] if x_dims == 3 else 1, 0 if x is None else x.shape[-1], dev, pages, kv, page, D, g, heads, table.shape[1],
+            *_rope_args(rope, D, dev))
+
+
+def _output(out, shape, like):
+    if out is None:
+        return torch.zeros(shape, dtype=torch.float16, device=like.device)
+    if not (_is(out, torch.float16, len(shape), like.get_device()) and out.shape == shape):
+        _check_tensor(out, "out", dtype=torch.float16)
+        _need(tuple(out.shape) == shape and out.device == like.device, f"Tensor out must have shape {list(shape)}")
+    return out
+
+
+def _guarded(dev, fn, *args):
+    """fn on CUDA device `dev` with the current stream behind the arguments."""
+    if torch.cuda.current_device() == dev:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+
+
 def kv4_append(qkv, pool, table, pos, heads: int, rope=None, counts=None):
     """Keys and values of qkv fp16 [B, S, >= (heads + 2 kv_heads) * head_dim] into the pages of positions pos[b] ..: quantised to 4
     bits, keys rotated by `rope` = (cos, sin) fp16 [positions, head_dim] first.  pool: one layer's [pages, kv_heads, page_size / 16,
     tile bytes], updated in place; table int32 [B, width]; pos int32 [B], negative for a batch row without a sequence; counts int32 [B]
     tokens a row has of the S (None: all)."""
-    _check_tensor(qkv, "qkv", dtype=torch.float16, dims=3)
-    pages, kv, page, D, g = _pool_shape(pool)
-    dev, (B, S, N), heads = qkv.get_device(), qkv.shape, int(heads)
-    _need(pool.get_device() == dev, "all tensors must be on the same device")
-    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
-    _need(N >= (heads + 2 * kv) * D, "qkv must be [B, S, >= (heads + 2 kv_heads) * head_dim]")
-    _ints(table, "table", dev, 2)
-    _need(table.shape[0] == B, "table must have a row for every batch row")
-    _ints(pos, "pos", dev, numel=B)
-    if counts is not None:
-        _ints(counts, "counts", dev, numel=B)
-    cos, sin, rope_rows = _rope_args(rope, D, dev)
+    B, S, N, dev, pages, kv, page, D, g, heads, width, cos, sin, rope_rows = _call_shape(qkv, 3, pool, table, pos, counts, rope, heads, 2)
     if B == 0 or S == 0:
         return
-    lib = load_library()
-    with _on(dev):
-        st = lib.w4a16_kv4_append(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
-                                  None if counts is None else counts.data_ptr(), cos, sin, B, S, heads, kv, D, g, page, pages,
-                                  table.shape[1], N, rope_rows, _stream(qkv))
-    _check(st, "kv4_append")
+    st = _guarded(dev, load_library().w4a16_kv4_append, qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
+                  None if counts is None else counts.data_ptr(), cos, sin, B, S, heads, kv, D, g, page, pages, width, N, rope_rows)
+    if st:
+        _check(st, "kv4_append")
 
 
 def kv4_read(pool, table, pos, count: int, counts=None):
     """(k, v) fp16 [B, kv_heads, count, head_dim]: what the cache holds for positions pos[b] .. pos[b] + count - 1 (counts int32 [B]: only
     that many of them), zeros where the row has no sequence (pos < 0)."""
-    pages, kv, page, D, g = _pool_shape(pool)
-    dev, count = pool.get_device(), int(count)
-    _ints(table, "table", dev, 2)
-    B = table.shape[0]
-    _ints(pos, "pos", dev, numel=B)
-    if counts is not None:
-        _ints(counts, "counts", dev, numel=B)
+    B, _, _, dev, pages, kv, page, D, g, _, width, _, _, _ = _call_shape(None, 0, pool, table, pos, counts, None, 0, 0)
+    count = int(count)
     _need(count >= 0, "count must not be negative")
-    k = torch.empty((B, kv, count, D), dtype=torch.float16, device=pool.device)
-    v = torch.empty_like(k)
+    k, v = torch.empty((2, B, kv, count, D), dtype=torch.float16, device=pool.device).unbind()
     if B == 0 or count == 0:
         return k, v
-    lib = load_library()
-    with _on(dev):
-        st = lib.w4a16_kv4_read(pool.data_ptr(), table.data_ptr(), pos.data_ptr(), None if counts is None else counts.data_ptr(),
-                                k.data_ptr(), v.data_ptr(), B, count, kv, D, g, page, pages, table.shape[1], _stream(pool))
-    _check(st, "kv4_read")
+    st = _guarded(dev, load_library().w4a16_kv4_read, pool.data_ptr(), table.data_ptr(), pos.data_ptr(), None if counts is None else counts.data_ptr(),
+                  k.data_ptr(), v.data_ptr(), B, count, kv, D, g, page, pages, width)
+    if st:
+        _check(st, "kv4_read")
     return k, v
 
 
@@ -124,35 +166,19 @@ def kv4_decode_attention(qkv, pool, table, pos, heads: int, rope=None, scale=Non
     """One token step: the new token of every row (qkv fp16 [B, >= (heads + 2 kv_heads) * head_dim], position pos[b]) is appended to the
     4-bit cache and attends to positions 0 .. pos[b].  Returns fp16 [B, heads * head_dim]; rows with pos < 0 keep what `out` held
     (without `out`: zeros).  Other arguments as for kv4_append; scale defaults to head_dim ** -0.5."""
-    _check_tensor(qkv, "qkv", dtype=torch.float16, dims=2)
-    pages, kv, page, D, g = _pool_shape(pool)
-    dev, (B, N), heads = qkv.get_device(), qkv.shape, int(heads)
-    _need(pool.get_device() == dev, "all tensors must be on the same device")
-    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
-    _need(N >= (heads + 2 * kv) * D, "qkv must be [B, >= (heads + 2 kv_heads) * head_dim]")
-    _ints(table, "table", dev, 2)
-    _need(table.shape[0] == B, "table must have a row for every batch row")
-    _ints(pos, "pos", dev, numel=B)
-    cos, sin, rope_rows = _rope_args(rope, D, dev)
+    B, _, N, dev, pages, kv, page, D, g, heads, width, cos, sin, rope_rows = _call_shape(qkv, 2, pool, table, pos, None, rope, heads, 2)
     out = _output(out, (B, heads * D), qkv)
     if B == 0:
         return out
     lib = load_library()
-    with _on(dev):
-        ws_bytes = lib.w4a16_kv4_decode_workspace(B, heads, kv, D, page, table.shape[1])
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device) if ws_bytes else None
-        st = lib.w4a16_kv4_decode_attention(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(), cos, sin, out.data_ptr(),
-                                            None if ws is None else ws.data_ptr(), ws_bytes, B, heads, kv, D, g, page, pages, table.shape[1], N, rope_rows,
-                                            float(D ** -0.5 if scale is None else scale), _stream(qkv))
-    _check(st, "kv4_decode_attention")
-    return out
-
-
-def _output(out, shape, like):
-    if out is None:
-        return torch.zeros(shape, dtype=torch.float16, device=like.device)
-    _check_tensor(out, "out", dtype=torch.float16)
-    _need(tuple(out.shape) == shape and out.device == like.device, f"Tensor out must have shape {list(shape)}")
+    ws, ws_bytes = None, lib.w4a16_kv4_decode_workspace(B, heads, kv, D, page, width)
+    if ws_bytes:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
+    st = _guarded(dev, lib.w4a16_kv4_decode_attention, qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(), cos, sin, out.data_ptr(),
+                  None if ws is None else ws.data_ptr(), ws_bytes, B, heads, kv, D, g, page, pages, width, N, rope_rows,
+                  D ** -0.5 if scale is None else float(scale))
+    if st:
+        _check(st, "kv4_decode_attention")
     return out
 
 
@@ -161,27 +187,15 @@ def kv4_attention(qkv, pool, table, pos, heads: int, rope=None, scale=None, coun
     of row b stands at position pos[b] + i and attends to positions 0 .. pos[b] + i.  qkv fp16 [B, S, >= heads * head_dim], queries in
     front.  Returns fp16 [B, S, heads * head_dim]; queries past counts[b] and rows with pos < 0 keep what `out` held (without `out`:
     zeros)."""
-    _check_tensor(qkv, "qkv", dtype=torch.float16, dims=3)
-    pages, kv, page, D, g = _pool_shape(pool)
-    dev, (B, S, N), heads = qkv.get_device(), qkv.shape, int(heads)
-    _need(pool.get_device() == dev, "all tensors must be on the same device")
-    _need(heads > 0 and heads % kv == 0, "heads must be a multiple of the pool's kv_heads")
-    _need(N >= heads * D, "qkv must be [B, S, >= heads * head_dim]")
-    _ints(table, "table", dev, 2)
-    _need(table.shape[0] == B, "table must have a row for every batch row")
-    _ints(pos, "pos", dev, numel=B)
-    if counts is not None:
-        _ints(counts, "counts", dev, numel=B)
-    cos, sin, rope_rows = _rope_args(rope, D, dev)
+    B, S, N, dev, pages, kv, page, D, g, heads, width, cos, sin, rope_rows = _call_shape(qkv, 3, pool, table, pos, counts, rope, heads, 0)
     out = _output(out, (B, S, heads * D), qkv)
     if B == 0 or S == 0:
         return out
-    lib = load_library()
-    with _on(dev):
-        st = lib.w4a16_kv4_attention(qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
-                                     None if counts is None else counts.data_ptr(), cos, sin, out.data_ptr(), B, S, heads, kv, D, g, page,
-                                     pages, table.shape[1], N, rope_rows, float(D ** -0.5 if scale is None else scale), _stream(qkv))
-    _check(st, "kv4_attention")
+    st = _guarded(dev, load_library().w4a16_kv4_attention, qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
+                  None if counts is None else counts.data_ptr(), cos, sin, out.data_ptr(), B, S, heads, kv, D, g, page, pages, width, N, rope_rows,
+                  D ** -0.5 if scale is None else float(scale))
+    if st:
+        _check(st, "kv4_attention")
     return out
 
 

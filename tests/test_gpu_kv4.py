@@ -348,6 +348,58 @@ def test_chunk_attention(D, G, heads, kv, new, lens, counts):
                     assert (np.abs(got[b, i, h] - ref) <= tol).all(), (b, i, h, float(np.abs(got[b, i, h] - ref).max()), float(tol.max()))
 
 
+def test_chunk_attention_masked_values_that_are_not_finite():
+    """A value that is not finite reaches the queries that see its token, in the dims of its group, and no others; so does a key."""
+    import quant
+    D, heads = 128, 4
+    for what in ("v", "k"):
+        c = Case([150], 2, heads, D, 64, 16, seed=6, new=40)
+        at = 4 * D if what == "k" else 6 * D
+        c.qkv[0, 7, at + 3] = float("nan") if what == "k" else float("inf")     # token 157, head 0, the first group of dims
+        c.append()
+        d = c.device()
+        got = quant.kv4_attention(d["qkv"], d["pool"], d["table"], d["pos"], heads).view(40, heads, D).isnan().cpu()
+        want = torch.zeros_like(got)
+        want[7:, :2, :64 if what == "v" else D] = True
+        assert torch.equal(got, want), what
+        for i in (0, 6):
+            for h in range(heads):
+                ref, tol = c.attend(0, i, h, chunk=True)
+                out = quant.kv4_attention(d["qkv"], d["pool"], d["table"], d["pos"], heads).double().cpu().numpy().reshape(40, heads, D)
+                assert (np.abs(out[i, h] - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("heads,kv,S,ctx,counts", [(4, 1, 300, 700, None), (3, 3, 129, 0, None), (40, 8, 77, 500, [77, 5, 1, 64]), (32, 2, 1000, 30, [1000, 777])])
+def test_chunk_attention_long(heads, kv, S, ctx, counts):
+    """Several blocks of rows and steps of tokens, checked with torch in float64 on what the cache reads back to."""
+    import quant
+    D, G, P, B = 128, 64, 64, 1 if counts is None else len(counts)
+    g = torch.Generator(device="cuda").manual_seed(S)
+    need = (ctx + S) // P + 1
+    pool = quant.kv4_pool(1, B * need, kv, D, P, G)
+    table = torch.randperm(B * need, device="cuda", generator=g).int().view(B, -1)
+    x = torch.randn(B, ctx + S, (heads + 2 * kv) * D, device="cuda", generator=g).half()
+    zero = torch.zeros(B, dtype=torch.int32, device="cuda")
+    cnt = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda")
+    quant.kv4_append(x, pool[0], table, zero, heads, counts=None if cnt is None else cnt + ctx)
+    pos = zero + ctx
+    out = quant.kv4_attention(x[:, ctx:].contiguous(), pool[0], table, pos, heads, counts=cnt).double().view(B, S, heads, D)
+    k, v = quant.kv4_read(pool[0], table, zero, ctx + S, counts=None if cnt is None else cnt + ctx)
+    for b in range(B):
+        n = S if counts is None else counts[b]
+        q = x[b, ctx:ctx + n, :heads * D].view(n, heads, D).transpose(0, 1).double()
+        kk, vv = (t[b, :, :ctx + n].double().repeat_interleave(heads // kv, 0) for t in (k, v))
+        sc = (q @ kk.transpose(1, 2)) * D ** -0.5
+        sc.masked_fill_(torch.arange(ctx + n, device="cuda") > torch.arange(ctx, ctx + n, device="cuda").unsqueeze(1), -float("inf"))
+        ref = (torch.softmax(sc, -1) @ vv).transpose(0, 1)
+        # as at the head of this file; keys and values as the kernel rounds them, read back
+        X = float((q.abs() @ kk.abs().transpose(1, 2)).max()) * D ** -0.5
+        tol = float(vv.abs().max()) * (2 * X * (D * 2.0 ** -23 + 2.0 ** -11) + 4 * 2.0 ** -11 + (ctx + n) * 2.0 ** -24) + 2.0 ** -11 * ref.abs()
+        assert ((out[b, :n] - ref).abs() <= tol).all(), float((out[b, :n] - ref).abs().max())
+        assert float((out[b, :n] - ref).norm() / ref.norm()) <= 2e-3            # and far closer on average: rounding errors of both signs
+        assert not out[b, n:].any()
+
+
 def test_chunk_attention_takes_queries_alone():
     """Rows of heads * head_dim elements: the queries without keys and values behind them."""
     import quant
