@@ -1,0 +1,55 @@
+"""The paged 4-bit key/value cache of a decoder stack: the pool of all layers, the rows' page tables, lengths and the pages' reference
+counts, all on the device (the operations are quant.kv4_*)."""
+from __future__ import annotations
+
+import torch
+
+from quant import kv4_compact, kv4_fork, kv4_free, kv4_pool, kv4_reserve
+
+
+class PagedCache:
+    def __init__(self, layers, rows, max_len, kv_heads, head_dim, page_size=64, group=64, pages=None, heads=None,
+                 device="cuda"):
+        """Room for `rows` sequences of up to max_len tokens; `pages` of the pool (default: all rows at their longest, none shared);
+        `heads`: query heads (default: as many as key/value heads)."""
+        width = -(-int(max_len) // page_size)
+        self.page_size = page_size
+        self.pool = kv4_pool(layers, rows * width if pages is None else pages, kv_heads, head_dim, page_size, group, device)
+        self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(self.pool.shape[1], dtype=torch.int32, device=device)
+        # the token steps' attention output, for all layers: rows without a sequence keep zeros
+        self.out = torch.zeros((rows, (heads or kv_heads) * head_dim), dtype=torch.float16, device=device)
+        self._pos = torch.zeros(rows, dtype=torch.int32, device=device)
+
+    def reserve(self, counts):
+        """Room for counts[r] more tokens of every row; returns the positions they start at (-1: none asked for, or no room)."""
+        return kv4_reserve(self.table, self.lens, self.refs, counts.to(torch.int32), self.page_size)
+
+    def reserve_rows(self, tokens: int):
+        return self.reserve(torch.full_like(self.lens, tokens))
+
+    def fork(self, src, dst):
+        """Rows dst (empty) continue rows src."""
+        kv4_fork(self.pool, self.table, self.lens, self.refs, src, dst)
+
+    def free(self, rows):
+        """The rows give their pages back."""
+        kv4_free(self.table, self.lens, self.refs, rows)
+
+    def compact(self):
+        """The pages in use become the pool's first ones."""
+        kv4_compact(self.pool, self.table, self.refs)
+
+    def positions(self, pos_t):
+        """The position in the one-element int64 tensor pos_t for every row, int32, at a fixed address."""
+        self._pos.copy_(pos_t.expand(self._pos.shape[0]))
+        return self._pos
+
+    def rows(self, a: int, b: int) -> "PagedCache":
+        """This cache seen through rows a .. b - 1 only (the same pool and tables; its own output and positions)."""
+        view = object.__new__(PagedCache)
+        view.page_size, view.pool, view.refs = self.page_size, self.pool, self.refs
+        view.table, view.lens = self.table[a:b], self.lens[a:b]
+        view.out, view._pos = torch.zeros_like(self.out[a:b]), torch.zeros_like(self._pos[a:b])
+        return view

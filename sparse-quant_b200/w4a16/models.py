@@ -47,6 +47,11 @@ class DecoderConfig:
     # the block outputs (5 launches per layer); False keeps them as separate add+norm launches (7 per layer)
     fold_norms: bool = True
     fold_norms_max_batch: int = 4
+    # 4: keys and values are held in 4 bits, in pages (kv4.PagedCache; GPU only) - a quarter of what the token step reads of a
+    # long context, and rows that share a prefix share its pages; 16: the static fp16 cache
+    kv_bits: int = 16
+    kv_group: int = 64                # dims of a head that share a step and a minimum
+    kv_page: int = 64                 # tokens of a page
 
     @staticmethod
     def opt_6_7b():
@@ -139,6 +144,7 @@ class DecoderLayer(nn.Module):
             self.ln2 = source.norm(idx, "ln2", RMSNorm(H, cfg.rms_eps, device))
             self.fc2 = RowParallelWALinear(source.linear(idx, "down_proj", cfg.ffn, H), rank, world, group, ranges=ffn_ranges, exchange=exchange)
         self.k_cache = self.v_cache = None
+        self.idx = idx
 
     def alloc_cache(self, batch, max_len, device):
         shape = (batch, self.local_heads, max_len, self.head_dim)
@@ -196,11 +202,10 @@ def _norm_as_built(norm, x) -> bool:
     return w is not None and _halves(w) and w.numel() == x.shape[-1] and (b is None or _halves(b)) and w.device == x.device
 
 
-def _kernels_apply(layer, x, pos0: int, rope) -> bool:
-    """Whether _layer_forward_kernels stands for the op-by-op body of DecoderLayer.forward: on the GPU, with sizes the
-    kernels take, the modules it reads or hands epilogues to still the ones the layer was built with and without hooks
-    (they are not called one by one there), caches and tables in the layout the kernels write and read, no gradient."""
-    B, S, H = x.shape
+def _modules_as_built(layer, x) -> bool:
+    """Whether the library's kernels can stand for a decoder layer's modules: on the GPU, with sizes they take, the modules still the ones
+    the layer was built with and without hooks, no gradient."""
+    H = x.shape[-1]
     if not (x.is_cuda and H <= 8192 and H % 8 == 0 and layer.head_dim % 16 == 0 and x.dtype == torch.float16):
         return False
     if torch.is_grad_enabled() and x.requires_grad:
@@ -213,6 +218,16 @@ def _kernels_apply(layer, x, pos0: int, rope) -> bool:
             _as_built(m["fc2"], RowParallelWALinear) and _as_built(m["fc2"].linear, WALinear) and
             (_as_built(m["gate_up_proj"], WALinear) if fc1 is None else _as_built(fc1, ColumnParallelWALinear) and _as_built(fc1.linear, WALinear)) and
             _norm_as_built(m["ln1"], x) and _norm_as_built(m["ln2"], x)):
+        return False
+    return True
+
+
+def _kernels_apply(layer, x, pos0: int, rope) -> bool:
+    """Whether _layer_forward_kernels stands for the op-by-op body of DecoderLayer.forward: on the GPU, with sizes the
+    kernels take, the modules it reads or hands epilogues to still the ones the layer was built with and without hooks
+    (they are not called one by one there), caches and tables in the layout the kernels write and read, no gradient."""
+    B, S, H = x.shape
+    if not _modules_as_built(layer, x):
         return False
     k, v = layer.k_cache, layer.v_cache
     if not (_halves(k) and _halves(v) and k.device == v.device == x.device and k.shape == v.shape == (B, layer.local_heads, k.shape[2], layer.head_dim) and
@@ -259,6 +274,43 @@ def _layer_forward_kernels(self, x, pos0: int, rope=None):
 DecoderLayer._forward_kernels = _layer_forward_kernels
 
 
+def _layer_forward_kv4(self, x, pos, kv, rope=None):
+    """A prompt, or the next chunk of one, over the paged 4-bit cache `kv` (kv4.PagedCache): row b's tokens stand at pos[b] .. (int32 on
+    the device).  Keys and values are appended first and attention reads all of them, the chunk's own among them, from the cache, as the
+    token step does.  `rope`: the (cos, sin) tables over all positions, or None."""
+    from quant import RELU_KEEPS_NAN, add_norm, kv4_append, kv4_attention, silu_mul_tiles
+    B, S, H = x.shape
+    heads, pool = self.local_heads, kv.pool[self.idx]
+    built = _modules_as_built(self, x)
+    fold = built and B * S >= 256                                    # as in _layer_forward_kernels
+    x = x if x.is_contiguous() else x.contiguous()
+    qkv = self.qkv_proj(add_norm(x, None, *_norm_args(self.ln1))[1] if built else self.ln1(x))
+    kv4_append(qkv, pool, kv.table, pos, heads, rope=rope)
+    a = kv4_attention(qkv, pool, kv.table, pos, heads, rope=rope)
+    if fold:
+        x = self.out_proj(a, residual=x)
+        _, h = add_norm(x, None, *_norm_args(self.ln2))
+    elif built:
+        x, h = add_norm(x, self.out_proj(a), *_norm_args(self.ln2))
+    else:
+        x = x + self.out_proj(a)
+        h = self.ln2(x)
+    if self.cfg.kind == "opt":
+        h = h.reshape(1, B * S, H)
+        f = self.fc1(h, relu=RELU_KEEPS_NAN) if fold and self.fc1.linear.group_size != 32 else torch.relu(self.fc1(h))
+    elif built:
+        f = silu_mul_tiles(self.gate_up_proj(h))
+    else:
+        gate, up = split_gate_up(self.gate_up_proj(h))
+        f = F.silu(gate) * up
+    if fold:
+        return self.fc2(f, residual=x.view(f.shape[:-1] + (H,))).view(B, S, H)
+    return x + self.fc2(f).reshape(B, S, H)
+
+
+DecoderLayer._forward_kv4 = _layer_forward_kv4
+
+
 def _norm_args(norm):
     """(weight, bias, eps, rms) of an nn.LayerNorm or RMSNorm, as quant.add_norm takes them."""
     if isinstance(norm, RMSNorm):
@@ -266,7 +318,15 @@ def _norm_args(norm):
     return norm.weight, norm.bias, norm.eps, False
 
 
-def _layer_forward_static(self, x, pos_t, rope, stats=None):
+def _token_attention(self, qkv, pos_t, rope, kv):
+    """Attention of one new token a row over the static cache, or over the paged 4-bit cache `kv` (pos_t: int32 positions by row)."""
+    from quant import decode_attention, kv4_decode_attention
+    if kv is None:
+        return decode_attention(qkv, self.k_cache, self.v_cache, pos_t, self.local_heads, rope=rope)
+    return kv4_decode_attention(qkv, kv.pool[self.idx], kv.table, pos_t, self.local_heads, rope=rope, out=kv.out)
+
+
+def _layer_forward_static(self, x, pos_t, rope, stats=None, kv=None):
     """One-token step with the position held in a device tensor (fixed shapes: capturable in a CUDA graph).
     `x` is the residual stream [B, 1, H].  With cfg.fold_norms and up to 16 sequences a layer is five launches: both
     residual adds run in the epilogue of the GEMV that produces the block's output (after the cross-rank sum under
@@ -274,13 +334,14 @@ def _layer_forward_static(self, x, pos_t, rope, stats=None):
     inside the GEMV that consumes them, from those statistics.  `stats` = (buffer holding the statistics of x or None,
     buffer for the attention block's output, buffer for this layer's output).  The fused q/k/v GEMV feeds the decode
     attention kernel, which also appends to the cache and applies the rotary embedding (`rope` = the full (cos, sin)
-    tables or None).  Returns the new residual stream."""
-    from quant import add_norm, decode_attention, silu_mul_tiles
+    tables or None).  kv: the paged 4-bit cache (kv4.PagedCache) instead of the layer's static one; pos_t then holds int32
+    positions by row.  Returns the new residual stream."""
+    from quant import add_norm, silu_mul_tiles
     B, S, H = x.shape
     if stats is None:
         _, h = add_norm(x, None, *_norm_args(self.ln1))
         qkv = self.qkv_proj(h).view(B, -1)
-        a = decode_attention(qkv, self.k_cache, self.v_cache, pos_t, self.local_heads, rope=rope).view(B, 1, -1)
+        a = _token_attention(self, qkv, pos_t, rope, kv).view(B, 1, -1)
         x, h = add_norm(x, self.out_proj(a), *_norm_args(self.ln2))
         if self.cfg.kind == "opt":
             f = self.fc1(h.reshape(1, B, H), relu=True)
@@ -291,7 +352,7 @@ def _layer_forward_static(self, x, pos_t, rope, stats=None):
         return self.fc2(f, residual=x.reshape(f.shape[:-1] + (H,))).reshape(B, 1, H)
     s_in, s_mid, s_out = stats
     qkv = self.qkv_proj(x, pre_norm=(*_norm_args(self.ln1), s_in)).view(B, -1)
-    a = decode_attention(qkv, self.k_cache, self.v_cache, pos_t, self.local_heads, rope=rope).view(B, 1, -1)
+    a = _token_attention(self, qkv, pos_t, rope, kv).view(B, 1, -1)
     x = self.out_proj(a, residual=x, stats_out=s_mid)
     ln2 = (*_norm_args(self.ln2), s_mid)
     if self.cfg.kind == "opt":
@@ -340,6 +401,9 @@ class Decoder(nn.Module):
         self.lm_head = head_full[v0:v1].contiguous()
         self.layers = nn.ModuleList(DecoderLayer(cfg, i, rank, world, group, device, source, exchange) for i in range(cfg.layers))
         self.pos = 0
+        self.kv4 = None                   # the paged cache, where cfg.kv_bits is 4 (made by reset)
+        if cfg.kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 16 or 4")
 
     def mark_static(self):
         """Call once the weights are in place and the device is synchronised (enables weight prefetch)."""
@@ -350,24 +414,24 @@ class Decoder(nn.Module):
         return self
 
     def reset(self, batch, max_len):
-        for layer in self.layers:
-            layer.alloc_cache(batch, max_len, self.device)
+        if self.cfg.kv_bits == 4:
+            self._new_kv4(batch, max_len).reserve_rows(max_len)
+        else:
+            for layer in self.layers:
+                layer.alloc_cache(batch, max_len, self.device)
         self.pos = 0
 
-    @torch.no_grad()
-    def forward(self, ids):
-        """ids [B, S] -> logits of the last position [B, vocab] (fp16); advances the KV cache by S."""
-        B, S = ids.shape
-        x = self.embed[ids]
-        rope = None
-        if self.cfg.kind == "opt":
-            x = x + self.pos_embed[self.pos + 2:self.pos + 2 + S]
-        else:
-            rope = (self.rope_cos[self.pos:self.pos + S], self.rope_sin[self.pos:self.pos + S])
-        for layer in self.layers:
-            x = layer(x, self.pos, rope)
-        self.pos += S
-        h = x[:, -1]
+    def _new_kv4(self, rows, max_len, pages=None):
+        from .kv4 import PagedCache
+        cfg = self.cfg
+        if self.device.type != "cuda" or (cfg.hidden // cfg.heads) not in (64, 128) or cfg.hidden > 8192 or cfg.hidden % 8:
+            raise RuntimeError("kv_bits = 4 needs a GPU, heads of 64 or 128 dims and a hidden size of at most 8192")
+        self.kv4 = PagedCache(cfg.layers, rows, max_len, cfg.heads // self.world, cfg.hidden // cfg.heads, page_size=cfg.kv_page,
+                              group=cfg.kv_group, pages=pages, device=self.device)
+        return self.kv4
+
+    def _final_logits(self, h):
+        """fp16 logits of the hidden states [B, hidden], all of the vocabulary on every rank."""
         if h.is_cuda and h.dtype == torch.float16 and h.shape[-1] <= 8192 and h.shape[-1] % 8 == 0 and \
                 _norm_as_built(self.final_norm, h) and not _global_hooks():
             from quant import add_norm
@@ -377,10 +441,44 @@ class Decoder(nn.Module):
         logits = h @ self.lm_head.t()
         if self.world > 1:
             sizes = [b - a for a, b in self.vocab_ranges]
-            parts = [torch.empty((B, n), dtype=logits.dtype, device=logits.device) for n in sizes]
+            parts = [torch.empty((h.shape[0], n), dtype=logits.dtype, device=logits.device) for n in sizes]
             dist.all_gather(parts, logits.contiguous(), group=self.group)
             logits = torch.cat(parts, dim=-1)
         return logits
+
+    @torch.no_grad()
+    def forward_kv4(self, ids, pos, start: int):
+        """ids [B, S] at positions start .. start + S - 1 of the paged cache's rows (pos: the same int32 [B] on the device, negative for
+        rows to be left alone) -> logits of the last position [B, vocab]."""
+        S = ids.shape[1]
+        x = self.embed[ids]
+        rope = None
+        if self.cfg.kind == "opt":
+            x = x + self.pos_embed[start + 2:start + 2 + S]
+        else:
+            rope = (self.rope_cos, self.rope_sin)
+        for layer in self.layers:
+            x = layer._forward_kv4(x, pos, self.kv4, rope)
+        return self._final_logits(x[:, -1])
+
+    @torch.no_grad()
+    def forward(self, ids):
+        """ids [B, S] -> logits of the last position [B, vocab] (fp16); advances the KV cache by S."""
+        B, S = ids.shape
+        if self.cfg.kv_bits == 4:
+            logits = self.forward_kv4(ids, torch.full((B,), self.pos, dtype=torch.int32, device=ids.device), self.pos)
+            self.pos += S
+            return logits
+        x = self.embed[ids]
+        rope = None
+        if self.cfg.kind == "opt":
+            x = x + self.pos_embed[self.pos + 2:self.pos + 2 + S]
+        else:
+            rope = (self.rope_cos[self.pos:self.pos + S], self.rope_sin[self.pos:self.pos + S])
+        for layer in self.layers:
+            x = layer(x, self.pos, rope)
+        self.pos += S
+        return self._final_logits(x[:, -1])
 
     @torch.no_grad()
     def step_static(self, tok, pos_t, arange):
@@ -400,14 +498,17 @@ class Decoder(nn.Module):
         if fold and self._row_stats is None:
             from quant import row_stats_buffer
             self._row_stats = tuple(row_stats_buffer(self.cfg.hidden, x.device) for _ in range(2))
+        kv, at = self.kv4, pos_t
+        if kv is not None:
+            at = kv.positions(pos_t)                     # the same position in every row, as the kernel reads them: int32 by row
         have = False                                     # the first layer's input comes from the embedding: no statistics
         for layer in self.layers:
             if fold:
                 mid, out = self._row_stats
-                x = layer.forward_static(x, pos_t, rope, (out if have else None, mid, out))
+                x = layer.forward_static(x, at, rope, (out if have else None, mid, out), kv)
                 have = True
             else:
-                x = layer.forward_static(x, pos_t, rope)
+                x = layer.forward_static(x, at, rope, None, kv)
         _, h = add_norm(x, None, *_norm_args(self.final_norm))
         logits = h[:, -1] @ self.lm_head.t()
         if self.world > 1 and self.exchange is not None:
@@ -495,3 +596,42 @@ class Decoder(nn.Module):
         sync()
         t2 = time.perf_counter()
         return torch.cat(out, dim=1), t1 - t0, t2 - t1
+
+    @torch.no_grad()
+    def generate_shared(self, prefix_ids, suffix_ids, new_tokens: int):
+        """Greedy decoding of B prompts that begin alike (kv_bits = 4): prefix_ids [1, S0] runs through the model once, the B rows continue
+        it - its pages are shared, the last, partly filled one is copied -, then suffix_ids [B, S1] and the token steps run on all rows.
+        Returns tokens [B, new_tokens].  The rows' pages are given back at the end; `kv4.compact()` then leaves the prefix in front."""
+        if self.cfg.kv_bits != 4:
+            raise RuntimeError("generate_shared needs kv_bits = 4")
+        S0, (B, S1) = prefix_ids.shape[1], suffix_ids.shape
+        if prefix_ids.shape[0] != 1 or S0 < 1 or S1 < 1 or new_tokens < 1:
+            raise RuntimeError("prefix_ids must be [1, S0], suffix_ids [B, S1] with at least one token each")
+        page, dev = self.cfg.kv_page, self.device
+        own = (S0 % page + S1 + new_tokens + page - 1) // page        # pages a row needs for itself: the copied one and what follows
+        kv = self._new_kv4(B + 1, S0 + S1 + new_tokens, pages=(S0 + page - 1) // page + B * own)
+        rows = torch.arange(B + 1, dtype=torch.int32, device=dev)     # row B holds the prefix
+        pos = kv.reserve((rows == B) * S0)
+        self._on_row(B).forward_kv4(prefix_ids, pos[B:], 0)
+        kv.fork(torch.full((B,), B, dtype=torch.int32, device=dev), rows[:B])
+        pos = kv.reserve((rows < B) * (S1 + new_tokens))
+        full, self.kv4 = kv, kv.rows(0, B)
+        try:
+            tok = self.forward_kv4(suffix_ids, pos[:B], S0).argmax(-1, keepdim=True)
+            out = [tok]
+            pos_t = torch.full((1,), S0 + S1, dtype=torch.long, device=dev)
+            for _ in range(new_tokens - 1):
+                tok = self.step_static(tok, pos_t, None)
+                out.append(tok)
+        finally:
+            self.kv4 = full
+        kv.free(rows[:B])
+        self.pos = S0
+        return torch.cat(out, dim=1)
+
+    def _on_row(self, row: int):
+        """This decoder on one row of its paged cache."""
+        import copy
+        one = copy.copy(self)
+        one.kv4 = self.kv4.rows(row, row + 1)
+        return one

@@ -170,3 +170,13 @@ def test_oracle_pages():
     want = pool[:, 4].copy()
     kv4.compact(pool, table, refs)
     assert table[1] == [0, 1, -1] and refs == [1, 1, 0, 0, 0, 0] and (pool[:, 1] == want).all()
+
+
+def test_decoder_on_the_host_refuses_the_paged_cache():
+    from w4a16.models import Decoder, DecoderConfig
+    cfg = DecoderConfig("opt", layers=1, hidden=256, heads=4, ffn=512, vocab=64, group_size=128, max_positions=32, kv_bits=4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        Decoder(cfg, device="cpu", seed=1).reset(1, 8)
+    cfg.kv_bits = 8
+    with pytest.raises(ValueError):
+        Decoder(cfg, device="cpu", seed=1)
