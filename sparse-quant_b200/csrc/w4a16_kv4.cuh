@@ -68,34 +68,50 @@ struct Cache {
     }
 };
 
-// Eight dims of a row from a quantisation group spread over `lanes` adjacent lanes: (s, m) of the group and the eight codes.
-// Every step is one IEEE fp32 operation, so the codes are the same integers that elementary tensor operations give.
-__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], int lanes, __half2& par)
+// Eight dims of a row (fp16, packed) from a quantisation group spread over `lanes` adjacent lanes: (s, m) of the group and the eight
+// codes.  Minimum and maximum travel as one pair (lo, -hi).  A code is d = x - m over s rounded to the nearest integer, ties to even:
+// d times the rounded reciprocal, rounded by adding 1.5 2^23 in the same operation, is right except next to the half-way points, where
+// the remainder d - n s (exact: it has few bits) tells.  Eight IEEE divisions and conversions took 60 % of the append kernel's time.
+__device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half2& par)
 {
-    float lo = x[0], hi = x[0];
-    bool odd = !(fabsf(x[0]) <= 65504.f);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        odd |= !(fabsf(x[i]) <= 65504.f);
-    }
-    int any = odd;
-    for (int o = 1; o < lanes; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        any |= __shfl_xor_sync(0xffffffffu, any, o);
-    }
-    const __half sh = any ? __ushort_as_half(0x7fff) : __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+    const __half2* x = reinterpret_cast<const __half2*>(&x8);
+    const __half2 lo2 = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
+    const __half2 hi2 = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+    __half2 ends = __halves2half2(__hmin_nan(__low2half(lo2), __high2half(lo2)), __hneg(__hmax_nan(__low2half(hi2), __high2half(hi2))));
+    for (int o = 1; o < lanes; o <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+    const float lo = __low2float(ends), hi = -__high2float(ends);
+    const bool finite = fabsf(lo) <= 65504.f && fabsf(hi) <= 65504.f;           // (a NaN anywhere is one here)
+    const __half sh = finite ? __float2half_rn(__fdiv_rn(hi - lo, 15.f)) : __ushort_as_half(0x7fff);
+    par = __halves2half2(sh, __low2half(ends));
     const float s = __half2float(sh);
-    par = __halves2half2(sh, __float2half_rn(lo));
-    uint32_t word = 0;
-    if (s > 0.f) {                                                              // not at s = 0 (all values m) and NaN
+    if (!(s > 0.f)) return 0;                                                   // all values m, or not finite
+    constexpr float kMagic = 12582912.f;                                        // 1.5 * 2^23: an integer's last bits are the float's
+    const float r = __frcp_rn(s);
+    float d[8], t[8];
+    bool near = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            word |= (uint32_t)fminf(rintf(__fdiv_rn(__fsub_rn(x[i], lo), s)), 15.f) << (4 * i);
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(x[e]);
+        d[2 * e] = f.x - lo;
+        d[2 * e + 1] = f.y - lo;
     }
-    return word;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        t[i] = fminf(fmaf(d[i], r, kMagic), kMagic + 15.f);
+        near |= 2.f * fabsf(fmaf(kMagic - t[i], s, d[i])) >= s;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float rem = fmaf(kMagic - t[i], s, d[i]), two = 2.f * fabsf(rem);
+            if (two > s || (two == s && (__float_as_int(t[i]) & 1))) t[i] += rem > 0.f ? 1.f : -1.f;
+            t[i] = fminf(t[i], kMagic + 15.f);
+        }
+    }
+    uint32_t word = 0;                                                          // (modulo 2^32: the float's other bits come off at the end)
+#pragma unroll
+    for (int i = 7; i >= 0; --i) word = word * 16u + __float_as_uint(t[i]);
+    return word - 0x4b400000u * 0x11111111u;
 }
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
@@ -112,18 +128,27 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
 // Word w (dims 8w .. 8w+7) of a head row at `src` with the rotary embedding of position t ("rotate half"), rounded to fp16 as the
 // fp16 cache holds keys; fp32 products and sum, each rounded.
 template <int D>
-__device__ __forceinline__ void load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t, float (&x)[8])
+__device__ __forceinline__ uint4 load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t)
 {
-    unpack8(*reinterpret_cast<const uint4*>(src + 8 * w), x);
-    if (!cos) return;
-    float y[8], c[8], s[8];
+    uint4 out = *reinterpret_cast<const uint4*>(src + 8 * w);
+    if (!cos) return out;
+    float x[8], y[8], c[8], s[8];
+    unpack8(out, x);
     unpack8(*reinterpret_cast<const uint4*>(src + 8 * (w ^ (D / 16))), y);
     unpack8(*reinterpret_cast<const uint4*>(cos + (size_t)t * D + 8 * w), c);
     unpack8(*reinterpret_cast<const uint4*>(sin + (size_t)t * D + 8 * w), s);
     const float sign = w < D / 16 ? -1.f : 1.f;
+    __half2* o = reinterpret_cast<__half2*>(&out);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = __half2float(__float2half_rn(__fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(sign * y[i], s[i]))));
+    for (int e = 0; e < 4; ++e)
+        o[e] = __floats2half2_rn(__fadd_rn(__fmul_rn(x[2 * e], c[2 * e]), __fmul_rn(sign * y[2 * e], s[2 * e])),
+                                 __fadd_rn(__fmul_rn(x[2 * e + 1], c[2 * e + 1]), __fmul_rn(sign * y[2 * e + 1], s[2 * e + 1])));
+    return out;
+}
+template <int D>
+__device__ __forceinline__ void load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t, float (&x)[8])
+{
+    unpack8(load_rotated<D>(src, w, cos, sin, t), x);
 }
 
 // Arguments every entry point with a pool checks alike; fills c.

@@ -33,56 +33,66 @@ struct AppendArgs {
     int* error;
     int seq, rope_rows;
     int key_at, val_at;           // first element of the keys and of the values in a token's row
+    int runs;                     // blocks of a (batch row, head)
     long long stride;
-    long long units;              // batch * kv heads * seq
 };
 
-// A (token, head) unit is 2 D/8 lanes: the first half take the key row's words of 8 dims, the others the value row's.  Tokens run
-// fastest, so that the 16 rows of a tile are written close together.  Bound: memory (reads 4 D bytes, writes tile bytes / 16).
+// A block takes one tile: the 16 positions 16 (p/16 + run) .. of one (batch row, head), of which those of the call are written.  D/8
+// adjacent lanes take a row's words of 8 dims; at D = 128 a thread takes a key row's word, then the value row's, at D = 64 half of the
+// warps take keys: no warp has both, since only keys are rotated.  One look at the page table a block.
+template <class F, int D>
+struct Block {
+    static constexpr int kEach = D / 64;                                        // rows' words of a thread
+    __device__ static __forceinline__ bool value(int k) { return kEach == 2 ? k == 1 : threadIdx.x >= 128; }
+    __device__ static __forceinline__ int token() { return threadIdx.x / F::NW % kTile; }
+};
+int runs_of(int seq) { return (seq + 2 * kTile - 2) / kTile; }                  // tiles that seq positions can touch
+
+// Bound: memory (reads 4 D bytes, writes tile bytes / 16 for a token and head).  8 x 2048 tokens, 8 heads of 128 in groups of 32, rotated:
+// 96 us with a division a value, 64-bit index arithmetic a thread, and keys and values in one warp.
 template <class F, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
 {
-    constexpr int kUnit = 2 * F::NW, kPer = 256 / kUnit;
-    const long long u = (long long)blockIdx.x * kPer + threadIdx.x / kUnit;
-    const int l = threadIdx.x % kUnit, w = l % F::NW;
-    const bool value = l >= F::NW;
-    bool live = u < a.units;
-    int s = 0, head = 0, b = 0, t = 0;
-    if (live) {
-        s = (int)(u % a.seq);
-        const long long bh = u / a.seq;
-        head = (int)(bh % a.c.kv_heads);
-        b = (int)(bh / a.c.kv_heads);
-        const int p = a.pos[b];
-        live = p >= 0 && (!a.counts || s < a.counts[b]);
-        if (live && (p > a.c.capacity() || p + s >= a.c.capacity() || (a.cos && p + s >= a.rope_rows))) {
-            live = false;
-            atomicExch(a.error, kErrPosition);
-        }
-        t = p + s;
+    using B = Block<F, D>;
+    const int run = blockIdx.x % a.runs, bh = blockIdx.x / a.runs, head = bh % a.c.kv_heads, b = bh / a.c.kv_heads;
+    const int p = a.pos[b], count = p < 0 ? 0 : min(a.counts ? a.counts[b] : a.seq, a.seq);
+    const int room = min(a.c.capacity(), a.cos ? a.rope_rows : 0x7fffffff);
+    const int s_first = run * kTile - (p & 15);                                 // of the tile's first position
+    if (s_first >= count || count <= 0) return;
+    if (p >= room || s_first >= room - p) {                                     // all of the tile's tokens are outside
+        if (threadIdx.x == 0) atomicExch(a.error, kErrPosition);
+        return;
     }
-    unsigned char* tile = nullptr;
-    if (live) {
-        tile = a.c.tile(b, head, t, F::kBytes);
-        if (!tile) atomicExch(a.error, kErrPage);
+    unsigned char* tile = a.c.tile(b, head, p + max(s_first, 0), F::kBytes);
+    if (!tile) {
+        if (threadIdx.x == 0) atomicExch(a.error, kErrPage);
+        return;
     }
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (tile) {
-        const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + (value ? a.val_at : a.key_at) + head * D;
-        load_rotated<D>(row, w, value ? nullptr : a.cos, a.sin, t, x);
+    const int w = threadIdx.x % F::NW, r = B::token(), s = s_first + r;
+    const bool mine = s >= 0 && s < count && s < room - p;
+    if (s >= room - p && s < count) atomicExch(a.error, kErrPosition);
+    uint4 x[B::kEach];
+    const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + head * D;
+#pragma unroll
+    for (int k = 0; k < B::kEach; ++k) {
+        const bool value = B::value(k);
+        x[k] = make_uint4(0, 0, 0, 0);
+        if (mine) x[k] = load_rotated<D>(row + (value ? a.val_at : a.key_at), w, value ? nullptr : a.cos, a.sin, p + s);
     }
     constexpr int kLanes = D / F::NG / 8;                                       // lanes of a group
-    __half2 par;
-    const uint32_t word = quantize8(x, kLanes, par);                            // (all lanes: shuffles)
-    if (!tile) return;
-    const int r = t & 15;
-    if (!value) {
-        *reinterpret_cast<uint32_t*>(tile + F::key_word(r, w)) = word;
-    } else {
-        *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w)) = (uint16_t)word;
-        *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w + 1)) = (uint16_t)(word >> 16);
+#pragma unroll
+    for (int k = 0; k < B::kEach; ++k) {
+        __half2 par;
+        const uint32_t word = quantize8(x[k], kLanes, par);                     // (all lanes: shuffles)
+        if (!mine) continue;
+        if (!B::value(k)) {
+            *reinterpret_cast<uint32_t*>(tile + F::key_word(r, w)) = word;
+        } else {
+            *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w)) = (uint16_t)word;
+            *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w + 1)) = (uint16_t)(word >> 16);
+        }
+        if (w % kLanes == 0) *reinterpret_cast<__half2*>(tile + (B::value(k) ? F::val_par(r, w / kLanes) : F::key_par(r, w / kLanes))) = par;
     }
-    if (w % kLanes == 0) *reinterpret_cast<__half2*>(tile + (value ? F::val_par(r, w / kLanes) : F::key_par(r, w / kLanes))) = par;
 }
 
 struct ReadArgs {
@@ -92,49 +102,58 @@ struct ReadArgs {
     __half* k;
     __half* v;
     int* error;
-    int seq;
-    long long units;
+    int seq, runs;
 };
 
-// The same units as append_kernel; out [batch][kv heads][seq][D], zeros where a row has no such token.
+// The same blocks; out [batch][kv heads][seq][D], zeros where a row has no such token.  (A row without a sequence is walked as if it stood
+// at position 0.)
 template <class F, int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a)
 {
-    constexpr int kUnit = 2 * F::NW, kPer = 256 / kUnit;
-    const long long u = (long long)blockIdx.x * kPer + threadIdx.x / kUnit;
-    const int l = threadIdx.x % kUnit, w = l % F::NW;
-    const bool value = l >= F::NW;
-    if (u >= a.units) return;
-    const int s = (int)(u % a.seq);
-    const long long bh = u / a.seq;
-    const int head = (int)(bh % a.c.kv_heads), b = (int)(bh / a.c.kv_heads);
-    const int p = a.pos[b];
+    using B = Block<F, D>;
+    const int run = blockIdx.x % a.runs, bh = blockIdx.x / a.runs, head = bh % a.c.kv_heads, b = bh / a.c.kv_heads;
+    const int p = max(a.pos[b], 0), count = a.pos[b] < 0 ? 0 : min(a.counts ? a.counts[b] : a.seq, a.seq), room = a.c.capacity();
+    const int s_first = run * kTile - (p & 15);
+    if (s_first >= a.seq) return;
     const unsigned char* tile = nullptr;
-    if (p >= 0 && (!a.counts || s < a.counts[b])) {
-        if (p > a.c.capacity() || p + s >= a.c.capacity()) {
-            atomicExch(a.error, kErrPosition);
+    if (s_first < count) {
+        if (p >= room || s_first >= room - p) {
+            if (threadIdx.x == 0) atomicExch(a.error, kErrPosition);
         } else {
-            tile = a.c.tile(b, head, p + s, F::kBytes);
-            if (!tile) atomicExch(a.error, kErrPage);
+            tile = a.c.tile(b, head, p + max(s_first, 0), F::kBytes);
+            if (!tile && threadIdx.x == 0) atomicExch(a.error, kErrPage);
         }
     }
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (tile) {
-        const int r = (p + s) & 15, g = w * 8 * F::NG / D;
-        uint32_t word;
-        if (!value) {
-            word = *reinterpret_cast<const uint32_t*>(tile + F::key_word(r, w));
+    const int w = threadIdx.x % F::NW, r = B::token(), s = s_first + r, g = w * 8 * F::NG / D;
+    if (s < 0 || s >= a.seq) return;
+    const bool mine = tile && s < count && s < room - p;
+    if (tile && s < count && s >= room - p) atomicExch(a.error, kErrPosition);
+    uint32_t word[B::kEach];
+    __half2 par[B::kEach];
+#pragma unroll
+    for (int k = 0; k < B::kEach; ++k) {
+        word[k] = 0;
+        par[k] = __half2half2(__ushort_as_half(0));
+        if (!mine) continue;
+        if (!B::value(k)) {
+            word[k] = *reinterpret_cast<const uint32_t*>(tile + F::key_word(r, w));
+            par[k] = *reinterpret_cast<const __half2*>(tile + F::key_par(r, g));
         } else {
-            word = *reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w)) |
-                   (uint32_t)*reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w + 1)) << 16;
+            word[k] = *reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w)) |
+                      (uint32_t)*reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w + 1)) << 16;
+            par[k] = *reinterpret_cast<const __half2*>(tile + F::val_par(r, g));
         }
-        const float2 par = __half22float2(*reinterpret_cast<const __half2*>(tile + (value ? F::val_par(r, g) : F::key_par(r, g))));
+    }
+#pragma unroll
+    for (int k = 0; k < B::kEach; ++k) {
+        const float2 f = __half22float2(par[k]);
+        uint4 out;
         __half2* o = reinterpret_cast<__half2*>(&out);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            o[e] = __floats2half2_rn(fmaf((float)((word >> (8 * e)) & 15), par.x, par.y), fmaf((float)((word >> (8 * e + 4)) & 15), par.x, par.y));
+            o[e] = __floats2half2_rn(fmaf((float)((word[k] >> (8 * e)) & 15), f.x, f.y), fmaf((float)((word[k] >> (8 * e + 4)) & 15), f.x, f.y));
+        *reinterpret_cast<uint4*>((B::value(k) ? a.v : a.k) + ((long long)bh * a.seq + s) * D + 8 * w) = out;
     }
-    *reinterpret_cast<uint4*>((value ? a.v : a.k) + u * D + 8 * w) = out;
 }
 
 // ---- pages -------------------------------------------------------------------------------------------------------------------
@@ -473,9 +492,9 @@ extern "C" int w4a16_kv4_append(const void* qkv, void* pool, const void* table, 
         return W4A16_ERR_BAD_SHAPE;
     if (((uintptr_t)qkv | (uintptr_t)rope_cos | (uintptr_t)rope_sin) & 15 || ((uintptr_t)pos | (uintptr_t)counts) & 3) return W4A16_ERR_MISALIGNED;
     if ((heads + 2ll * kv_heads) * head_dim >= (1ll << 30) || seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
-    a.units = (long long)batch * seq * kv_heads;
-    if (a.units == 0) return W4A16_OK;
-    const long long blocks = (a.units * 2 * (head_dim / 8) + 255) / 256;
+    if (batch == 0 || seq == 0) return W4A16_OK;
+    a.runs = runs_of(seq);
+    const long long blocks = (long long)batch * kv_heads * a.runs;
     if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
     a.qkv = (const __half*)qkv; a.pos = (const int*)pos; a.counts = (const int*)counts;
     a.cos = (const __half*)rope_cos; a.sin = (const __half*)rope_sin;
@@ -500,9 +519,9 @@ extern "C" int w4a16_kv4_read(const void* pool, const void* table, const void* p
     if (batch < 0 || seq < 0) return W4A16_ERR_BAD_SHAPE;
     if (((uintptr_t)k | (uintptr_t)v) & 15 || ((uintptr_t)pos | (uintptr_t)counts) & 3) return W4A16_ERR_MISALIGNED;
     if (seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
-    a.units = (long long)batch * seq * kv_heads;
-    if (a.units == 0) return W4A16_OK;
-    const long long blocks = (a.units * 2 * (head_dim / 8) + 255) / 256;
+    if (batch == 0 || seq == 0) return W4A16_OK;
+    a.runs = runs_of(seq);
+    const long long blocks = (long long)batch * kv_heads * a.runs;
     if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
     a.pos = (const int*)pos; a.counts = (const int*)counts; a.k = (__half*)k; a.v = (__half*)v; a.seq = seq;
     a.error = device_error_word();

@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                     const bool value = (lane / F::NW) & 1;
                     const int w = lane % F::NW, r = pos & 15;
                     constexpr int kLanes = D / NG / 8;
-                    float x[8];
-                    load_rotated<D>(a.qkv + b * a.stride + (a.heads + (value ? a.c.kv_heads : 0) + kvh) * D, w, value ? nullptr : a.cos, a.sin, pos, x);
+                    const uint4 x = load_rotated<D>(a.qkv + b * a.stride + (a.heads + (value ? a.c.kv_heads : 0) + kvh) * D, w,
+                                                    value ? nullptr : a.cos, a.sin, pos);
                     __half2 par;
                     const uint32_t word = quantize8(x, kLanes, par);
                     auto put = [&](unsigned char* to) {

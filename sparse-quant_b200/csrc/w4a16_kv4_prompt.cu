@@ -1,15 +1,18 @@
 // Attention of a chunk of queries over the paged 4-bit cache, on the 5th-generation tensor cores.
 //
-// A CTA takes 128 rows of one (batch row, key/value head): row f of the chunk's S x R is query f / R of head f % R of the R that share the
-// key/value head.  It walks over tiles of 128 cached tokens, up to its last query's position:
+// A CTA takes T x 128 rows of one (batch row, key/value head): row f of the chunk's S x R is query f / R of head f % R of the R that share
+// the key/value head.  It walks over tiles of 128 cached tokens, up to its last query's position, for each of its T row tiles:
 //     S = Q K^T     128 x 128, Q and K in shared memory, S in tensor memory
 //     P = 2^(S scale - ref), rounded to fp16, over S's place in tensor memory; ref follows the row's maximum by steps of 2^8 and more
 //     O += P V      P in tensor memory, V^T in shared memory, O in tensor memory
-// K and V come as codes: all eight warps turn m + n s into fp16 (one rounding, 2^-11 of the value) while the matrix products of the step
-// before run, and write the 128-byte swizzled layouts the products read - keys by tokens (dims of a word of 8 in the order 0 4 1 5 2 6
-// 3 7 that the codes unpack in; the queries are stored in the same order), values by dims (pairs of tokens unpack side by side).  Codes
-// travel from global memory through registers, one tile ahead.  256 threads, two for each row in the softmax, and two CTAs an SM: what
-// one of them waits for - S, then P V, one after the other, since P stands where S stood - is time for the other's arithmetic.
+// K and V come as codes: the worker warps turn m + n s into fp16 (one rounding, 2^-11 of the value) while the products run, and write the
+// 128-byte swizzled layouts the products read - keys by tokens (dims of a word of 8 in the order 0 4 1 5 2 6 3 7 that the codes unpack
+// in; the queries are stored in the same order), values by dims (pairs of tokens unpack side by side).  The codes of the next step are on
+// their way to shared memory meanwhile, and where its tiles stand is looked up two steps ahead.  Two threads a row in the softmax, eight
+// warps a row tile, and one warp that issues the products (issuing eight takes as long as they run).
+//
+// What bounds it is what the workers can issue: a tile of K and V costs them as much as its softmax.  So T = 2 (one CTA an SM) for more
+// than 128 rows of 128 dims, which halves that cost; otherwise T = 1, two CTAs an SM.
 //
 // A value whose group is not finite is multiplied as 0, so that rows that must not see its token stay clean, and the rows that do see it
 // get NaN for that group's dims at the end.
@@ -22,10 +25,9 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kRows = 128, kTokens = 128, kThreads = 256;
+constexpr int kRows = 128, kTokens = 128;
 constexpr int kTilesOf = kTokens / kTile;         // 16-token tiles of a step
 constexpr uint64_t kWaitNs = 400000000ull;        // a product that has not finished by then never will: error word 1
-constexpr uint32_t kTmemCols = 256;               // S (then P) in columns 0 .. 127, O behind it: two CTAs an SM
 
 struct PromptArgs {
     Cache c;
@@ -37,22 +39,26 @@ struct PromptArgs {
     const __half* sin;
     int* error;
     int seq, heads, share;        // share: query heads of a key/value head
-    int blocks;                   // of 128 rows
+    int blocks;                   // of T x 128 rows
     int rope_rows;
     long long stride, page_bytes;
     float scale_log2;             // scale * log2(e)
 };
 
-template <int D>
+template <int D, int half_tile, int T>
 struct Smem {
-    alignas(1024) unsigned char q[kRows * D * 2], k[kTokens * D * 2], v[kTokens * D * 2];
-    uint64_t s_done, pv_done;
+    alignas(1024) unsigned char q[T][kRows * D * 2], k[kTokens * D * 2], v[kTokens * D * 2];
+    // codes of the next step, with steps and minima (T = 1: the keys' come through registers, or two CTAs would not fit)
+    alignas(16) unsigned char v_codes[kTilesOf][half_tile], k_codes[T == 1 ? 1 : kTilesOf][half_tile];
+    const unsigned char* tile[4][kTilesOf];       // by step modulo 4: where its tiles stand; null: behind the last token, or no page
+    unsigned char page_ok[4][kTilesOf];           // 0: a page is needed and is none of the pool
+    uint64_t s_done[T], pv_done[T];               // products over
+    uint64_t k_ready, v_ready, p_ready[T];        // operands written
     uint32_t tmem;
     int abort_flag;
-    unsigned char page_ok[2][kTilesOf];           // 1: the tile's page is one of the pool
     int bad[kTokens];                             // groups of a token's value that are not finite
-    float swap[2][kRows];                         // what the two threads of a row tell each other
-    int swap_bad[kRows];
+    float swap[2][T * kRows];                     // what the two threads of a row tell each other
+    int swap_bad[T * kRows];
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -60,6 +66,37 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 h2_of(uint32_t b) { return *reinterpret_cast<const __half2*>(&b); }
@@ -75,6 +112,13 @@ __device__ __forceinline__ void codes8(uint32_t w, __half2 (&n)[4])
     n[3] = __hfma2(h2_of(lop3_and_or(top, 0x00f000f0u, 0x64006400u)), k16th, k64);
 }
 __device__ __forceinline__ bool finite2(__half2 p) { return (h2_bits(p) & 0x7c00u) != 0x7c00u && (h2_bits(p) & 0x7c000000u) != 0x7c000000u; }
+template <int N>
+__device__ __forceinline__ void load_params(const unsigned char* at, __half2 (&p)[N])
+{
+    if constexpr (N == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(at);
+    else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(at);
+    else p[0] = *reinterpret_cast<const __half2*>(at);
+}
 
 // D[tmem] (+)= A[smem] * B[smem], both K-major fp16
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
@@ -92,17 +136,39 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
           "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-__device__ __forceinline__ void smem_for_mma() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }      // this thread's
+// barriers of the worker warps
+template <int N>
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 9, %0;" ::"n"(N) : "memory"); }
+template <int N>
+__device__ __forceinline__ bool workers_any(bool mine)
+{
+    int any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, 10, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"((int)mine), "n"(N) : "memory");
+    return any != 0;
+}
+// the warp's operand writes of either kind, made visible to the products, and its arrival
+__device__ __forceinline__ void written(uint32_t bar, int lane)
+{
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
 
 // byte of 16-byte chunk `c` (8 halves) of row r in an operand of `rows` rows, 64 halves a sub-tile, 128-byte swizzle
 __device__ __forceinline__ int operand_at(int rows, int r, int c) { return (c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 
-template <class F, int D>
-__global__ void __launch_bounds__(kThreads, 2) prompt_kernel(const PromptArgs a)
+template <class F, int D, int T>
+__global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(const PromptArgs a)
 {
-    constexpr int J = F::J, NG = F::NG, kBytes = F::kBytes;
+    constexpr int J = F::J, NG = F::NG, kBytes = F::kBytes, kHalf = kBytes / 2, kWorkers = 256 * T, kWarps = 8 * T;
+    constexpr uint32_t kTmemCols = 256 * T;       // a row tile's S (then P) in 128 columns, O in the 128 behind them
+    static_assert(F::kVal == kHalf, "keys and values are halves of a tile");
     extern __shared__ unsigned char raw[];
-    Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    using S = Smem<D, kHalf, T>;
+    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int block = a.blocks - 1 - (int)blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;         // the longest rows first
     const int pos = a.pos[b], count = a.counts ? min(a.counts[b], a.seq) : a.seq;
@@ -110,80 +176,163 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_kernel(const PromptArgs a)
     const int room = min(a.c.capacity(), a.cos ? a.rope_rows : 0x7fffffff);
     const int fit = pos >= room ? 0 : min(count, room - pos);                                    // queries that can be served
     if (fit < count && block == 0 && kvh == 0 && tid == 0) atomicExch(a.error, kErrPosition);
-    const long long rows = (long long)fit * a.share;
-    if ((long long)block * kRows >= rows) return;
-    const int first_i = (int)((long long)block * kRows / a.share);
-    const int last_i = (int)(min((long long)(block + 1) * kRows, rows) - 1) / a.share;
+    const long long rows = (long long)fit * a.share, row0 = (long long)block * (T * kRows);
+    if (row0 >= rows) return;
+    const int first_i = (int)(row0 / a.share), last_i = (int)(min(row0 + T * kRows, rows) - 1) / a.share;
     const int last = pos + last_i;                                                               // the last token anybody here sees
     const int steps = last / kTokens + 1;
 
-    if (warp == 0) {
+    if (warp == kWarps) {
         tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
         tmem_relinquish();
     }
     if (tid == 0) {
-        mbar_init(smem_u32(&sm.s_done), 1);
-        mbar_init(smem_u32(&sm.pv_done), 1);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            mbar_init(smem_u32(&sm.s_done[t]), 1);
+            mbar_init(smem_u32(&sm.pv_done[t]), 1);
+            mbar_init(smem_u32(&sm.p_ready[t]), 8);
+        }
+        mbar_init(smem_u32(&sm.k_ready), kWarps);
+        mbar_init(smem_u32(&sm.v_ready), kWarps);
         sm.abort_flag = 0;
     }
     mbar_fence_init();
     if (tid < kTokens) sm.bad[tid] = 0;
 
-    // ---- codes on their way: what a thread turns into K and V of a step, in registers from one step to the next
+    // ---- where the tiles of a step stand (threads 0 .. 7)
     const int tshift = a.c.page_shift - 4, per1 = (1 << tshift) - 1;
     const int* ids = a.c.table + (size_t)b * a.c.width;
     const unsigned char* head = a.c.pool + ((size_t)kvh << tshift) * kBytes;
-    auto tile_at = [&](int t16) -> const unsigned char* {                                       // null: behind the last token, or no page
-        if (t16 > last >> 4) return nullptr;
-        const int page = ids[t16 >> tshift];
-        if ((unsigned)page >= (unsigned)a.c.pages) return nullptr;
-        return head + page * a.page_bytes + (t16 & per1) * kBytes;
+    int next_id = -1;
+    auto look = [&](int step) {
+        const int t16 = step * kTilesOf + tid;
+        next_id = t16 <= last >> 4 ? ids[t16 >> tshift] : -1;
     };
-    // keys: 16-byte pieces (4 words of 8 dims) of rows kt0 and, at D = 128, kt0 + 64; eight lanes take eight rows, so that their stores
-    // fall on different banks
-    constexpr int kPieces = D / 64;
-    const int kt0 = D == 128 ? 8 * warp + (lane & 7) : 8 * (2 * warp + (lane >> 4)) + (lane & 7), kc = D == 128 ? lane >> 3 : (lane >> 3) & 1;
-    // values: 8 tokens (group vt) by the half-words vh0 .. of lane-row vr; the lanes of a store fall on different banks as well
-    constexpr int kHalves = J / 2;
-    const int vt = 4 * (warp >> 1) + (lane & 3), vr = ((lane >> 2) & 1) | ((lane >> 3) << 1), vh0 = (warp & 1) * kHalves;
-    constexpr int kVGroups = D / NG == 32 && kHalves == 2 ? 2 : 1;
-    uint4 kw[kPieces];
-    __half2 kp[kPieces][NG], vp[8][kVGroups];
-    uint32_t vw[8];
-    auto load_k = [&](int step) {
-        if (tid < kTilesOf) {                                                                    // which tiles of the step have a page
-            const int t16 = step * kTilesOf + tid;
-            const bool ok = t16 > last >> 4 || tile_at(t16) != nullptr;
-            sm.page_ok[step & 1][tid] = ok;
-            if (!ok) atomicExch(a.error, kErrPage);
+    auto note = [&](int step) {
+        const int t16 = step * kTilesOf + tid;
+        const bool needed = t16 <= last >> 4, there = needed && (unsigned)next_id < (unsigned)a.c.pages;
+        sm.tile[step & 3][tid] = there ? head + next_id * a.page_bytes + (t16 & per1) * kBytes : nullptr;
+        sm.page_ok[step & 3][tid] = there || !needed;
+        if (needed && !there) atomicExch(a.error, kErrPage);
+    };
+    if (tid < kTilesOf) {
+        look(0);
+        note(0);
+        look(1);
+        note(1);
+    }
+    __syncthreads();
+    const uint32_t tmem = sm.tmem;
+    const uint32_t k_bar = smem_u32(&sm.k_ready), v_bar = smem_u32(&sm.v_ready);
+    bool ok = true;
+
+    if (warp == kWarps) {
+        // ---- the products.  P stands where S stood: S of a step is issued when P V of the step before is over
+        const uint64_t k_desc = smem_desc_sw128(smem_u32(sm.k)), v_desc = smem_desc_sw128(smem_u32(sm.v));
+        for (int step = 0; step < steps; ++step) {
+            ok = ok && mbar_wait(k_bar, step & 1, &sm.abort_flag, kWaitNs);                      // (the queries, at the first step)
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                if (step > 0) ok = ok && mbar_wait(smem_u32(&sm.pv_done[t]), (step - 1) & 1, &sm.abort_flag, kWaitNs);
+                tc_fence_after_sync();
+                __syncwarp();
+                const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q[t]));
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint64_t at = (uint64_t)((kk >> 2) * (kRows * 128 / 16) + 2 * (kk & 3));
+                    if (elect_one()) mma_f16_ss(tmem + 256 * t, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
+                }
+                if (elect_one()) tc_commit(smem_u32(&sm.s_done[t]));
+                __syncwarp();
+            }
+            ok = ok && mbar_wait(v_bar, step & 1, &sm.abort_flag, kWaitNs);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                ok = ok && mbar_wait(smem_u32(&sm.p_ready[t]), step & 1, &sm.abort_flag, kWaitNs);
+                tc_fence_after_sync();
+                __syncwarp();
+#pragma unroll
+                for (int kk = 0; kk < kTokens / 16; ++kk) {
+                    // P of tokens 0 .. 63 stands in columns 0 .. 31, of tokens 64 .. 127 in columns 64 .. 95
+                    const uint32_t p = tmem + 256 * t + (kk >> 2) * 64 + (kk & 3) * 8;
+                    const uint64_t at = (uint64_t)((kk >> 2) * (D * 128 / 16) + 2 * (kk & 3));
+                    if (elect_one()) mma_f16_ts(tmem + 256 * t + kTokens, p, v_desc + at, idesc_f16_m128(D), step > 0 || kk > 0);
+                }
+                if (elect_one()) tc_commit(smem_u32(&sm.pv_done[t]));
+                __syncwarp();
+            }
         }
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            const int t = step * kTokens + kt0 + 64 * k, r = t & 15;
-            const unsigned char* tile = tile_at(t >> 4);
-            kw[k] = make_uint4(0, 0, 0, 0);
+        for (int t = 0; t < T; ++t) ok = ok && mbar_wait(smem_u32(&sm.pv_done[t]), (steps - 1) & 1, &sm.abort_flag, kWaitNs);
+        if (!ok && lane == 0) atomicExch(a.error, 1);
+        __syncthreads();                                                                         // the workers have read O
+        tmem_dealloc(tmem, kTmemCols);
+        return;
+    }
+
+    // ---- codes of a step to shared memory, keys or values: tiles are contiguous halves
+    auto load_codes = [&](unsigned char* to, int step, int half_at) {
+        constexpr int kPieces = kHalf / 16;                                                      // of a tile
 #pragma unroll
-            for (int g = 0; g < NG; ++g) kp[k][g] = h2_of(0);
-            if (tile && t <= last) {
-                kw[k] = *reinterpret_cast<const uint4*>(tile + r * (D / 2) + 16 * kc);
+        for (int i = 0; i < (kTilesOf * kPieces + kWorkers - 1) / kWorkers; ++i) {
+            const int at = tid + i * kWorkers;
+            if (at >= kTilesOf * kPieces) break;
+            const unsigned char* tile = sm.tile[step & 3][at / kPieces];
+            // (a tile that is none is filled with zeros: its values are 0, its keys are hidden)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                         ::"r"(smem_u32(to) + at * 16), "l"(tile ? tile + half_at + (at % kPieces) * 16 : a.c.pool), "r"(tile ? 16 : 0) : "memory");
+        }
+    };
+    // keys: 16-byte pieces (4 words of 8 dims); eight lanes take eight rows, so that their stores fall on different banks
+    constexpr int kPieces = kTokens * D / 32 / kWorkers < 1 ? 1 : kTokens * D / 32 / kWorkers;  // of a thread
+    const int kp = lane >> 3, kt0 = D == 128 ? 8 * warp + (lane & 7) : 8 * (2 * warp + (kp >> 1)) + (lane & 7), kc = D == 128 ? kp : kp & 1;
+    const bool has_k = kt0 < kTokens;                                                            // (D = 64, T = 2: half of the threads)
+    uint4 kreg[T == 1 ? kPieces : 1];
+    __half2 kpar[T == 1 ? kPieces : 1][NG];
+    auto fetch_k = [&](int step) {
+        if constexpr (T == 2) {
+            load_codes(sm.k_codes[0], step, 0);
+        } else {
 #pragma unroll
-                for (int g = 0; g < NG; ++g) kp[k][g] = *reinterpret_cast<const __half2*>(tile + F::key_par(r, g));
+            for (int k = 0; k < kPieces; ++k) {
+                const int row = kt0 + 8 * kWarps * k;
+                const unsigned char* tile = sm.tile[step & 3][row >> 4];
+                kreg[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) kpar[k][g] = h2_of(0);
+                if (tile) {
+                    kreg[k] = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * kc);
+                    load_params<NG>(tile + F::key_par(row & 15, 0), kpar[k]);
+                }
             }
         }
     };
     auto put_k = [&]() {
+        if (!has_k) return;
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
-            const uint32_t w4[4] = {kw[k].x, kw[k].y, kw[k].z, kw[k].w};
-            __half2 s[NG], m[NG];
+            const int row = kt0 + 8 * kWarps * k;
+            uint4 kw;
+            __half2 par[NG], s[NG], m[NG];
+            if constexpr (T == 2) {
+                const unsigned char* tile = sm.k_codes[row >> 4];
+                kw = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * kc);
+                load_params<NG>(tile + F::key_par(row & 15, 0), par);
+            } else {
+                kw = kreg[k];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) par[g] = kpar[k][g];
+            }
+            const uint32_t w4[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                s[g] = __low2half2(kp[k][g]);
-                m[g] = __high2half2(kp[k][g]);
+                s[g] = __low2half2(par[g]);
+                m[g] = __high2half2(par[g]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                // stored word 4 kc + i is word w of the row; its group is known here where a piece holds one word of each 32 dims
+                // stored word 4 kc + i is word w of the row
                 const int j = D == 128 ? i : i & 1, w = D == 128 ? 4 * i + kc : 4 * (i & 1) + 2 * kc + (i >> 1);
                 const int g = 32 * j * NG / D;
                 __half2 n[4];
@@ -193,40 +342,53 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_kernel(const PromptArgs a)
                 o.y = h2_bits(__hfma2(n[1], s[g], m[g]));
                 o.z = h2_bits(__hfma2(n[2], s[g], m[g]));
                 o.w = h2_bits(__hfma2(n[3], s[g], m[g]));
-                *reinterpret_cast<uint4*>(sm.k + operand_at(kTokens, kt0 + 64 * k, w)) = o;
+                *reinterpret_cast<uint4*>(sm.k + operand_at(kTokens, row, w)) = o;
             }
         }
     };
-    auto load_v = [&](int step) {
-        const int t = step * kTokens + 8 * vt, r0 = t & 15;
-        const unsigned char* tile = tile_at(t >> 4);
+    // values: 8 tokens (group vt) by kHalves half-words of lane-row vr; the lanes of a store fall on different banks as well
+    constexpr int kVWarps = kWarps / 4, kHalves = J / kVWarps < 1 ? 1 : J / kVWarps;            // warps that share a group of tokens
+    const int vt = 4 * (warp / kVWarps) + (lane & 3), vr = ((lane >> 2) & 1) | ((lane >> 3) << 1), vh0 = warp % kVWarps * kHalves;
+    const bool has_v = vh0 < J;                                                                  // (D = 64, T = 2: half of the warps)
+    constexpr int kVGroups = D / NG == 32 && kHalves == 2 ? 2 : 1;
+    auto put_v = [&](int step) {                                                                 // true: some value is not finite
+        if (!has_v) return false;
+        const unsigned char* tile = sm.v_codes[vt >> 1];
+        const int r0 = 8 * (vt & 1), left = last - (step * kTokens + 8 * vt);                    // tokens behind the group's first
+        uint32_t vw[8];
+        __half2 vp[8][kVGroups], zero = h2_of(0);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            vw[k] = 0;
+            const int at = 2 * (vr * J + vh0);
+            const unsigned char* from = tile + (r0 + k) * (D / 2) + (D == 128 ? at ^ (((k >> 1) & 1) << 5) : at);
+            if constexpr (kHalves == 2) vw[k] = *reinterpret_cast<const uint32_t*>(from);
+            else vw[k] = *reinterpret_cast<const uint16_t*>(from);
 #pragma unroll
-            for (int g = 0; g < kVGroups; ++g) vp[k][g] = h2_of(0);
-            if (tile && t + k <= last) {
-                const int at = 2 * (vr * J + vh0);
-                const unsigned char* from = tile + F::kVal + (r0 + k) * (D / 2) + (D == 128 ? at ^ (((k >> 1) & 1) << 5) : at);
-                if constexpr (kHalves == 2) vw[k] = *reinterpret_cast<const uint32_t*>(from);
-                else vw[k] = *reinterpret_cast<const uint16_t*>(from);
+            for (int g = 0; g < kVGroups; ++g)
+                vp[k][g] = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + k, 32 * (vh0 + g) * NG / D) - F::kVal);
+        }
+        if (left < 7) {                                                                          // behind the last token: whatever the page holds
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
 #pragma unroll
                 for (int g = 0; g < kVGroups; ++g)
-                    vp[k][g] = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + k, 32 * (vh0 + g) * NG / D));
-            }
+                    if (k > left) vp[k][g] = h2_of(0);
         }
-    };
-    auto put_v = [&]() {                                                                         // true: some value is not finite
-        bool found = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int g = 0; g < kVGroups; ++g)
-                if (!finite2(vp[k][g])) {
-                    vp[k][g] = h2_of(0);
-                    atomicOr(&sm.bad[8 * vt + k], 1 << (32 * (vh0 + g) * NG / D));
-                    found = true;
-                }
+            for (int g = 0; g < kVGroups; ++g) zero = __hfma2(vp[k][g], h2_of(0), zero);         // NaN if one of them is not finite
+        const bool found = !__hbeq2(zero, zero);
+        if (found) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int g = 0; g < kVGroups; ++g)
+                    if (!finite2(vp[k][g])) {
+                        vp[k][g] = h2_of(0);
+                        atomicOr(&sm.bad[8 * vt + k], 1 << (32 * (vh0 + g) * NG / D));
+                    }
+        }
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
             constexpr int last_group = kVGroups - 1;
@@ -247,13 +409,14 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_kernel(const PromptArgs a)
         }
         return found;
     };
-    load_k(0);
-    load_v(0);
 
+    fetch_k(0);
+    load_codes(sm.v_codes[0], 0, kHalf);
     // ---- queries: two threads a row, rotated as the decode kernel does, in the order of the keys' dims
+    const int mine = warp >> 3;                                                                  // the thread's row tile
     {
-        const int r = tid >> 1;
-        const long long f = (long long)block * kRows + r;
+        const int r = (tid & 255) >> 1;
+        const long long f = row0 + mine * kRows + r;
         const int i = (int)(f / a.share), h = (int)(f % a.share);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -265,170 +428,153 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_kernel(const PromptArgs a)
             o.y = h2_bits(__floats2half2_rn(x[1], x[5]));
             o.z = h2_bits(__floats2half2_rn(x[2], x[6]));
             o.w = h2_bits(__floats2half2_rn(x[3], x[7]));
-            *reinterpret_cast<uint4*>(sm.q + operand_at(kRows, r, w)) = o;
+            *reinterpret_cast<uint4*>(sm.q[mine] + operand_at(kRows, r, w)) = o;
         }
     }
+    copies_landed();
+    workers_sync<kWorkers>();
     put_k();
-    smem_for_mma();
-    tc_fence_before_sync();
-    __syncthreads();
-    tc_fence_after_sync();
-    const uint32_t tmem = sm.tmem, lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_bar = smem_u32(&sm.s_done), pv_bar = smem_u32(&sm.pv_done);
-    const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q)), k_desc = smem_desc_sw128(smem_u32(sm.k)), v_desc = smem_desc_sw128(smem_u32(sm.v));
-    auto issue_s = [&]() {                                                                       // warp 0
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t at = (uint64_t)((kk >> 2) * (kRows * 128 / 16) + 2 * (kk & 3));
-            if (elect_one()) mma_f16_ss(tmem, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
-        }
-        if (elect_one()) tc_commit(s_bar);
-        __syncwarp();
-    };
-    auto issue_pv = [&](bool first) {
-#pragma unroll
-        for (int kk = 0; kk < kTokens / 16; ++kk) {
-            // P of tokens 0 .. 63 stands in columns 0 .. 31, of tokens 64 .. 127 in columns 64 .. 95
-            const uint32_t p = tmem + (kk >> 2) * 64 + (kk & 3) * 8;
-            const uint64_t at = (uint64_t)((kk >> 2) * (D * 128 / 16) + 2 * (kk & 3));
-            if (elect_one()) mma_f16_ts(tmem + kTokens, p, v_desc + at, idesc_f16_m128(D), !first || kk > 0);
-        }
-        if (elect_one()) tc_commit(pv_bar);
-        __syncwarp();
-    };
-    if (warp == 0) issue_s();
+    written(k_bar, lane);
+    workers_sync<kWorkers>();                                                                    // the keys' codes have been read
+    if (T == 2 && steps > 1) fetch_k(1);
 
     // ---- the row of this thread in the softmax, and its half of the columns
-    const int row = 32 * (warp & 3) + lane, half = warp >> 2;
-    const int sees = pos + min((int)(((long long)block * kRows + row) / a.share), last_i);      // last token it sees (rows behind the last: as that one)
+    const int row = 32 * (warp & 3) + lane, half = (warp >> 2) & 1, slot = mine * kRows + row;
+    const uint32_t at_s = tmem + 256 * mine + ((uint32_t)(32 * (warp & 3)) << 16), at_o = at_s + kTokens + half * (D / 2);
+    const uint32_t s_bar = smem_u32(&sm.s_done[mine]), p_bar = smem_u32(&sm.p_ready[mine]);
+    const int sees = pos + min((int)((row0 + slot) / a.share), last_i);                         // last token it sees (rows behind the last: as that one)
     const int first_sees = pos + first_i;
     // (the sign of a negative scale goes into the scores, so that `unit` is positive; a scale of zero makes them zero)
     const float unit = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2), sign = a.scale_log2 == 0.f ? 0.f : a.scale_log2 < 0.f ? -1.f : 1.f;
-    float ref = -INFINITY, sum = 0.f;
+    const uint64_t unit2 = pair(unit, unit);
+    float ref = -INFINITY;
+    uint64_t sum2 = pair(0.f, 0.f);
     int nan_groups = 0;
-    bool ok = true;
     for (int step = 0; step < steps; ++step) {
-        const bool found = put_v();                                                              // (P V of the step before is over)
-        smem_for_mma();
-        if (step + 1 < steps) load_k(step + 1);
+        const bool found = put_v(step);                                                          // (P V of the step before is over)
+        written(v_bar, lane);
+        if (T == 1 && step + 1 < steps) fetch_k(step + 1);
+        if (tid < kTilesOf) look(step + 2);
         ok = ok && mbar_wait(s_bar, step & 1, &sm.abort_flag, kWaitNs);
         tc_fence_after_sync();
-        const uint64_t pages = *reinterpret_cast<const uint64_t*>(sm.page_ok[step & 1]);
+        const uint64_t pages = *reinterpret_cast<const uint64_t*>(sm.page_ok[step & 3]);
         const bool masked = (step + 1) * kTokens - 1 > first_sees || pages != 0x0101010101010101ull;
         const int from = step * kTokens + 64 * half;                                             // the thread's first token
         uint32_t s[32];
-        float top = -INFINITY;
-        auto hide = [&](int c0) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int t = from + c0 + i;
-                const bool seen = t <= sees && (pages >> (8 * ((64 * half + c0 + i) >> 4)) & 1);
-                if (!seen) s[i] = 0xff800000u;
-            }
-        };
-        auto fetch = [&](int c0) {
-            tmem_ld_32x32b_x32(tmem + lanes + 64 * half + c0, s);
+        auto fetch = [&](int c) {                                                                // scores of 32 tokens
+            tmem_ld_32x32b_x32(at_s + 64 * half + 32 * c, s);
             tmem_wait_ld();
             if (sign != 1.f) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * sign);
             }
-            if (masked) hide(c0);
+            if (masked) {
+                const int seen = sees - (from + 32 * c);
+                const uint32_t p0 = (uint32_t)(pages >> (8 * (4 * half + 2 * c))) & 1, p1 = (uint32_t)(pages >> (8 * (4 * half + 2 * c + 1))) & 1;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (i > seen || !(i < 16 ? p0 : p1)) s[i] = 0xff800000u;
+            }
         };
+        float top = -INFINITY;
 #pragma unroll
         for (int c = 1; c >= 0; --c) {
-            fetch(32 * c);
+            fetch(c);
+            float t0 = top, t1 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(s[i]));
+            for (int i = 0; i < 32; i += 4) {
+                t0 = max3(t0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                t1 = max3(t1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+            }
+            top = fmaxf(t0, t1);
         }
         // both threads of a row move the reference alike
-        sm.swap[half][row] = top;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
-        top = fmaxf(top, sm.swap[half ^ 1][row]) * unit;
-        bool move = top - ref > 8.f;                                                             // (from minus infinity as well; not with nothing seen)
+        sm.swap[half][slot] = top;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + mine * 4 + (warp & 3)) : "memory");
+        top = fmaxf(top, sm.swap[half ^ 1][slot]) * unit;
+        const bool move = top - ref > 8.f;                                                       // (from minus infinity as well; not with nothing seen)
         if (__any_sync(0xffffffffu, move)) {
             const float to = move ? top : ref, keep = ref == -INFINITY ? 0.f : ex2(ref - to);
             ref = to;
-            sum *= keep;
+            const float2 f = unpair(sum2);
+            sum2 = pair(f.x * keep, f.y * keep);
             if (step > 0) {
                 uint32_t o[16];
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
-                    const uint32_t at = tmem + lanes + kTokens + half * (D / 2) + 16 * c;
-                    tmem_ld_32x32b_x16(at, o);
+                    tmem_ld_32x32b_x16(at_o + 16 * c, o);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                    tmem_st_32x32b_x16(at, o);
+                    tmem_st_32x32b_x16(at_o + 16 * c, o);
                 }
             }
         }
-        const float shift = ref == -INFINITY ? 0.f : ref;                                        // nothing seen yet: weights 0
+        const float shift = ref == -INFINITY ? 0.f : -ref;                                       // nothing seen yet: weights 0
+        const uint64_t shift2 = pair(shift, shift);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            if (c == 1) fetch(32);
+            if (c == 1) fetch(1);                                                                // (again: 64 at a time are too many registers)
             uint32_t p[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float p0 = ex2(fmaf(__uint_as_float(s[2 * i]), unit, -shift)), p1 = ex2(fmaf(__uint_as_float(s[2 * i + 1]), unit, -shift));
-                sum += p0 + p1;
+                const float2 x = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), unit2, shift2));
+                const float p0 = ex2(x.x), p1 = ex2(x.y);
+                sum2 = add2(sum2, pair(p0, p1));
                 p[i] = h2_bits(__floats2half2_rn(p0, p1));
             }
-            // over columns of S that this thread has read (its tokens 32 .. 63 are read again)
-            tmem_st_32x32b_x16(tmem + lanes + 64 * half + 16 * c, p);
+            tmem_st_32x32b_x16(at_s + 64 * half + 16 * c, p);                                    // over columns that this thread has read
         }
         tmem_wait_st();
-        tc_fence_before_sync();
-        if (__syncthreads_or(found)) {
+        written(p_bar, lane);
+        copies_landed();
+        if (workers_any<kWorkers>(found)) {
             // rows that see a value that is not finite
 #pragma unroll 1
             for (int i = 0; i < 64; ++i) {
                 const int t = from + i;
                 if (t <= sees && (pages >> (8 * ((64 * half + i) >> 4)) & 1)) nan_groups |= sm.bad[64 * half + i];
             }
-            __syncthreads();
+            workers_sync<kWorkers>();
             if (tid < kTokens) sm.bad[tid] = 0;
         }
-        if (warp == 0) {
-            tc_fence_after_sync();
-            issue_pv(step == 0);
-        }
         if (step + 1 < steps) {
-            put_k();                                                                             // (S of this step is over)
-            smem_for_mma();
-            load_v(step + 1);
-            ok = ok && mbar_wait(pv_bar, step & 1, &sm.abort_flag, kWaitNs);
+            load_codes(sm.v_codes[0], step + 1, kHalf);                                             // (everybody has read the codes of this step)
+            put_k();                                                                             // (S of this step is over in all row tiles)
+            written(k_bar, lane);
+            if (tid < kTilesOf) note(step + 2);
+            copies_landed();
+            workers_sync<kWorkers>();
+            if (T == 2 && step + 2 < steps) fetch_k(step + 2);
+#pragma unroll
+            for (int t = 0; t < T; ++t) ok = ok && mbar_wait(smem_u32(&sm.pv_done[t]), step & 1, &sm.abort_flag, kWaitNs);
             tc_fence_after_sync();
-            tc_fence_before_sync();
-            __syncthreads();
-            if (warp == 0) {
-                tc_fence_after_sync();
-                issue_s();
-            }
         }
     }
-    ok = ok && mbar_wait(pv_bar, (steps - 1) & 1, &sm.abort_flag, kWaitNs);
+    ok = ok && mbar_wait(smem_u32(&sm.pv_done[mine]), (steps - 1) & 1, &sm.abort_flag, kWaitNs);
     tc_fence_after_sync();
     if (!ok && lane == 0) atomicExch(a.error, 1);
 
     // ---- out = O / sum
-    sm.swap[half][row] = sum;
-    if (half) sm.swap_bad[row] = nan_groups;
-    __syncthreads();
-    sum += sm.swap[half ^ 1][row];
+    const float2 sums = unpair(sum2);
+    float sum = sums.x + sums.y;
+    sm.swap[half][slot] = sum;
+    if (half) sm.swap_bad[slot] = nan_groups;
+    workers_sync<kWorkers>();
+    sum += sm.swap[half ^ 1][slot];
     if (!half) {
-        nan_groups |= sm.swap_bad[row];
-        sm.swap_bad[row] = nan_groups;
+        nan_groups |= sm.swap_bad[slot];
+        sm.swap_bad[slot] = nan_groups;
     }
-    __syncthreads();
-    nan_groups = sm.swap_bad[row];
+    workers_sync<kWorkers>();
+    nan_groups = sm.swap_bad[slot];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const long long f = (long long)block * kRows + row;
+    const long long f = row0 + slot;
     __half* to = a.out + ((long long)b * a.seq + (int)(f / a.share)) * a.heads * D + (kvh * a.share + (int)(f % a.share)) * D + half * (D / 2);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
         uint32_t o[16];
-        tmem_ld_32x32b_x16(tmem + lanes + kTokens + half * (D / 2) + 16 * c, o);
+        tmem_ld_32x32b_x16(at_o + 16 * c, o);
         tmem_wait_ld();
         if (f >= rows) continue;
         const int g = (half * (D / 2) + 16 * c) * NG / D;
@@ -441,23 +587,24 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_kernel(const PromptArgs a)
     }
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
-template <class F, int D>
-int launch_prompt_as(const PromptArgs& a, int batch, cudaStream_t st)
+template <class F, int D, int T>
+int launch_prompt_as(PromptArgs& a, long long rows, int batch, cudaStream_t st)
 {
     static int configured[64] = {0};   // benign race: the attribute call is idempotent
-    const int smem = (int)sizeof(Smem<D>) + 1024;
+    const int smem = (int)sizeof(Smem<D, F::kBytes / 2, T>) + 1024;
+    static_assert(sizeof(Smem<D, F::kBytes / 2, T>) + 1024 <= (T == 1 ? 115712 : 232448), "fits the SM");
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(prompt_kernel<F, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = cudaFuncSetAttribute(prompt_kernel<F, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return record_cuda_error(e);
         if (dev < 64) configured[dev] = 1;
     }
-    prompt_kernel<F, D><<<dim3(a.blocks, a.c.kv_heads, batch), kThreads, smem, st>>>(a);
+    a.blocks = (int)((rows + T * kRows - 1) / (T * kRows));
+    prompt_kernel<F, D, T><<<dim3(a.blocks, a.c.kv_heads, batch), 256 * T + 32, smem, st>>>(a);
     count_launch();
     e = cudaGetLastError();
     return e == cudaSuccess ? W4A16_OK : record_cuda_error(e);
@@ -486,18 +633,23 @@ extern "C" int w4a16_kv4_attention(const void* qkv, const void* pool, const void
         return W4A16_ERR_MISALIGNED;
     if ((heads + 2ll * kv_heads) * head_dim >= (1ll << 30) || batch > 65535 || kv_heads > 65535 || seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
     a.share = heads / kv_heads;
-    const long long blocks = ((long long)seq * a.share + kRows - 1) / kRows;
-    if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
+    const long long rows = (long long)seq * a.share;
+    if (rows >= (1ll << 37)) return W4A16_ERR_TOO_LARGE;
     if (batch == 0 || seq == 0) return W4A16_OK;
     a.qkv = (const __half*)qkv; a.out = (__half*)out; a.pos = (const int*)pos; a.counts = (const int*)counts;
     a.cos = (const __half*)rope_cos; a.sin = (const __half*)rope_sin;
-    a.seq = seq; a.heads = heads; a.blocks = (int)blocks; a.rope_rows = rope_rows; a.stride = qkv_stride;
+    a.seq = seq; a.heads = heads; a.rope_rows = rope_rows; a.stride = qkv_stride;
     a.page_bytes = (long long)kv_heads * (page_size / kTile) * tile_bytes(head_dim, group);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.error = device_error_word();
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        return launch_prompt_as<F, F::NW * 8>(a, batch, (cudaStream_t)stream);
+        // (at 64 dims a tile of K and V costs half as much, and two CTAs that wait for each other's products do better: 243 / 265 us for
+        // 2 x 2048 queries behind 1000 tokens, 32 heads on 8; at 128 dims 1014 / 788 us for 4096 behind 4096)
+        if constexpr (F::NW == 16) {
+            if (rows > kRows) return launch_prompt_as<F, 128, 2>(a, rows, batch, (cudaStream_t)stream);
+        }
+        return launch_prompt_as<F, F::NW * 8, 1>(a, rows, batch, (cudaStream_t)stream);
     });
 }
