@@ -7,7 +7,9 @@
 //     O += P V      P in tensor memory, V^T in shared memory, O in tensor memory
 // K and V come as codes: the worker warps turn m + n s into fp16 (one rounding, 2^-11 of the value) while the products run, and write the
 // 128-byte swizzled layouts the products read - keys by tokens (dims of a word of 8 in the order 0 4 1 5 2 6 3 7 that the codes unpack
-// in; the queries are stored in the same order), values by dims (pairs of tokens unpack side by side).  The codes of the next step are on
+// in; the queries are stored in the same order), values by dims: a transposing matrix load gives a lane the same four dims of two tokens,
+// which unpack side by side.  The rows of V^T, and with them the columns of O, stand in the order 8 n + h + 32 p of dim n of the half-word
+// 8 p + h that the cache stores, which puts the eight rows that one store instruction touches on different banks.  The codes of the next step are on
 // their way to shared memory meanwhile, and where its tiles stand is looked up two steps ahead.  Two threads a row in the softmax, eight
 // warps a row tile, and one warp that issues the products (issuing eight takes as long as they run).
 //
@@ -271,17 +273,24 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
         return;
     }
 
-    // ---- codes of a step to shared memory, keys or values: tiles are contiguous halves
+    // ---- codes of a step to shared memory, keys or values: tiles are contiguous halves of 16-byte pieces.  A code row's pieces change
+    // places, so that the eight rows that are read together stand on different banks: by rows' bits 1 and 2 (keys; values stand
+    // exchanged by bit 1 already), at D = 64 by bit 2.
+    auto piece_of = [&](int row, int piece, bool values) {
+        return D == 128 ? piece ^ (values ? (row >> 2) & 1 : (row >> 1) & 3) : piece ^ ((row >> 2) & 1);
+    };
     auto load_codes = [&](unsigned char* to, int step, int half_at) {
-        constexpr int kPieces = kHalf / 16;                                                      // of a tile
+        constexpr int kPieces = kHalf / 16, kRowPieces = D / 32;                                 // of a tile, of a code row
 #pragma unroll
         for (int i = 0; i < (kTilesOf * kPieces + kWorkers - 1) / kWorkers; ++i) {
             const int at = tid + i * kWorkers;
             if (at >= kTilesOf * kPieces) break;
             const unsigned char* tile = sm.tile[step & 3][at / kPieces];
+            const int piece = at % kPieces, row = piece / kRowPieces;
+            const int there = row < kTile ? row * kRowPieces + piece_of(row, piece % kRowPieces, half_at != 0) : piece;
             // (a tile that is none is filled with zeros: its values are 0, its keys are hidden)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                         ::"r"(smem_u32(to) + at * 16), "l"(tile ? tile + half_at + (at % kPieces) * 16 : a.c.pool), "r"(tile ? 16 : 0) : "memory");
+                         ::"r"(smem_u32(to) + (at - piece + there) * 16), "l"(tile ? tile + half_at + piece * 16 : a.c.pool), "r"(tile ? 16 : 0) : "memory");
         }
     };
     // keys: 16-byte pieces (4 words of 8 dims); eight lanes take eight rows, so that their stores fall on different banks
@@ -317,7 +326,7 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
             __half2 par[NG], s[NG], m[NG];
             if constexpr (T == 2) {
                 const unsigned char* tile = sm.k_codes[row >> 4];
-                kw = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * kc);
+                kw = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * piece_of(row & 15, kc, false));
                 load_params<NG>(tile + F::key_par(row & 15, 0), par);
             } else {
                 kw = kreg[k];
@@ -346,66 +355,51 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
             }
         }
     };
-    // values: 8 tokens (group vt) by kHalves half-words of lane-row vr; the lanes of a store fall on different banks as well
-    constexpr int kVWarps = kWarps / 4, kHalves = J / kVWarps < 1 ? 1 : J / kVWarps;            // warps that share a group of tokens
-    const int vt = 4 * (warp / kVWarps) + (lane & 3), vr = ((lane >> 2) & 1) | ((lane >> 3) << 1), vh0 = warp % kVWarps * kHalves;
-    const bool has_v = vh0 < J;                                                                  // (D = 64, T = 2: half of the warps)
-    constexpr int kVGroups = D / NG == 32 && kHalves == 2 ? 2 : 1;
+    // values: a warp takes groups of 8 tokens.  Matrix p of the load is the 16-byte piece p of the tokens' rows: the lane gets half-word
+    // 8 p + lane / 4 of tokens 2 (lane % 4) and the next one, all of one group of dims.
+    const int vh = lane >> 2, vp2 = 2 * (lane & 3), vgroup = 32 * (vh % J) * NG / D;
     auto put_v = [&](int step) {                                                                 // true: some value is not finite
-        if (!has_v) return false;
-        const unsigned char* tile = sm.v_codes[vt >> 1];
-        const int r0 = 8 * (vt & 1), left = last - (step * kTokens + 8 * vt);                    // tokens behind the group's first
-        uint32_t vw[8];
-        __half2 vp[8][kVGroups], zero = h2_of(0);
+        bool found = false;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int at = 2 * (vr * J + vh0);
-            const unsigned char* from = tile + (r0 + k) * (D / 2) + (D == 128 ? at ^ (((k >> 1) & 1) << 5) : at);
-            if constexpr (kHalves == 2) vw[k] = *reinterpret_cast<const uint32_t*>(from);
-            else vw[k] = *reinterpret_cast<const uint16_t*>(from);
-#pragma unroll
-            for (int g = 0; g < kVGroups; ++g)
-                vp[k][g] = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + k, 32 * (vh0 + g) * NG / D) - F::kVal);
-        }
-        if (left < 7) {                                                                          // behind the last token: whatever the page holds
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-#pragma unroll
-                for (int g = 0; g < kVGroups; ++g)
-                    if (k > left) vp[k][g] = h2_of(0);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-            for (int g = 0; g < kVGroups; ++g) zero = __hfma2(vp[k][g], h2_of(0), zero);         // NaN if one of them is not finite
-        const bool found = !__hbeq2(zero, zero);
-        if (found) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-#pragma unroll
-                for (int g = 0; g < kVGroups; ++g)
-                    if (!finite2(vp[k][g])) {
-                        vp[k][g] = h2_of(0);
-                        atomicOr(&sm.bad[8 * vt + k], 1 << (32 * (vh0 + g) * NG / D));
-                    }
-        }
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            constexpr int last_group = kVGroups - 1;
-            const int g = h < last_group ? h : last_group;
-            uint32_t o[4][4];                                                                    // [dim of the half-word][pair of tokens]
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t pa = h2_bits(vp[2 * k][g]), pb = h2_bits(vp[2 * k + 1][g]);
-                const __half2 s = h2_of(__byte_perm(pa, pb, 0x5410)), m = h2_of(__byte_perm(pa, pb, 0x7632));
-                __half2 n[4];
-                codes8(__byte_perm(vw[2 * k], vw[2 * k + 1], h ? 0x7632 : 0x5410), n);
-#pragma unroll
-                for (int d = 0; d < 4; ++d) o[d][k] = h2_bits(__hfma2(n[d], s, m));
+        for (int i = 0; i < kTokens / 8 / kWarps; ++i) {
+            const int vt = warp + i * kWarps, r0 = 8 * (vt & 1);
+            const unsigned char* tile = sm.v_codes[vt >> 1];
+            const int left = last - (step * kTokens + 8 * vt) - vp2;                             // tokens behind the lane's first
+            // lane l gives the address of row l % 8 of matrix l / 8 (at D = 64, two matrices: lanes 16 .. 31 repeat)
+            const int lr = r0 + (lane & 7), lp = (lane >> 3) & (J - 1);
+            const int stored = D == 128 ? lp ^ (((lr >> 1) & 1) << 1) : lp;
+            const uint32_t from = smem_u32(tile + lr * (D / 2) + 16 * piece_of(lr, stored, true));
+            uint32_t w[J];
+            if constexpr (J == 4)
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+            else
+                asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
+            __half2 pa = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2, vgroup) - F::kVal);
+            __half2 pb = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2 + 1, vgroup) - F::kVal);
+            if (left < 0) pa = h2_of(0);                                                         // behind the last token: whatever the page holds
+            if (left < 1) pb = h2_of(0);
+            const __half2 zero = __hfma2(pa, h2_of(0), __hmul2(pb, h2_of(0)));                   // NaN if one of them is not finite
+            if (!__hbeq2(zero, zero)) {
+                found = true;
+                if (!finite2(pa)) {
+                    pa = h2_of(0);
+                    atomicOr(&sm.bad[8 * vt + vp2], 1 << vgroup);
+                }
+                if (!finite2(pb)) {
+                    pb = h2_of(0);
+                    atomicOr(&sm.bad[8 * vt + vp2 + 1], 1 << vgroup);
+                }
             }
+            const __half2 s = __lows2half2(pa, pb), m = __highs2half2(pa, pb);
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
-                *reinterpret_cast<uint4*>(sm.v + operand_at(D, 32 * (vh0 + h) + 4 * vr + d, vt)) = make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
+            for (int q = 0; q < J; ++q) {
+                __half2 n[4];
+                codes8(w[q], n);
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    *reinterpret_cast<__half2*>(sm.v + operand_at(D, 32 * q + 8 * d + vh, vt) + 2 * vp2) = __hfma2(n[d], s, m);
+            }
         }
         return found;
     };
@@ -570,20 +564,29 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
     nan_groups = sm.swap_bad[slot];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const long long f = row0 + slot;
-    __half* to = a.out + ((long long)b * a.seq + (int)(f / a.share)) * a.heads * D + (kvh * a.share + (int)(f % a.share)) * D + half * (D / 2);
+    __half* to = a.out + ((long long)b * a.seq + (int)(f / a.share)) * a.heads * D + (kvh * a.share + (int)(f % a.share)) * D;
+    // columns of this half: pieces p = half D/64 .. of half-words, 32 columns each; 32/J adjacent dims of each 32 stand in a piece
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[16];
-        tmem_ld_32x32b_x16(at_o + 16 * c, o);
+    for (int c = 0; c < D / 64; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(at_o + 32 * c, o);
         tmem_wait_ld();
         if (f >= rows) continue;
-        const int g = (half * (D / 2) + 16 * c) * NG / D;
-        const float mul = nan_groups >> g & 1 ? __int_as_float(0x7fffffff) : inv;
-        uint32_t h[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = h2_bits(__floats2half2_rn(__uint_as_float(o[2 * i]) * mul, __uint_as_float(o[2 * i + 1]) * mul));
-        *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(to + 16 * c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+        for (int j = 0; j < J; ++j) {
+            const float mul = nan_groups >> (32 * j * NG / D) & 1 ? __int_as_float(0x7fffffff) : inv;
+            __half* dims = to + 32 * j + (half * (D / 64) + c) * (32 / J);
+#pragma unroll
+            for (int r = 0; r < 8 / J; r += 2) {                                                 // half-words r J + j of the piece: four dims each
+                uint32_t h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = (r + i / 2) * J + j + 16 * (i % 2);
+                    h[i] = h2_bits(__floats2half2_rn(__uint_as_float(o[at]) * mul, __uint_as_float(o[at + 8]) * mul));
+                }
+                *reinterpret_cast<uint4*>(dims + 4 * r) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+        }
     }
     tc_fence_before_sync();
     __syncthreads();
