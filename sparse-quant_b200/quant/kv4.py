@@ -9,9 +9,10 @@ from __future__ import annotations
 
 import torch
 
-from . import _check, _check_tensor, _need, _stream, load_library
+from . import _check, _check_tensor, _need, load_library
 
 # tile bytes -> (head_dim, group): 16 head_dim + 128 head_dim / group are different for all formats
+_U8, _I32, _F16 = torch.uint8, torch.int32, torch.float16
 _FORMATS = {16 * d + 128 * d // g: (d, g) for d in (64, 128) for g in (32, 64, 128) if g <= d}
 
 
@@ -55,49 +56,43 @@ def _rope_args(rope, D, device):
     return cos.data_ptr(), sin.data_ptr(), cos.shape[0]
 
 
-class _on:
-    """The device guard of a call, where the tensors are not on the current device."""
-
-    def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
 def _is(t, dtype, dims: int, device: int) -> bool:
-    """A contiguous CUDA tensor of this type, dimension number and device."""
-    return isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == dims and t.get_device() == device and t.is_contiguous()
+    """A contiguous CUDA tensor of this type, dimension number and device (of what is no tensor: AttributeError)."""
+    return t.dtype is dtype and t.get_device() == device and t.dim() == dims and t.is_contiguous()
 
 
 def _call_shape(x, x_dims, pool, table, pos, counts, rope, heads, row_parts):
     """(B, S, N, device, pages, kv_heads, page_size, head_dim, group, heads, table width, cos, sin, rope rows) of a call on a layer's pool, all arguments
     checked: x fp16 [B, (S,) N] with N at least heads + row_parts kv_heads head rows, or None (kv4_read).  One pass over the checks where
     they hold - an eager call is host time -, the checks one by one, each with its message, where one does not."""
-    ref = pool if x is None else x
-    dev = ref.get_device() if isinstance(ref, torch.Tensor) and ref.is_cuda else -1
-    fmt = _FORMATS.get(pool.shape[-1]) if dev >= 0 and _is(pool, torch.uint8, 4, dev) and pool.numel() else None
-    if fmt is not None and _is(table, torch.int32, 2, dev) and _is(pos, torch.int32, 1, dev) and (x is None or _is(x, torch.float16, x_dims, dev)):
-        D, g = fmt
-        pages, kv, per, _ = pool.shape
-        B, width = table.shape
-        N = 0 if x is None else x.shape[-1]
-        heads = kv if x is None else int(heads)
-        ok = pos.shape[0] == B and heads > 0 and heads % kv == 0 and (x is None or x.shape[0] == B and N >= (heads + row_parts * kv) * D) and \
-            (counts is None or _is(counts, torch.int32, 1, dev) and counts.shape[0] == B)
-        if ok and rope is not None:
-            cos, sin = rope
-            ok = _is(cos, torch.float16, 2, dev) and _is(sin, torch.float16, 2, dev) and cos.shape == sin.shape and cos.shape[1] == D
-        if ok:
-            S = x.shape[1] if x_dims == 3 else 1
+    try:
+        dev = pool.get_device()
+        fmt = _FORMATS.get(pool.shape[-1])
+        if dev >= 0 and fmt is not None and _is(pool, _U8, 4, dev) and _is(table, _I32, 2, dev) and _is(pos, _I32, 1, dev) and \
+                (x is None or _is(x, _F16, x_dims, dev)):
+            D, g = fmt
+            pages, kv, per, _ = pool.shape
+            B, width = table.shape
+            S, N = 1, 0
+            if x is None:
+                heads, ok = kv, True
+            else:
+                heads = int(heads)
+                if x_dims == 3:
+                    rows, S, N = x.shape
+                else:
+                    rows, N = x.shape
+                ok = rows == B and heads > 0 and kv > 0 and heads % kv == 0 and N >= (heads + row_parts * kv) * D
+            ok = ok and pages > 0 and kv > 0 and per > 0 and pos.shape[0] == B and (counts is None or _is(counts, _I32, 1, dev) and counts.shape[0] == B)
             if rope is None:
-                return B, S, N, dev, pages, kv, 16 * per, D, g, heads, width, None, None, 0
-            return B, S, N, dev, pages, kv, 16 * per, D, g, heads, width, cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+                if ok:
+                    return B, S, N, dev, pages, kv, 16 * per, D, g, heads, width, None, None, 0
+            elif ok:
+                cos, sin = rope
+                if _is(cos, _F16, 2, dev) and _is(sin, _F16, 2, dev) and cos.shape == sin.shape and cos.shape[1] == D:
+                    return B, S, N, dev, pages, kv, 16 * per, D, g, heads, width, cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    except AttributeError:
+        pass
     if x is not None:
         _check_tensor(x, "qkv", dtype=torch.float16, dims=x_dims)
     pages, kv, page, D, g = _pool_shape(pool)
@@ -118,7 +113,7 @@ def _call_shape(x, x_dims, pool, table, pos, counts, rope, heads, row_parts):
 def _output(out, shape, like):
     if out is None:
         return torch.zeros(shape, dtype=torch.float16, device=like.device)
-    if not (_is(out, torch.float16, len(shape), like.get_device()) and out.shape == shape):
+    if not (isinstance(out, torch.Tensor) and _is(out, _F16, len(shape), like.get_device()) and out.shape == shape):
         _check_tensor(out, "out", dtype=torch.float16)
         _need(tuple(out.shape) == shape and out.device == like.device, f"Tensor out must have shape {list(shape)}")
     return out
@@ -126,7 +121,7 @@ def _output(out, shape, like):
 
 def _guarded(dev, fn, *args):
     """fn on CUDA device `dev` with the current stream behind the arguments."""
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     with torch.cuda.device(dev):
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
@@ -199,71 +194,82 @@ def kv4_attention(qkv, pool, table, pos, heads: int, rope=None, scale=None, coun
     return out
 
 
-def _bookkeeping(table, refs, lens):
+def _book_device(table, lens, refs, ints=(), pool=None) -> int:
+    """The device of a call on page tables, all arguments checked: table int32 [rows, width], lens int32 [rows] or None, refs int32 [pages]
+    (as many as the pool has), `ints` int32 vectors with their lengths (None: any)."""
+    try:
+        dev = table.get_device()
+        ok = dev >= 0 and _is(table, _I32, 2, dev) and table.numel() and _is(refs, _I32, 1, dev) and \
+            (lens is None or _is(lens, _I32, 1, dev) and lens.shape[0] == table.shape[0]) and \
+            (pool is None or _is(pool, _U8, 5, dev) and pool.numel() and pool.shape[1] == refs.shape[0] and pool.shape[4] in _FORMATS)
+        for t, n, _ in ints:
+            ok = ok and _is(t, _I32, 1, dev) and (n is None or t.shape[0] == n)
+        if ok:
+            return dev
+    except AttributeError:
+        pass
     _check_tensor(table, "table", dtype=torch.int32, dims=2)
     dev = table.get_device()
     _need(table.numel() > 0, "table must not be empty")
     _ints(refs, "refs", dev)
     if lens is not None:
         _ints(lens, "lens", dev, numel=table.shape[0])
+    for t, n, name in ints:
+        _ints(t, name, dev, numel=n)
+    if pool is not None:
+        layers, pages = _pool_shape(pool, layers=True)[:2]
+        _need(pool.get_device() == dev and layers > 0, "all tensors must be on the same device")
+        _need(refs.numel() == pages, "refs must have an element for every page of the pool")
     return dev
 
 
 def kv4_reserve(table, lens, refs, counts, page_size: int):
     """Room for counts[r] (int32 [rows]) more tokens of every row: lens grow by them and the table gets the pages they need, lowest free
     numbers first.  Returns pos int32 [rows]: where the new tokens start, -1 for rows that asked for none or could not be served."""
-    dev = _bookkeeping(table, refs, lens)
+    dev = _book_device(table, lens, refs, ((counts, None, "counts"),))
     rows, width = table.shape
-    _ints(counts, "counts", dev, numel=rows)
+    _need(counts.shape[0] == rows, f"Tensor counts must have {rows} elements")
     pos = torch.empty_like(lens)
-    lib = load_library()
-    with _on(dev):
-        st = lib.w4a16_kv4_reserve(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), counts.data_ptr(), pos.data_ptr(), rows, width,
-                                   refs.numel(), int(page_size), _stream(table))
-    _check(st, "kv4_reserve")
+    st = _guarded(dev, load_library().w4a16_kv4_reserve, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), counts.data_ptr(), pos.data_ptr(), rows,
+                  width, refs.shape[0], int(page_size))
+    if st:
+        _check(st, "kv4_reserve")
     return pos
 
 
 def kv4_free(table, lens, refs, rows):
     """The rows (int32 [n]) give their pages back and are empty afterwards."""
-    dev = _bookkeeping(table, refs, lens)
-    _ints(rows, "rows", dev)
-    lib = load_library()
-    with _on(dev):
-        st = lib.w4a16_kv4_free(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), rows.data_ptr(), rows.numel(), table.shape[0],
-                                table.shape[1], refs.numel(), _stream(table))
-    _check(st, "kv4_free")
+    dev = _book_device(table, lens, refs, ((rows, None, "rows"),))
+    st = _guarded(dev, load_library().w4a16_kv4_free, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), rows.data_ptr(), rows.shape[0],
+                  table.shape[0], table.shape[1], refs.shape[0])
+    if st:
+        _check(st, "kv4_free")
 
 
 def kv4_fork(pool, table, lens, refs, src, dst):
     """Row dst[i] (empty) continues row src[i] (int32 [n] both): whole pages are shared, the last, partly filled one is copied in every
     layer.  pool: the whole [layers, pages, kv_heads, page_size / 16, tile bytes]."""
-    layers, pages, kv, page, D, g = _pool_shape(pool, layers=True)
-    dev = _bookkeeping(table, refs, lens)
-    _need(pool.get_device() == dev and layers > 0, "all tensors must be on the same device")
-    _need(refs.numel() == pages, "refs must have an element for every page of the pool")
-    _ints(src, "src", dev)
-    _ints(dst, "dst", dev, numel=src.numel())
-    lib = load_library()
-    n, (rows, width) = src.numel(), table.shape
+    dev = _book_device(table, lens, refs, ((src, None, "src"), (dst, None, "dst")), pool)
+    layers, pages, kv, per, tile = pool.shape
+    D, g = _FORMATS[tile]
+    n, (rows, width) = src.shape[0], table.shape
+    _need(dst.shape[0] == n, f"Tensor dst must have {n} elements")
     if n == 0:
         return
-    ws = torch.empty(lib.w4a16_kv4_fork_workspace(n, rows), dtype=torch.uint8, device=pool.device)
-    with _on(dev):
-        st = lib.w4a16_kv4_fork(pool.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(),
-                                ws.data_ptr(), ws.numel(), n, rows, width, layers, pages, kv, D, g, page, _stream(pool))
-    _check(st, "kv4_fork")
+    ws = torch.empty(4 * (4 * n + rows), dtype=torch.uint8, device=pool.device)          # w4a16_kv4_fork_workspace
+    st = _guarded(dev, load_library().w4a16_kv4_fork, pool.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(),
+                  dst.data_ptr(), ws.data_ptr(), ws.shape[0], n, rows, width, layers, pages, kv, D, g, 16 * per)
+    if st:
+        _check(st, "kv4_fork")
 
 
 def kv4_compact(pool, table, refs):
     """The pages in use become the pool's first ones (their contents move in every layer, table and refs follow)."""
-    layers, pages, kv, page, D, g = _pool_shape(pool, layers=True)
-    dev = _bookkeeping(table, refs, None)
-    _need(pool.get_device() == dev and layers > 0, "all tensors must be on the same device")
-    _need(refs.numel() == pages, "refs must have an element for every page of the pool")
-    lib = load_library()
-    ws = torch.empty(lib.w4a16_kv4_compact_workspace(pages), dtype=torch.uint8, device=pool.device)
-    with _on(dev):
-        st = lib.w4a16_kv4_compact(pool.data_ptr(), table.data_ptr(), refs.data_ptr(), ws.data_ptr(), ws.numel(), table.shape[0],
-                                   table.shape[1], layers, pages, kv, D, g, page, _stream(pool))
-    _check(st, "kv4_compact")
+    dev = _book_device(table, None, refs, (), pool)
+    layers, pages, kv, per, tile = pool.shape
+    D, g = _FORMATS[tile]
+    ws = torch.empty(4 * (3 * pages + 2), dtype=torch.uint8, device=pool.device)         # w4a16_kv4_compact_workspace
+    st = _guarded(dev, load_library().w4a16_kv4_compact, pool.data_ptr(), table.data_ptr(), refs.data_ptr(), ws.data_ptr(), ws.shape[0],
+                  table.shape[0], table.shape[1], layers, pages, kv, D, g, 16 * per)
+    if st:
+        _check(st, "kv4_compact")
