@@ -353,7 +353,7 @@ int w4a16_kv4_read(const void* pool, const void* table, const void* pos, const v
  * out fp16 [batch][heads*head_dim], 16-byte aligned.  q is rotated and rounded to fp16; scores, softmax and sums are fp32.  The work
  * of all rows is dealt evenly to the GPU and joined through a workspace of w4a16_kv4_decode_workspace bytes (0 for narrow tables; 16-byte
  * aligned, not shared by calls in flight). */
-size_t w4a16_kv4_decode_workspace(int batch, int heads, int kv_heads, int head_dim, int page_size, int width);
+size_t w4a16_kv4_decode_workspace(int batch, int heads, int kv_heads, int head_dim, int group, int page_size, int width);
 int w4a16_kv4_decode_attention(const void* qkv, void* pool, const void* table, const void* pos, const void* rope_cos,
                                const void* rope_sin, void* out, void* workspace, size_t workspace_bytes, int batch, int heads, int kv_heads, int head_dim, int group,
                                int page_size, int pages, int width, long long qkv_stride, int rope_rows, float scale, void* stream);

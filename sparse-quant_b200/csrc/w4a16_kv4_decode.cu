@@ -18,9 +18,13 @@
 // of its own in shared memory (16-byte asynchronous copies; two adjacent tiles are one run, from pages of 32 tokens on), across segments.
 // (Copies by one lane in bulk cost three times the instructions here: the loop is bound by what the warps can issue.)
 //
-// Queries that share the key/value head are the 8 columns of mma.m16n8k16:
+// Queries that share the key/value head are columns of mma.m16n8k16:
 //     scores  A = keys (16 tokens x 16 dims), B = queries;   output  A = values^T (16 dims x 16 tokens), B = weights
-// and the accumulator of the first is the layout the second needs after an 8x8 transpose (movmatrix).  Weights are 2^(score - ref)
+// and the accumulator of the first is the layout the second needs after an 8x8 transpose (movmatrix).  A weight p s depends on the group
+// of the dim.  Where the eight columns hold all (head, group) pairs (kSplit: up to 4 heads, 2 in groups of 32 of 128 dims) one product
+// runs with all of them and each dim takes the column of its group at the end: values then come transposed from a matrix load, whatever
+// groups its rows mix, and a lane has one score a token instead of two.  Otherwise the columns are 8 heads and a group of dims has its
+// own weights.  Weights are 2^(score - ref)
 // with ref = maximum + log2 of the largest step, moved only when a score exceeds the maximum by 2^8 or a step the largest by 2^5.
 #include "w4a16_kv4.cuh"
 
@@ -29,7 +33,8 @@ namespace kv4 {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kCols = 8;                          // query heads of one pass
+constexpr int kCols = 8;                          // columns of a product
+constexpr int kStages = 2;                        // chunks of a warp's ring (three left no room for a cache beside the shared memory: slower)
 constexpr int kChunk = 2 * kTile;                 // tokens
 constexpr int kStart = 2;                         // what a segment costs besides its chunks (queries, result), in chunks
 constexpr int kLeast = 4;                         // a warp's share of the line at least, in chunks
@@ -46,9 +51,10 @@ struct DecodeArgs {
     int4* split_units;         // [warps]: (row, unit, warps that have a part of it, 0) of the unit that starts in the warp's stretch and ends behind it
     float* part;                  // [warps][2][columns][D + 4]: of the unit that starts before the stretch, and of the one that ends behind it
     int batch, heads, share;      // share: query heads of a key/value head
-    int blocks, units;            // passes of 8 query heads over a key/value head; kv heads * blocks: units of a row
-    int cols;                     // min(8, share)
-    int rope_rows, stages;
+    int per_pass;                 // query heads of a unit: 8, or as many as have columns for all their groups
+    int blocks, units;            // passes over a key/value head; kv heads * blocks: units of a row
+    int cols;                     // min(per_pass, share)
+    int rope_rows;
     long long stride, page_bytes;
     float scale_log2;             // scale * log2(e)
 };
@@ -167,18 +173,30 @@ struct Layout {                   // shared memory of a warp: ring, then queries
     static constexpr int kHead = kQPitch * 16 + (F::NG + 1) * 4 + (16 - (F::NG + 1) * 4 % 16) % 16;
     static constexpr int kStage = 2 * F::kBytes;
     static constexpr int kPitch = D + 4;                                        // floats of an output row where warps meet
-    static __host__ __device__ constexpr int warp_bytes(int stages, int cols) { return (stages * kStage + cols * kHead + 63) / 64 * 64; }
+    static __host__ __device__ constexpr int warp_bytes(int cols) { return (kStages * kStage + cols * kHead + 63) / 64 * 64; }
 };
+__host__ __device__ constexpr int split_columns(int NG) { return NG < 2 ? 2 : NG; }               // of a head, kSplit
 
-template <class F, int D>
+template <int J>
+__device__ __forceinline__ void load_transposed(uint32_t from, uint32_t (&w)[J])
+{
+    static_assert(J == 4, "four matrices");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+}
+
+template <class F, int D, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
 {
     using L = Layout<F, D>;
     constexpr int J = F::J, NG = F::NG, kBytes = F::kBytes, kPitch = L::kPitch;
+    constexpr int NC = split_columns(NG);         // kSplit: columns of a head
+    constexpr int KC = kSplit ? 1 : 2;            // heads of a lane
+    constexpr int OG = kSplit ? 1 : NG;           // groups of dims whose weights are separate operands
     extern __shared__ __align__(128) unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c4 = lane & 3;
-    unsigned char* ring = raw + warp * L::warp_bytes(a.stages, a.cols);
-    uint4* q_s = reinterpret_cast<uint4*>(ring + a.stages * L::kStage);
+    unsigned char* ring = raw + warp * L::warp_bytes(a.cols);
+    uint4* q_s = reinterpret_cast<uint4*>(ring + kStages * L::kStage);
     float* qsum_s = reinterpret_cast<float*>(q_s + a.cols * L::kQPitch);        // [columns][NG], then unit [columns]
     float* unit_s = qsum_s + a.cols * NG;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -278,22 +296,24 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
             ++at;
             look();
         }
-        there_q |= there << (2 * a.stages);                                     // (shifted down by two when the next chunk is taken)
+        there_q |= there << (2 * kStages);                                     // (shifted down by two when the next chunk is taken)
         copies_issued();
     };
     enter();
     look();
-    for (int i = 0; i < a.stages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
         there_q >>= 2;
         fetch(i);
     }
     there_q >>= 2;
 
-    const int t0 = token_of(row), kcol = min(row, a.cols - 1);                  // columns that no head stands in repeat the last one
+    const int t0 = kSplit ? row : token_of(row);                                // the token of fragment row `row`
+    const int kcol = min(kSplit ? row / NC : row, a.cols - 1);                  // columns that no head stands in repeat the last one
+    const int head_k = kSplit ? 2 * c4 / NC : 2 * c4;                           // the lane's (first) head of the pass
     int stage = 0;
     for (;;) {
         const int b = line.b, kvh = line.unit / a.blocks, hb = line.unit % a.blocks, pos = a.pos[b];
-        const int cols = min(kCols, a.share - hb * kCols), head0 = kvh * a.share + hb * kCols;
+        const int cols = min(a.per_pass, a.share - hb * a.per_pass), head0 = kvh * a.share + hb * a.per_pass;
         if (line.lo < line.hi) {
             // ---- queries to shared memory, as B fragments: head n, word w of 8 dims -> low nibbles' dims (0,4)(2,6), high nibbles'
             // (1,5)(3,7) / 16, of q times the power of two that brings its largest element into [2^14, 2^15): a sixteenth is then
@@ -322,17 +342,17 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
             }
             __syncwarp();
         }
-        float qsum[NG][2], unit[2];
+        float qsum[NG][KC], unit[KC];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int n = min(2 * c4 + k, a.cols - 1);
+        for (int k = 0; k < KC; ++k) {
+            const int n = min(head_k + k, a.cols - 1);
             unit[k] = unit_s[n];
 #pragma unroll
             for (int g = 0; g < NG; ++g) qsum[g][k] = qsum_s[n * NG + g];
         }
         float acc[J][2][4];                                                     // [32 dims][pair of dims of a half-word][fragment]
-        float off[NG][2];                                                       // the minima's part
-        float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+        float off[OG][2];                                                       // the minima's part: by group and head, or (kSplit) the lane's columns
+        float ref[KC], sum[KC];
         int elog = -24;                                                         // steps are below 2^(elog + 5)
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -341,12 +361,16 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[j][e][i] = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) off[g][0] = off[g][1] = 0.f;
+        for (int g = 0; g < OG; ++g) off[g][0] = off[g][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            ref[k] = -INFINITY;
+            sum[k] = 0.f;
+        }
 
         for (int t = line.lo; t < line.hi; ++t) {
             unsigned char* chunk = ring + stage * L::kStage;
-            if (a.stages == 3) copies_wait<2>();
-            else copies_wait<1>();
+            copies_wait<kStages - 1>();
             __syncwarp();
             const int there = there_q & 3;
             const int left = pos + 1 - t * kChunk;                              // tokens from the chunk's first on
@@ -383,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
             }
             if (count0 > 0 || count1 > 0) {
                 // scores: fragment rows are the tokens t0 and t0 + 8 of a tile, columns the heads 2 c and 2 c + 1
-                float x[2][4];
+                float x[2][2 * KC];                                             // [tile][row half * KC + head]
                 uint32_t ka[2][J], kb[2][J];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -418,9 +442,9 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                         const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(chunk + u * kBytes + F::key_par(t0, g)));
                         const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(chunk + u * kBytes + F::key_par(t0 + 8, g)));
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
+                        for (int k = 0; k < KC; ++k) {
                             x[u][k] = fmaf(fa.x, s4[u][k], g ? fmaf(fa.y, qsum[g][k], x[u][k]) : fa.y * qsum[g][k]);
-                            x[u][2 + k] = fmaf(fb.x, s4[u][2 + k], g ? fmaf(fb.y, qsum[g][k], x[u][2 + k]) : fb.y * qsum[g][k]);
+                            x[u][KC + k] = fmaf(fb.x, s4[u][2 + k], g ? fmaf(fb.y, qsum[g][k], x[u][KC + k]) : fb.y * qsum[g][k]);
                         }
                     }
                 }
@@ -435,12 +459,14 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                     for (int u = 0; u < 2; ++u) {
                         const int count = u ? count1 : count0;
                         if (t0 >= count) {
-                            x[u][0] = x[u][1] = -INFINITY;
+#pragma unroll
+                            for (int k = 0; k < KC; ++k) x[u][k] = -INFINITY;
 #pragma unroll
                             for (int g = 0; g < NG; ++g) va[u][g] = __half2half2(__ushort_as_half(0));
                         }
                         if (t0 + 8 >= count) {
-                            x[u][2] = x[u][3] = -INFINITY;
+#pragma unroll
+                            for (int k = 0; k < KC; ++k) x[u][KC + k] = -INFINITY;
 #pragma unroll
                             for (int g = 0; g < NG; ++g) vb[u][g] = __half2half2(__ushort_as_half(0));
                         }
@@ -453,27 +479,38 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                     for (int g = 0; g < NG; ++g)
                         if (u || g) big = __hmax2(big, __hmax2(va[u][g], vb[u][g]));
                 float smax = __low2float(big);
-                const float m0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])) * unit[0];
-                const float m1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3])) * unit[1];
+                float m[KC];
+                bool move = smax > pow2(elog + 5);
                 const float room = 8.f - (float)elog;
-                if (__any_sync(0xffffffffu, m0 - ref[0] > room || m1 - ref[1] > room || smax > pow2(elog + 5))) {
-                    float n0 = fmaxf(m0, ref[0] - (float)elog), n1 = fmaxf(m1, ref[1] - (float)elog);
+#pragma unroll
+                for (int k = 0; k < KC; ++k) {
+                    m[k] = fmaxf(fmaxf(x[0][k], x[0][KC + k]), fmaxf(x[1][k], x[1][KC + k])) * unit[k];
+                    move |= m[k] - ref[k] > room;
+                }
+                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int k = 0; k < KC; ++k) m[k] = fmaxf(m[k], ref[k] - (float)elog);
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
-                        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-                        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+#pragma unroll
+                        for (int k = 0; k < KC; ++k) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
                         smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
                     }
                     if (smax > pow2(elog + 5)) elog = exponent(fminf(smax, 65504.f));
-                    const float r0 = n0 + (float)elog, r1 = n1 + (float)elog;
-                    const float keep[2] = {ref[0] == -INFINITY ? 0.f : ex2(ref[0] - r0), ref[1] == -INFINITY ? 0.f : ex2(ref[1] - r1)};
-                    ref[0] = r0;
-                    ref[1] = r1;
+                    float keep[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        sum[k] *= keep[k];
+                        const int h = kSplit ? 0 : k;
+                        if (!kSplit || k == 0) {
+                            const float to = m[h] + (float)elog;
+                            keep[k] = ref[h] == -INFINITY ? 0.f : ex2(ref[h] - to);
+                            ref[h] = to;
+                            sum[h] *= keep[k];
+                        } else {
+                            keep[k] = keep[0];
+                        }
 #pragma unroll
-                        for (int g = 0; g < NG; ++g) off[g][k] *= keep[k];
+                        for (int g = 0; g < OG; ++g) off[g][k] *= keep[k];
 #pragma unroll
                         for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -486,68 +523,119 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const unsigned char* tile = chunk + u * kBytes;
-                    float p[4];
+                    float p[2 * KC];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(x[u][k], unit[k & 1], -ref[k & 1]));
-                    sum[0] += p[0] + p[2];
-                    sum[1] += p[1] + p[3];
-                    uint32_t wf[NG][2];                                         // B fragments: tokens 2c, 2c+1 (+ 8) of column lane / 4
+                    for (int k = 0; k < 2 * KC; ++k) p[k] = ex2(fmaf(x[u][k], unit[k % KC], -ref[k % KC]));
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float2 fa = __half22float2(va[u][g]), fb = __half22float2(vb[u][g]);
-                        wf[g][0] = transpose8x8(pack2(p[0] * fa.x, p[1] * fa.x));
-                        wf[g][1] = transpose8x8(pack2(p[2] * fb.x, p[3] * fb.x));
+                    for (int k = 0; k < KC; ++k) sum[k] += p[k] + p[KC + k];
+                    if constexpr (kSplit) {
+                        // the lane's columns are groups ga and ga + 1 of its head (one group alone: its second column is empty)
+                        const int ga = 2 * c4 % NC;
+                        const float2 fa = __half22float2(NC == 4 && ga ? va[u][2 % NG] : va[u][0]), fb = __half22float2(NC == 4 && ga ? vb[u][2 % NG] : vb[u][0]);
+                        float2 ga1 = make_float2(0.f, 0.f), gb1 = ga1;
+                        if constexpr (NG > 1) {
+                            ga1 = __half22float2(NC == 4 && ga ? va[u][3 % NG] : va[u][1]);
+                            gb1 = __half22float2(NC == 4 && ga ? vb[u][3 % NG] : vb[u][1]);
+                        }
+                        const uint32_t w0 = transpose8x8(pack2(p[0] * fa.x, p[0] * ga1.x)), w1 = transpose8x8(pack2(p[1] * fb.x, p[1] * gb1.x));
+                        off[0][0] = fmaf(p[0], fa.y, fmaf(p[1], fb.y, off[0][0]));
+                        if constexpr (NG > 1) off[0][1] = fmaf(p[0], ga1.y, fmaf(p[1], gb1.y, off[0][1]));
+                        // output: fragment rows are dims 4 h + 2 e and the next one of half-word h = 8 j + row of the cache's order
+                        uint32_t v[2][J];
+                        if constexpr (J == 4) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) off[g][k] = fmaf(p[k], fa.y, fmaf(p[2 + k], fb.y, off[g][k]));
-                    }
-                    // output: fragment rows are dims 32 j + 4 row + 2 e and the next one
-                    uint32_t v[4][J / 2];
+                            for (int k = 0; k < 2; ++k) {
+                                const int lr = 8 * k + (lane & 7), piece = (lane >> 3) ^ (((lr >> 1) & 1) << 1);
+                                load_transposed(smem_u32(tile + F::kVal + lr * (D / 2) + 16 * piece), v[k]);
+                            }
+                        } else {
+                            uint32_t both[4];
+                            load_transposed(smem_u32(tile + F::kVal + (8 * (lane >> 4) + (lane & 7)) * (D / 2) + 16 * ((lane >> 3) & 1)), both);
+                            v[0][0] = both[0]; v[0][1] = both[1]; v[1][0] = both[2]; v[1][1] = both[3];
+                        }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int tk = token_of(2 * c4 + (k & 1)) + 8 * (k >> 1);
-                        const unsigned char* vat = tile + F::kVal + tk * (D / 2) + (D == 128 ? (8 * row) ^ (((tk >> 1) & 1) << 5) : 4 * row);
-                        if constexpr (J == 4) *reinterpret_cast<uint2*>(v[k]) = *reinterpret_cast<const uint2*>(vat);
-                        else v[k][0] = *reinterpret_cast<const uint32_t*>(vat);
-                    }
+                        for (int j = 0; j < J; ++j) {
+                            uint32_t h0[4], h1[4];
+                            unpack_s4x8_denorm(v[0][j], h0);
+                            unpack_s4x8_denorm(v[1][j], h1);
+                            const uint32_t f0[4] = {h0[0], h0[1], h1[0], h1[1]}, f1[4] = {h0[2], h0[3], h1[2], h1[3]};
+                            mma_m16n8k16(acc[j][0], f0, w0, w1);
+                            mma_m16n8k16(acc[j][1], f1, w0, w1);
+                        }
+                    } else {
+                        uint32_t wf[NG][2];                                     // B fragments: tokens 2c, 2c+1 (+ 8) of column lane / 4
 #pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        const uint32_t u0 = __byte_perm(v[0][j / 2], v[1][j / 2], j & 1 ? 0x7632 : 0x5410);
-                        const uint32_t u1 = __byte_perm(v[2][j / 2], v[3][j / 2], j & 1 ? 0x7632 : 0x5410);
-                        uint32_t h0[4], h1[4];
-                        unpack_s4x8_denorm(u0, h0);
-                        unpack_s4x8_denorm(u1, h1);
-                        const uint32_t f0[4] = {h0[0], h0[1], h1[0], h1[1]}, f1[4] = {h0[2], h0[3], h1[2], h1[3]};
-                        constexpr int per = D / NG;
-                        mma_m16n8k16(acc[j][0], f0, wf[32 * j / per][0], wf[32 * j / per][1]);
-                        mma_m16n8k16(acc[j][1], f1, wf[32 * j / per][0], wf[32 * j / per][1]);
+                        for (int g = 0; g < NG; ++g) {
+                            const float2 fa = __half22float2(va[u][g]), fb = __half22float2(vb[u][g]);
+                            wf[g][0] = transpose8x8(pack2(p[0] * fa.x, p[KC - 1] * fa.x));
+                            wf[g][1] = transpose8x8(pack2(p[KC] * fb.x, p[2 * KC - 1] * fb.x));
+#pragma unroll
+                            for (int k = 0; k < KC; ++k) off[g][k] = fmaf(p[k], fa.y, fmaf(p[KC + k], fb.y, off[g][k]));
+                        }
+                        // output: fragment rows are dims 32 j + 4 row + 2 e and the next one
+                        uint32_t v[4][J / 2];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int tk = token_of(2 * c4 + (k & 1)) + 8 * (k >> 1);
+                            const unsigned char* vat = tile + F::kVal + tk * (D / 2) + (D == 128 ? (8 * row) ^ (((tk >> 1) & 1) << 5) : 4 * row);
+                            if constexpr (J == 4) *reinterpret_cast<uint2*>(v[k]) = *reinterpret_cast<const uint2*>(vat);
+                            else v[k][0] = *reinterpret_cast<const uint32_t*>(vat);
+                        }
+#pragma unroll
+                        for (int j = 0; j < J; ++j) {
+                            const uint32_t u0 = __byte_perm(v[0][j / 2], v[1][j / 2], j & 1 ? 0x7632 : 0x5410);
+                            const uint32_t u1 = __byte_perm(v[2][j / 2], v[3][j / 2], j & 1 ? 0x7632 : 0x5410);
+                            uint32_t h0[4], h1[4];
+                            unpack_s4x8_denorm(u0, h0);
+                            unpack_s4x8_denorm(u1, h1);
+                            const uint32_t f0[4] = {h0[0], h0[1], h1[0], h1[1]}, f1[4] = {h0[2], h0[3], h1[2], h1[3]};
+                            constexpr int per = D / NG;
+                            mma_m16n8k16(acc[j][0], f0, wf[32 * j / per][0], wf[32 * j / per][1]);
+                            mma_m16n8k16(acc[j][1], f1, wf[32 * j / per][0], wf[32 * j / per][1]);
+                        }
                     }
                 }
             }
             __syncwarp();                                                       // everybody has read the chunk
             fetch(stage);
             there_q >>= 2;
-            if (++stage == a.stages) stage = 0;
+            stage ^= 1;
         }
 
-        // ---- the segment's result: dims 32 j + 4 row .. + 3 of columns 2 c and 2 c + 1
+        // ---- the segment's result: four dims of column k in acc[j][.][k]
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int o = 4; o < 32; o <<= 1) {
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+            for (int k = 0; k < KC; ++k) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) off[g][k] += __shfl_xor_sync(0xffffffffu, off[g][k], o);
-            }
+            for (int g = 0; g < OG; ++g)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) off[g][k] += __shfl_xor_sync(0xffffffffu, off[g][k], o);
+        }
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
             if (sum[k] != sum[k]) ref[k] = sum[k];                              // NaN scores: not to be taken for "no chunks"
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const float o = off[32 * j * NG / D][k];
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float o = off[kSplit ? 0 : 32 * j * NG / D][k];
                 acc[j][0][k] = fmaf(acc[j][0][k], kDenormScaleLo, o);
                 acc[j][0][2 + k] = fmaf(acc[j][0][2 + k], kDenormScaleHi, o);
                 acc[j][1][k] = fmaf(acc[j][1][k], kDenormScaleLo, o);
                 acc[j][1][2 + k] = fmaf(acc[j][1][2 + k], kDenormScaleHi, o);
             }
-        }
+        // the lane's heads, whether it holds the columns of its dims' group, and where its four dims of 32 j stand: at D dims a half-word
+        // 8 j + row of the cache's order is dims 32 (row % J) + 4 (8 j + row) / J .. + 3 (kSplit), or 32 j + 4 row .. + 3
+        const int own_group = 32 * (row % J) * NG / D, lane_col = own_group - 2 * c4 % NC;
+        const bool holds = !kSplit || lane_col == 0 || (lane_col == 1 && NC > 1);
+        auto dims_at = [&](int j) { return kSplit ? 32 * (row % J) + 4 * ((8 * j + row) / J) : 32 * j + 4 * row; };
+        auto value4 = [&](int j, int k) {
+            const bool second = kSplit ? lane_col == 1 : k == 1;
+            return make_float4(second ? acc[j][0][1] : acc[j][0][0], second ? acc[j][0][3] : acc[j][0][2], second ? acc[j][1][1] : acc[j][1][0],
+                               second ? acc[j][1][3] : acc[j][1][2]);
+        };
+        const bool tells = row == 0 && (!kSplit || 2 * c4 % NC == 0);           // the lane that leaves the head's reference and sum
         const bool starts = line.lo == 0 && line.hi > 0, whole = starts && line.hi == line.n;
         // the warps that a unit starting here is dealt to, this one first: its last chunk stands n - hi behind the segment's end
         auto dealt = [&]() {
@@ -557,20 +645,24 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
         if (!together) {
             if (line.lo < line.hi) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (2 * c4 + k >= cols) continue;
+                for (int k = 0; k < KC; ++k) {
+                    if (head_k + k >= cols) continue;
                     if (whole) {
                         const float l = sum[k] == 0.f ? 0.f : 1.f / sum[k];
-                        __half* to = a.out + ((size_t)b * a.heads + head0 + 2 * c4 + k) * D + 4 * row;
+                        __half* to = a.out + ((size_t)b * a.heads + head0 + head_k + k) * D;
 #pragma unroll
-                        for (int j = 0; j < J; ++j)
-                            *reinterpret_cast<uint2*>(to + 32 * j) = make_uint2(pack2(acc[j][0][k] * l, acc[j][0][2 + k] * l), pack2(acc[j][1][k] * l, acc[j][1][2 + k] * l));
+                        for (int j = 0; j < J; ++j) {
+                            const float4 v = value4(j, k);
+                            if (holds) *reinterpret_cast<uint2*>(to + dims_at(j)) = make_uint2(pack2(v.x * l, v.y * l), pack2(v.z * l, v.w * l));
+                        }
                     } else {
-                        float* to = a.part + ((me * 2 + starts) * a.cols + 2 * c4 + k) * (D + 4);
+                        float* to = a.part + ((me * 2 + starts) * a.cols + head_k + k) * (D + 4);
 #pragma unroll
-                        for (int j = 0; j < J; ++j)
-                            *reinterpret_cast<float4*>(to + 32 * j + 4 * row) = make_float4(acc[j][0][k], acc[j][0][2 + k], acc[j][1][k], acc[j][1][2 + k]);
-                        if (row == 0) *reinterpret_cast<float2*>(to + D) = make_float2(ref[k], sum[k]);
+                        for (int j = 0; j < J; ++j) {
+                            const float4 v = value4(j, k);
+                            if (holds) *reinterpret_cast<float4*>(to + dims_at(j)) = v;
+                        }
+                        if (tells) *reinterpret_cast<float2*>(to + D) = make_float2(ref[k], sum[k]);
                     }
                 }
                 if (starts && !whole) split_unit = dealt();
@@ -586,13 +678,15 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
         float* meet = reinterpret_cast<float*>(raw);                            // [warps][columns][kPitch], reference and sum behind the dims
         int* ends = reinterpret_cast<int*>(meet + kWarps * a.cols * kPitch);    // [warps]: chunks of the unit up to the warp's, -1: none of its own
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (2 * c4 + k >= cols) continue;
-            float* to = meet + (warp * a.cols + 2 * c4 + k) * kPitch;
+        for (int k = 0; k < KC; ++k) {
+            if (head_k + k >= cols) continue;
+            float* to = meet + (warp * a.cols + head_k + k) * kPitch;
 #pragma unroll
-            for (int j = 0; j < J; ++j)
-                *reinterpret_cast<float4*>(to + 32 * j + 4 * row) = make_float4(acc[j][0][k], acc[j][0][2 + k], acc[j][1][k], acc[j][1][2 + k]);
-            if (row == 0) *reinterpret_cast<float2*>(to + D) = make_float2(ref[k], sum[k]);
+            for (int j = 0; j < J; ++j) {
+                const float4 v = value4(j, k);
+                if (holds) *reinterpret_cast<float4*>(to + dims_at(j)) = v;
+            }
+            if (tells) *reinterpret_cast<float2*>(to + D) = make_float2(ref[k], sum[k]);
         }
         if (lane == 0) {
             ends[warp] = line.lo < line.hi ? line.hi : -1;
@@ -651,10 +745,10 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a, int warps
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int me = blockIdx.x * 8 + warp;
     int4 u = me < warps ? a.split_units[me] : make_int4(0, 0, 0, 0);
-    if (u.y % a.blocks * kCols + col >= a.share) u.z = 0;                       // a pass of fewer heads
+    if (u.y % a.blocks * a.per_pass + col >= a.share) u.z = 0;                       // a pass of fewer heads
     auto part = [&](int first, int i) { return a.part + (((first + (long long)i) * 2 + (i == 0)) * a.cols + col) * (D + 4); };
     auto out = [&](const int4& u) {
-        return a.out + ((size_t)u.x * a.heads + u.y / a.blocks * a.share + u.y % a.blocks * kCols + col) * D;
+        return a.out + ((size_t)u.x * a.heads + u.y / a.blocks * a.share + u.y % a.blocks * a.per_pass + col) * D;
     };
     if (lane == 0) many[warp] = make_int4(u.x, u.y, u.z > kFew ? u.z : 0, me);
     if (u.z > 0 && u.z <= kFew) {
@@ -743,7 +837,14 @@ int decode_ctas(int batch, int units, int page_size, int width)
     return longest * waves <= 40 ? 0 : (int)slots;
 }
 
-template <class F, int D>
+// Query heads of a unit: as many as have columns for all their groups, where that takes no more passes than 8 heads a pass.
+int heads_per_pass(int share, int head_dim, int group)
+{
+    const int split = kCols / split_columns(head_dim / group);
+    return share <= split ? split : kCols;
+}
+
+template <class F, int D, bool kSplit>
 static int launch_decode_as(DecodeArgs& a, int ctas, cudaStream_t st)
 {
     using L = Layout<F, D>;
@@ -752,25 +853,24 @@ static int launch_decode_as(DecodeArgs& a, int ctas, cudaStream_t st)
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(decode_kernel<F, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem4);
+        e = cudaFuncSetAttribute(decode_kernel<F, D, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem4);
         if (e != cudaSuccess) return record_cuda_error(e);
         if (dev < 64) configured[dev] = 1;
     }
-    static_assert(kWarps * L::warp_bytes(2, kCols) <= kSmem4, "two stages fit");
-    static_assert(kWarps * kCols * L::kPitch * 4 + 2 * kWarps * 4 <= kWarps * L::warp_bytes(2, kCols) &&
-                  kWarps * L::kPitch * 4 + 2 * kWarps * 4 <= kWarps * L::warp_bytes(2, 1), "the warps' results fit where the rings were");
-    a.stages = kWarps * L::warp_bytes(3, a.cols) <= kSmem4 ? 3 : 2;
+    static_assert(kWarps * L::warp_bytes(kCols) <= kSmem4, "four CTAs fit an SM");
+    static_assert(kWarps * kCols * L::kPitch * 4 + 2 * kWarps * 4 <= kWarps * L::warp_bytes(kCols) &&
+                  kWarps * L::kPitch * 4 + 2 * kWarps * 4 <= kWarps * L::warp_bytes(1), "the warps' results fit where the rings were");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas ? ctas : a.units * a.batch);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kWarps * L::warp_bytes(a.stages, a.cols);
+    cfg.dynamicSmemBytes = kWarps * L::warp_bytes(a.cols);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = aux_programmatic_launch() ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, decode_kernel<F, D>, (const DecodeArgs)a);
+    e = cudaLaunchKernelEx(&cfg, decode_kernel<F, D, kSplit>, (const DecodeArgs)a);
     if (e != cudaSuccess) return record_cuda_error(e);
     count_launch();
     if (ctas) {
@@ -794,11 +894,12 @@ using namespace w4a16::kv4;
 // Tuning hook for tests and benchmarks: CTAs of a call, 0 = automatic, negative: one per unit.  Not part of the drop-in surface.
 extern "C" void w4a16_tune_kv4(int ctas) { w4a16::kv4::g_force_ctas = ctas > 4096 ? 4096 : ctas; }
 
-extern "C" size_t w4a16_kv4_decode_workspace(int batch, int heads, int kv_heads, int head_dim, int page_size, int width)
+extern "C" size_t w4a16_kv4_decode_workspace(int batch, int heads, int kv_heads, int head_dim, int group, int page_size, int width)
 {
-    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || page_size <= 0 || width <= 0) return 0;
-    const int share = heads / kv_heads, cols = share < kCols ? share : kCols;
-    return (size_t)decode_ctas(batch, kv_heads * ((share + kCols - 1) / kCols), page_size, width) * kWarps * (sizeof(int4) + 2 * cols * (head_dim + 4) * sizeof(float));
+    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || w4a16_kv4_tile_bytes(head_dim, group) == 0 || page_size <= 0 || width <= 0)
+        return 0;
+    const int share = heads / kv_heads, per = heads_per_pass(share, head_dim, group), cols = share < per ? share : per;
+    return (size_t)decode_ctas(batch, kv_heads * ((share + per - 1) / per), page_size, width) * kWarps * (sizeof(int4) + 2 * cols * (head_dim + 4) * sizeof(float));
 }
 
 extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const void* table, const void* pos, const void* rope_cos,
@@ -817,8 +918,9 @@ extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const voi
         return W4A16_ERR_MISALIGNED;
     if ((heads + 2ll * kv_heads) * head_dim >= (1ll << 30) || batch > 65535) return W4A16_ERR_TOO_LARGE;
     a.share = heads / kv_heads;
-    a.blocks = (a.share + kCols - 1) / kCols;
-    a.cols = a.share < kCols ? a.share : kCols;
+    a.per_pass = heads_per_pass(a.share, head_dim, group);
+    a.blocks = (a.share + a.per_pass - 1) / a.per_pass;
+    a.cols = a.share < a.per_pass ? a.share : a.per_pass;
     a.units = kv_heads * a.blocks;
     if ((long long)a.units * batch >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
     if (batch == 0) return W4A16_OK;
@@ -826,7 +928,7 @@ extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const voi
     a.part = nullptr;
     a.split_units = nullptr;
     if (ctas) {
-        if (!workspace || workspace_bytes < w4a16_kv4_decode_workspace(batch, heads, kv_heads, head_dim, page_size, width)) return W4A16_ERR_WORKSPACE;
+        if (!workspace || workspace_bytes < w4a16_kv4_decode_workspace(batch, heads, kv_heads, head_dim, group, page_size, width)) return W4A16_ERR_WORKSPACE;
         a.split_units = (int4*)workspace;
         a.part = (float*)(a.split_units + (size_t)ctas * kWarps);
     }
@@ -839,6 +941,7 @@ extern "C" int w4a16_kv4_decode_attention(const void* qkv, void* pool, const voi
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        return launch_decode_as<F, F::NW * 8>(a, ctas, (cudaStream_t)stream);
+        return a.share <= kCols / split_columns(F::NG) ? launch_decode_as<F, F::NW * 8, true>(a, ctas, (cudaStream_t)stream)
+                                                         : launch_decode_as<F, F::NW * 8, false>(a, ctas, (cudaStream_t)stream);
     });
 }

@@ -90,7 +90,7 @@ C_ABI = {
     "w4a16_kv4_tile_bytes": (_sz, [_ci, _ci]),
     "w4a16_kv4_append": (_ci, [_vp] * 7 + [_ci] * 9 + [ctypes.c_longlong, _ci, _vp]),
     "w4a16_kv4_read": (_ci, [_vp] * 6 + [_ci] * 8 + [_vp]),
-    "w4a16_kv4_decode_workspace": (_sz, [_ci] * 6),
+    "w4a16_kv4_decode_workspace": (_sz, [_ci] * 7),
     "w4a16_tune_kv4": (None, [_ci]),
     "w4a16_kv4_decode_attention": (_ci, [_vp] * 8 + [_sz] + [_ci] * 8 + [ctypes.c_longlong, _ci, ctypes.c_float, _vp]),
     "w4a16_kv4_attention": (_ci, [_vp] * 8 + [_ci] * 9 + [ctypes.c_longlong, _ci, ctypes.c_float, _vp]),

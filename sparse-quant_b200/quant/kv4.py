@@ -166,7 +166,7 @@ def kv4_decode_attention(qkv, pool, table, pos, heads: int, rope=None, scale=Non
     if B == 0:
         return out
     lib = load_library()
-    ws, ws_bytes = None, lib.w4a16_kv4_decode_workspace(B, heads, kv, D, page, width)
+    ws, ws_bytes = None, lib.w4a16_kv4_decode_workspace(B, heads, kv, D, g, page, width)
     if ws_bytes:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
     st = _guarded(dev, lib.w4a16_kv4_decode_attention, qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(), cos, sin, out.data_ptr(),

@@ -62,8 +62,8 @@ def test_status_codes_of_cache_calls():
     assert read(k=None) == 1 and read(v=p + 2) == 4
     assert decode(out=None) == 1 and chunk(out=p + 2) == 4
     # rows over a wide table are dealt to the whole GPU: that needs a workspace
-    need = lib.w4a16_kv4_decode_workspace(1, 4, 2, 128, 16, 10000)
-    assert need > 0 and lib.w4a16_kv4_decode_workspace(64, 32, 32, 128, 16, 2) == 0
+    need = lib.w4a16_kv4_decode_workspace(1, 4, 2, 128, 64, 16, 10000)
+    assert need > 0 and lib.w4a16_kv4_decode_workspace(64, 32, 32, 128, 64, 16, 2) == 0
     assert decode(width=10000) == 5 and decode(width=10000, ws=p, ws_bytes=need - 1) == 5 and decode(width=10000, ws=p + 2, ws_bytes=need) == 4
     assert append(seq=0) == 0 and read(seq=0) == 0 and chunk(seq=0) == 0
     assert append(seq=-1) == 2 and read(seq=-1) == 2 and chunk(seq=-1) == 2
