@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
     constexpr int NC = split_columns(NG);         // kSplit: columns of a head
     constexpr int KC = kSplit ? 1 : 2;            // heads of a lane
     constexpr int OG = kSplit ? 1 : NG;           // groups of dims whose weights are separate operands
+    constexpr int kAtOnce = kSplit && NG < 4 ? 2 : 1;   // tiles side by side: two fill the waits of each other's chains, where registers allow
     extern __shared__ __align__(128) unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c4 = lane & 3;
     unsigned char* ring = raw + warp * L::warp_bytes(a.cols);
@@ -405,13 +406,17 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                     __syncwarp();
                 }
             }
-            if (count0 > 0 || count1 > 0) {
+#pragma unroll 1
+            for (int half = 0; half < 2; half += kAtOnce) {
+                const unsigned char* tiles = chunk + half * kBytes;
+                const int counts[2] = {half ? count1 : count0, count1};
+                if (counts[0] <= 0 && (kAtOnce == 1 || counts[1] <= 0)) continue;
                 // scores: fragment rows are the tokens t0 and t0 + 8 of a tile, columns the heads 2 c and 2 c + 1
-                float x[2][2 * KC];                                             // [tile][row half * KC + head]
-                uint32_t ka[2][J], kb[2][J];
+                float x[kAtOnce][2 * KC];                                             // [tile][row half * KC + head]
+                uint32_t ka[kAtOnce][J], kb[kAtOnce][J];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const unsigned char* tile = chunk + u * kBytes;
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const unsigned char* tile = tiles + u * kBytes;
                     if constexpr (J == 4) {
                         *reinterpret_cast<uint4*>(ka[u]) = *reinterpret_cast<const uint4*>(tile + t0 * (D / 2) + 16 * c4);
                         *reinterpret_cast<uint4*>(kb[u]) = *reinterpret_cast<const uint4*>(tile + (t0 + 8) * (D / 2) + 16 * c4);
@@ -422,12 +427,12 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                 }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    float s4[2][4];
+                    float s4[kAtOnce][4];
 #pragma unroll
                     for (int j = g * J / NG; j < (g + 1) * J / NG; ++j) {
                         const uint4 qf = q_s[kcol * L::kQPitch + 4 * j + c4];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < kAtOnce; ++u) {
                             uint32_t ha[4], hc[4];
                             unpack_s4x8_denorm(ka[u][j], ha);
                             unpack_s4x8_denorm(kb[u][j], hc);
@@ -438,9 +443,9 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                         }
                     }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(chunk + u * kBytes + F::key_par(t0, g)));
-                        const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(chunk + u * kBytes + F::key_par(t0 + 8, g)));
+                    for (int u = 0; u < kAtOnce; ++u) {
+                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(tiles + u * kBytes + F::key_par(t0, g)));
+                        const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(tiles + u * kBytes + F::key_par(t0 + 8, g)));
 #pragma unroll
                         for (int k = 0; k < KC; ++k) {
                             x[u][k] = fmaf(fa.x, s4[u][k], g ? fmaf(fa.y, qsum[g][k], x[u][k]) : fa.y * qsum[g][k]);
@@ -448,16 +453,16 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                         }
                     }
                 }
-                __half2 va[2][NG], vb[2][NG];                                   // (step, minimum) of the two tokens' values
+                __half2 va[kAtOnce][NG], vb[kAtOnce][NG];                                   // (step, minimum) of the two tokens' values
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    load_params<NG>(chunk + u * kBytes + F::val_par(t0, 0), va[u]);
-                    load_params<NG>(chunk + u * kBytes + F::val_par(t0 + 8, 0), vb[u]);
+                for (int u = 0; u < kAtOnce; ++u) {
+                    load_params<NG>(tiles + u * kBytes + F::val_par(t0, 0), va[u]);
+                    load_params<NG>(tiles + u * kBytes + F::val_par(t0 + 8, 0), vb[u]);
                 }
-                if (count0 < kTile || count1 < kTile) {                         // tokens behind the new one, pages that are none
+                if (counts[0] < kTile || (kAtOnce == 2 && counts[1] < kTile)) {                         // tokens behind the new one, pages that are none
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int count = u ? count1 : count0;
+                    for (int u = 0; u < kAtOnce; ++u) {
+                        const int count = counts[u];
                         if (t0 >= count) {
 #pragma unroll
                             for (int k = 0; k < KC; ++k) x[u][k] = -INFINITY;
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                 }
                 __half2 big = __hmax2(va[0][0], vb[0][0]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
                         if (u || g) big = __hmax2(big, __hmax2(va[u][g], vb[u][g]));
@@ -484,7 +489,9 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                 const float room = 8.f - (float)elog;
 #pragma unroll
                 for (int k = 0; k < KC; ++k) {
-                    m[k] = fmaxf(fmaxf(x[0][k], x[0][KC + k]), fmaxf(x[1][k], x[1][KC + k])) * unit[k];
+                    m[k] = fmaxf(x[0][k], x[0][KC + k]);
+                    if constexpr (kAtOnce == 2) m[k] = fmaxf(m[k], fmaxf(x[kAtOnce - 1][k], x[kAtOnce - 1][KC + k]));
+                    m[k] *= unit[k];
                     move |= m[k] - ref[k] > room;
                 }
                 if (__any_sync(0xffffffffu, move)) {
@@ -521,8 +528,8 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const unsigned char* tile = chunk + u * kBytes;
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const unsigned char* tile = tiles + u * kBytes;
                     float p[2 * KC];
 #pragma unroll
                     for (int k = 0; k < 2 * KC; ++k) p[k] = ex2(fmaf(x[u][k], unit[k % KC], -ref[k % KC]));
