@@ -1,20 +1,22 @@
 // Attention of a chunk of queries over the paged 4-bit cache, on the 5th-generation tensor cores.
 //
-// A CTA takes T x 128 rows of one (batch row, key/value head): row f of the chunk's S x R is query f / R of head f % R of the R that share
-// the key/value head.  It walks over tiles of 128 cached tokens, up to its last query's position, for each of its T row tiles:
+// Row f of the chunk's S x R is query f / R of head f % R of the R that share the key/value head.  128 rows are a row tile; for each of its
+// row tiles a CTA walks over steps of 128 cached tokens, up to its last query's position:
 //     S = Q K^T     128 x 128, Q and K in shared memory, S in tensor memory
 //     P = 2^(S scale - ref), rounded to fp16, over S's place in tensor memory; ref follows the row's maximum by steps of 2^8 and more
 //     O += P V      P in tensor memory, V^T in shared memory, O in tensor memory
-// K and V come as codes: the worker warps turn m + n s into fp16 (one rounding, 2^-11 of the value) while the products run, and write the
+// K and V come as codes: worker warps turn m + n s into fp16 (one rounding, 2^-11 of the value) while the products run, and write the
 // 128-byte swizzled layouts the products read - keys by tokens (dims of a word of 8 in the order 0 4 1 5 2 6 3 7 that the codes unpack
 // in; the queries are stored in the same order), values by dims: a transposing matrix load gives a lane the same four dims of two tokens,
 // which unpack side by side.  The rows of V^T, and with them the columns of O, stand in the order 8 n + h + 32 p of dim n of the half-word
-// 8 p + h that the cache stores, which puts the eight rows that one store instruction touches on different banks.  The codes of the next step are on
-// their way to shared memory meanwhile, and where its tiles stand is looked up two steps ahead.  Two threads a row in the softmax, eight
-// warps a row tile, and one warp that issues the products (issuing eight takes as long as they run).
+// 8 p + h that the cache stores, which puts the eight rows that one store instruction touches on different banks.  The codes of the next
+// step are on their way to shared memory meanwhile, and where its tiles stand is looked up two steps ahead.  Two threads a row in the
+// softmax, eight warps a row tile, and one warp that issues the products (issuing eight takes as long as they run).
 //
-// What bounds it is what the workers can issue: a tile of K and V costs them as much as its softmax.  So T = 2 (one CTA an SM) for more
-// than 128 rows of 128 dims, which halves that cost; otherwise T = 1, two CTAs an SM.
+// What bounds it is what the workers can issue, and the exponentials (16 a clock): a step of K and V costs as much to unpack as a row tile's
+// softmax.  For more than 128 rows of 128 dims a CTA has two row tiles (pair_kernel, one CTA an SM), whose warps take turns: while one
+// row tile is in its softmax the other's warps unpack - the first row tile's the values, the second's the keys, into two buffers each -, and
+// the tensor cores run the products of whichever is ready.  Otherwise (single_kernel) one row tile, two CTAs an SM.
 //
 // A value whose group is not finite is multiplied as 0, so that rows that must not see its token stay clean, and the rows that do see it
 // get NaN for that group's dims at the end.
@@ -29,6 +31,7 @@ using namespace sm100;
 
 constexpr int kRows = 128, kTokens = 128;
 constexpr int kTilesOf = kTokens / kTile;         // 16-token tiles of a step
+constexpr int kGroup = 256;                       // worker threads of a row tile
 constexpr uint64_t kWaitNs = 400000000ull;        // a product that has not finished by then never will: error word 1
 
 struct PromptArgs {
@@ -41,26 +44,10 @@ struct PromptArgs {
     const __half* sin;
     int* error;
     int seq, heads, share;        // share: query heads of a key/value head
-    int blocks;                   // of T x 128 rows
+    int blocks;                   // CTAs of a (batch row, key/value head)
     int rope_rows;
     long long stride, page_bytes;
     float scale_log2;             // scale * log2(e)
-};
-
-template <int D, int half_tile, int T>
-struct Smem {
-    alignas(1024) unsigned char q[T][kRows * D * 2], k[kTokens * D * 2], v[kTokens * D * 2];
-    // codes of the next step, with steps and minima (T = 1: the keys' come through registers, or two CTAs would not fit)
-    alignas(16) unsigned char v_codes[kTilesOf][half_tile], k_codes[T == 1 ? 1 : kTilesOf][half_tile];
-    const unsigned char* tile[4][kTilesOf];       // by step modulo 4: where its tiles stand; null: behind the last token, or no page
-    unsigned char page_ok[4][kTilesOf];           // 0: a page is needed and is none of the pool
-    uint64_t s_done[T], pv_done[T];               // products over
-    uint64_t k_ready, v_ready, p_ready[T];        // operands written
-    uint32_t tmem;
-    int abort_flag;
-    int bad[kTokens];                             // groups of a token's value that are not finite
-    float swap[2][T * kRows];                     // what the two threads of a row tell each other
-    int swap_bad[T * kRows];
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -139,17 +126,8 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
           "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }      // this thread's
-// barriers of the worker warps
-template <int N>
-__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 9, %0;" ::"n"(N) : "memory"); }
-template <int N>
-__device__ __forceinline__ bool workers_any(bool mine)
-{
-    int any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, 10, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-                 : "=r"(any) : "r"((int)mine), "n"(N) : "memory");
-    return any != 0;
-}
+// barriers of `threads` worker threads: 1 to 8 are the pairs of warps that share rows, 9 and 10 the row tiles'
+__device__ __forceinline__ void meet(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // the warp's operand writes of either kind, made visible to the products, and its arrival
 __device__ __forceinline__ void written(uint32_t bar, int lane)
 {
@@ -162,297 +140,244 @@ __device__ __forceinline__ void written(uint32_t bar, int lane)
 // byte of 16-byte chunk `c` (8 halves) of row r in an operand of `rows` rows, 64 halves a sub-tile, 128-byte swizzle
 __device__ __forceinline__ int operand_at(int rows, int r, int c) { return (c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 
-template <class F, int D, int T>
-__global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(const PromptArgs a)
-{
-    constexpr int J = F::J, NG = F::NG, kBytes = F::kBytes, kHalf = kBytes / 2, kWorkers = 256 * T, kWarps = 8 * T;
-    constexpr uint32_t kTmemCols = 256 * T;       // a row tile's S (then P) in 128 columns, O in the 128 behind them
-    static_assert(F::kVal == kHalf, "keys and values are halves of a tile");
-    extern __shared__ unsigned char raw[];
-    using S = Smem<D, kHalf, T>;
-    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int block = a.blocks - 1 - (int)blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;         // the longest rows first
-    const int pos = a.pos[b], count = a.counts ? min(a.counts[b], a.seq) : a.seq;
-    if (pos < 0 || count <= 0) return;
-    const int room = min(a.c.capacity(), a.cos ? a.rope_rows : 0x7fffffff);
-    const int fit = pos >= room ? 0 : min(count, room - pos);                                    // queries that can be served
-    if (fit < count && block == 0 && kvh == 0 && tid == 0) atomicExch(a.error, kErrPosition);
-    const long long rows = (long long)fit * a.share, row0 = (long long)block * (T * kRows);
-    if (row0 >= rows) return;
-    const int first_i = (int)(row0 / a.share), last_i = (int)(min(row0 + T * kRows, rows) - 1) / a.share;
-    const int last = pos + last_i;                                                               // the last token anybody here sees
-    const int steps = last / kTokens + 1;
-
-    if (warp == kWarps) {
-        tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
-        tmem_relinquish();
-    }
-    if (tid == 0) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            mbar_init(smem_u32(&sm.s_done[t]), 1);
-            mbar_init(smem_u32(&sm.pv_done[t]), 1);
-            mbar_init(smem_u32(&sm.p_ready[t]), 8);
-        }
-        mbar_init(smem_u32(&sm.k_ready), kWarps);
-        mbar_init(smem_u32(&sm.v_ready), kWarps);
-        sm.abort_flag = 0;
-    }
-    mbar_fence_init();
-    if (tid < kTokens) sm.bad[tid] = 0;
-
-    // ---- where the tiles of a step stand (threads 0 .. 7)
-    const int tshift = a.c.page_shift - 4, per1 = (1 << tshift) - 1;
-    const int* ids = a.c.table + (size_t)b * a.c.width;
-    const unsigned char* head = a.c.pool + ((size_t)kvh << tshift) * kBytes;
-    int next_id = -1;
-    auto look = [&](int step) {
-        const int t16 = step * kTilesOf + tid;
-        next_id = t16 <= last >> 4 ? ids[t16 >> tshift] : -1;
-    };
-    auto note = [&](int step) {
-        const int t16 = step * kTilesOf + tid;
-        const bool needed = t16 <= last >> 4, there = needed && (unsigned)next_id < (unsigned)a.c.pages;
-        sm.tile[step & 3][tid] = there ? head + next_id * a.page_bytes + (t16 & per1) * kBytes : nullptr;
-        sm.page_ok[step & 3][tid] = there || !needed;
-        if (needed && !there) atomicExch(a.error, kErrPage);
-    };
-    if (tid < kTilesOf) {
-        look(0);
-        note(0);
-        look(1);
-        note(1);
-    }
-    __syncthreads();
-    const uint32_t tmem = sm.tmem;
-    const uint32_t k_bar = smem_u32(&sm.k_ready), v_bar = smem_u32(&sm.v_ready);
-    bool ok = true;
-
-    if (warp == kWarps) {
-        // ---- the products.  P stands where S stood: S of a step is issued when P V of the step before is over
-        const uint64_t k_desc = smem_desc_sw128(smem_u32(sm.k)), v_desc = smem_desc_sw128(smem_u32(sm.v));
-        for (int step = 0; step < steps; ++step) {
-            ok = ok && mbar_wait(k_bar, step & 1, &sm.abort_flag, kWaitNs);                      // (the queries, at the first step)
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                if (step > 0) ok = ok && mbar_wait(smem_u32(&sm.pv_done[t]), (step - 1) & 1, &sm.abort_flag, kWaitNs);
-                tc_fence_after_sync();
-                __syncwarp();
-                const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q[t]));
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint64_t at = (uint64_t)((kk >> 2) * (kRows * 128 / 16) + 2 * (kk & 3));
-                    if (elect_one()) mma_f16_ss(tmem + 256 * t, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
-                }
-                if (elect_one()) tc_commit(smem_u32(&sm.s_done[t]));
-                __syncwarp();
-            }
-            ok = ok && mbar_wait(v_bar, step & 1, &sm.abort_flag, kWaitNs);
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                ok = ok && mbar_wait(smem_u32(&sm.p_ready[t]), step & 1, &sm.abort_flag, kWaitNs);
-                tc_fence_after_sync();
-                __syncwarp();
-#pragma unroll
-                for (int kk = 0; kk < kTokens / 16; ++kk) {
-                    // P of tokens 0 .. 63 stands in columns 0 .. 31, of tokens 64 .. 127 in columns 64 .. 95
-                    const uint32_t p = tmem + 256 * t + (kk >> 2) * 64 + (kk & 3) * 8;
-                    const uint64_t at = (uint64_t)((kk >> 2) * (D * 128 / 16) + 2 * (kk & 3));
-                    if (elect_one()) mma_f16_ts(tmem + 256 * t + kTokens, p, v_desc + at, idesc_f16_m128(D), step > 0 || kk > 0);
-                }
-                if (elect_one()) tc_commit(smem_u32(&sm.pv_done[t]));
-                __syncwarp();
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < T; ++t) ok = ok && mbar_wait(smem_u32(&sm.pv_done[t]), (steps - 1) & 1, &sm.abort_flag, kWaitNs);
-        if (!ok && lane == 0) atomicExch(a.error, 1);
-        __syncthreads();                                                                         // the workers have read O
-        tmem_dealloc(tmem, kTmemCols);
-        return;
-    }
-
-    // ---- codes of a step to shared memory, keys or values: tiles are contiguous halves of 16-byte pieces.  A code row's pieces change
-    // places, so that the eight rows that are read together stand on different banks: by rows' bits 1 and 2 (keys; values stand
-    // exchanged by bit 1 already), at D = 64 by bit 2.
-    auto piece_of = [&](int row, int piece, bool values) {
-        return D == 128 ? piece ^ (values ? (row >> 2) & 1 : (row >> 1) & 3) : piece ^ ((row >> 2) & 1);
-    };
-    auto load_codes = [&](unsigned char* to, int step, int half_at) {
-        constexpr int kPieces = kHalf / 16, kRowPieces = D / 32;                                 // of a tile, of a code row
-#pragma unroll
-        for (int i = 0; i < (kTilesOf * kPieces + kWorkers - 1) / kWorkers; ++i) {
-            const int at = tid + i * kWorkers;
-            if (at >= kTilesOf * kPieces) break;
-            const unsigned char* tile = sm.tile[step & 3][at / kPieces];
-            const int piece = at % kPieces, row = piece / kRowPieces;
-            const int there = row < kTile ? row * kRowPieces + piece_of(row, piece % kRowPieces, half_at != 0) : piece;
-            // (a tile that is none is filled with zeros: its values are 0, its keys are hidden)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                         ::"r"(smem_u32(to) + (at - piece + there) * 16), "l"(tile ? tile + half_at + piece * 16 : a.c.pool), "r"(tile ? 16 : 0) : "memory");
-        }
-    };
-    // keys: 16-byte pieces (4 words of 8 dims); eight lanes take eight rows, so that their stores fall on different banks
-    constexpr int kPieces = kTokens * D / 32 / kWorkers < 1 ? 1 : kTokens * D / 32 / kWorkers;  // of a thread
-    const int kp = lane >> 3, kt0 = D == 128 ? 8 * warp + (lane & 7) : 8 * (2 * warp + (kp >> 1)) + (lane & 7), kc = D == 128 ? kp : kp & 1;
-    const bool has_k = kt0 < kTokens;                                                            // (D = 64, T = 2: half of the threads)
-    uint4 kreg[T == 1 ? kPieces : 1];
-    __half2 kpar[T == 1 ? kPieces : 1][NG];
-    auto fetch_k = [&](int step) {
-        if constexpr (T == 2) {
-            load_codes(sm.k_codes[0], step, 0);
-        } else {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) {
-                const int row = kt0 + 8 * kWarps * k;
-                const unsigned char* tile = sm.tile[step & 3][row >> 4];
-                kreg[k] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int g = 0; g < NG; ++g) kpar[k][g] = h2_of(0);
-                if (tile) {
-                    kreg[k] = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * kc);
-                    load_params<NG>(tile + F::key_par(row & 15, 0), kpar[k]);
-                }
-            }
-        }
-    };
-    auto put_k = [&]() {
-        if (!has_k) return;
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            const int row = kt0 + 8 * kWarps * k;
-            uint4 kw;
-            __half2 par[NG], s[NG], m[NG];
-            if constexpr (T == 2) {
-                const unsigned char* tile = sm.k_codes[row >> 4];
-                kw = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * piece_of(row & 15, kc, false));
-                load_params<NG>(tile + F::key_par(row & 15, 0), par);
-            } else {
-                kw = kreg[k];
-#pragma unroll
-                for (int g = 0; g < NG; ++g) par[g] = kpar[k][g];
-            }
-            const uint32_t w4[4] = {kw.x, kw.y, kw.z, kw.w};
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                s[g] = __low2half2(par[g]);
-                m[g] = __high2half2(par[g]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // stored word 4 kc + i is word w of the row
-                const int j = D == 128 ? i : i & 1, w = D == 128 ? 4 * i + kc : 4 * (i & 1) + 2 * kc + (i >> 1);
-                const int g = 32 * j * NG / D;
-                __half2 n[4];
-                codes8(w4[i], n);
-                uint4 o;
-                o.x = h2_bits(__hfma2(n[0], s[g], m[g]));
-                o.y = h2_bits(__hfma2(n[1], s[g], m[g]));
-                o.z = h2_bits(__hfma2(n[2], s[g], m[g]));
-                o.w = h2_bits(__hfma2(n[3], s[g], m[g]));
-                *reinterpret_cast<uint4*>(sm.k + operand_at(kTokens, row, w)) = o;
-            }
-        }
-    };
-    // values: a warp takes groups of 8 tokens.  Matrix p of the load is the 16-byte piece p of the tokens' rows: the lane gets half-word
-    // 8 p + lane / 4 of tokens 2 (lane % 4) and the next one, all of one group of dims.
-    const int vh = lane >> 2, vp2 = 2 * (lane & 3), vgroup = 32 * (vh % J) * NG / D;
-    auto put_v = [&](int step) {                                                                 // true: some value is not finite
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < kTokens / 8 / kWarps; ++i) {
-            const int vt = warp + i * kWarps, r0 = 8 * (vt & 1);
-            const unsigned char* tile = sm.v_codes[vt >> 1];
-            const int left = last - (step * kTokens + 8 * vt) - vp2;                             // tokens behind the lane's first
-            // lane l gives the address of row l % 8 of matrix l / 8 (at D = 64, two matrices: lanes 16 .. 31 repeat)
-            const int lr = r0 + (lane & 7), lp = (lane >> 3) & (J - 1);
-            const int stored = D == 128 ? lp ^ (((lr >> 1) & 1) << 1) : lp;
-            const uint32_t from = smem_u32(tile + lr * (D / 2) + 16 * piece_of(lr, stored, true));
-            uint32_t w[J];
-            if constexpr (J == 4)
-                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
-            else
-                asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
-            __half2 pa = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2, vgroup) - F::kVal);
-            __half2 pb = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2 + 1, vgroup) - F::kVal);
-            if (left < 0) pa = h2_of(0);                                                         // behind the last token: whatever the page holds
-            if (left < 1) pb = h2_of(0);
-            const __half2 zero = __hfma2(pa, h2_of(0), __hmul2(pb, h2_of(0)));                   // NaN if one of them is not finite
-            if (!__hbeq2(zero, zero)) {
-                found = true;
-                if (!finite2(pa)) {
-                    pa = h2_of(0);
-                    atomicOr(&sm.bad[8 * vt + vp2], 1 << vgroup);
-                }
-                if (!finite2(pb)) {
-                    pb = h2_of(0);
-                    atomicOr(&sm.bad[8 * vt + vp2 + 1], 1 << vgroup);
-                }
-            }
-            const __half2 s = __lows2half2(pa, pb), m = __highs2half2(pa, pb);
-#pragma unroll
-            for (int q = 0; q < J; ++q) {
-                __half2 n[4];
-                codes8(w[q], n);
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    *reinterpret_cast<__half2*>(sm.v + operand_at(D, 32 * q + 8 * d + vh, vt) + 2 * vp2) = __hfma2(n[d], s, m);
-            }
-        }
-        return found;
-    };
-
-    fetch_k(0);
-    load_codes(sm.v_codes[0], 0, kHalf);
-    // ---- queries: two threads a row, rotated as the decode kernel does, in the order of the keys' dims
-    const int mine = warp >> 3;                                                                  // the thread's row tile
+// What a CTA works on: `tiles` row tiles of one (batch row, key/value head).
+struct Task {
+    int b, kvh, pos, last, steps; // last: the last token that any of its rows sees
+    int first_sees;               // ... and that its first row sees
+    int last_i;
+    long long rows, row0;         // rows there are, its first
+    __device__ __forceinline__ bool take(const PromptArgs& a, int tiles)
     {
-        const int r = (tid & 255) >> 1;
-        const long long f = row0 + mine * kRows + r;
-        const int i = (int)(f / a.share), h = (int)(f % a.share);
+        const int block = a.blocks - 1 - (int)blockIdx.x;                                        // the longest rows first
+        kvh = blockIdx.y;
+        b = blockIdx.z;
+        pos = a.pos[b];
+        const int count = a.counts ? min(a.counts[b], a.seq) : a.seq;
+        if (pos < 0 || count <= 0) return false;
+        const int room = min(a.c.capacity(), a.cos ? a.rope_rows : 0x7fffffff);
+        const int fit = pos >= room ? 0 : min(count, room - pos);                                // queries that can be served
+        if (fit < count && block == 0 && kvh == 0 && threadIdx.x == 0) atomicExch(a.error, kErrPosition);
+        rows = (long long)fit * a.share;
+        row0 = (long long)block * (tiles * kRows);
+        if (row0 >= rows) return false;
+        last_i = (int)(min(row0 + tiles * kRows, rows) - 1) / a.share;
+        last = pos + last_i;
+        first_sees = pos + (int)(row0 / a.share);
+        steps = last / kTokens + 1;
+        return true;
+    }
+};
+
+// Where the 16-token tiles of the steps stand, by step modulo 8: looked up by threads 0 .. 7 of a row tile's group, two steps ahead.
+struct Places {
+    const unsigned char* tile[8][kTilesOf];       // null: behind the last token, or no page
+    unsigned char page_ok[8][kTilesOf];           // 0: a page is needed and is none of the pool
+};
+template <class F>
+struct Lookup {
+    const int* ids;
+    const unsigned char* head;
+    int tshift, next_id;
+    __device__ __forceinline__ Lookup(const PromptArgs& a, const Task& w) : tshift(a.c.page_shift - 4), next_id(-1)
+    {
+        ids = a.c.table + (size_t)w.b * a.c.width;
+        head = a.c.pool + ((size_t)w.kvh << tshift) * F::kBytes;
+    }
+    __device__ __forceinline__ void look(const Task& w, int step, int i)
+    {
+        const int t16 = step * kTilesOf + i;
+        next_id = t16 <= w.last >> 4 ? ids[t16 >> tshift] : -1;
+    }
+    __device__ __forceinline__ void note(const PromptArgs& a, const Task& w, Places& p, int step, int i) const
+    {
+        const int t16 = step * kTilesOf + i;
+        const bool needed = t16 <= w.last >> 4, there = needed && (unsigned)next_id < (unsigned)a.c.pages;
+        p.tile[step & 7][i] = there ? head + next_id * a.page_bytes + (t16 & ((1 << tshift) - 1)) * F::kBytes : nullptr;
+        p.page_ok[step & 7][i] = there || !needed;
+        if (needed && !there) atomicExch(a.error, kErrPage);
+    }
+};
+
+// A code row's 16-byte pieces change places on their way to shared memory, so that the eight rows that are read together stand on different
+// banks: by rows' bits 1 and 2 (keys; values stand exchanged by bit 1 already), at D = 64 by bit 2.
+template <int D>
+__device__ __forceinline__ int piece_of(int row, int piece, bool values)
+{
+    return D == 128 ? piece ^ (values ? (row >> 2) & 1 : (row >> 1) & 3) : piece ^ ((row >> 2) & 1);
+}
+// The keys' or the values' halves of a step's tiles to shared memory, by a row tile's group.
+template <class F, int D>
+__device__ __forceinline__ void load_codes(unsigned char* to, const Places& p, int step, bool values, int tid, const unsigned char* any)
+{
+    constexpr int kHalf = F::kBytes / 2, kPieces = kHalf / 16, kRowPieces = D / 32;              // of a tile, of a code row
+    static_assert(F::kVal == kHalf, "keys and values are halves of a tile");
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            const int w = (tid & 1) * (D / 16) + k;
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (f < rows) load_rotated<D>(a.qkv + ((long long)b * a.seq + i) * a.stride + (kvh * a.share + h) * D, w, a.cos, a.sin, pos + i, x);
-            uint4 o;
-            o.x = h2_bits(__floats2half2_rn(x[0], x[4]));
-            o.y = h2_bits(__floats2half2_rn(x[1], x[5]));
-            o.z = h2_bits(__floats2half2_rn(x[2], x[6]));
-            o.w = h2_bits(__floats2half2_rn(x[3], x[7]));
-            *reinterpret_cast<uint4*>(sm.q[mine] + operand_at(kRows, r, w)) = o;
+    for (int i = 0; i < (kTilesOf * kPieces + kGroup - 1) / kGroup; ++i) {
+        const int at = tid + i * kGroup;
+        if (at >= kTilesOf * kPieces) break;
+        const unsigned char* tile = p.tile[step & 7][at / kPieces];
+        const int piece = at % kPieces, row = piece / kRowPieces;
+        const int there = row < kTile ? row * kRowPieces + piece_of<D>(row, piece % kRowPieces, values) : piece;
+        // (a tile that is none is filled with zeros: its values are 0, its keys are hidden)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(smem_u32(to) + (at - piece + there) * 16), "l"(tile ? tile + (values ? kHalf : 0) + piece * 16 : any), "r"(tile ? 16 : 0) : "memory");
+    }
+}
+
+// Four words of 8 dims (16-byte piece kc of a key row) to the operand.
+template <class F, int D>
+__device__ __forceinline__ void put_key_piece(unsigned char* k, int row, int kc, const uint4& kw, const __half2 (&par)[F::NG])
+{
+    const uint32_t w4[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // stored word 4 kc + i is word w of the row
+        const int j = D == 128 ? i : i & 1, w = D == 128 ? 4 * i + kc : 4 * (i & 1) + 2 * kc + (i >> 1);
+        const __half2 p = par[32 * j * F::NG / D], s = __low2half2(p), m = __high2half2(p);
+        __half2 n[4];
+        codes8(w4[i], n);
+        *reinterpret_cast<uint4*>(k + operand_at(kTokens, row, w)) = make_uint4(h2_bits(__hfma2(n[0], s, m)), h2_bits(__hfma2(n[1], s, m)),
+                                                                               h2_bits(__hfma2(n[2], s, m)), h2_bits(__hfma2(n[3], s, m)));
+    }
+}
+// The keys a thread of a group takes: rows kt0 and (D = 128) kt0 + 64; eight lanes take eight rows, so that their stores fall on different banks.
+template <int D>
+struct KeyPlace {
+    static constexpr int kPieces = D / 64;
+    int row, kc;
+    __device__ __forceinline__ KeyPlace(int warp, int lane)
+        : row(D == 128 ? 8 * warp + (lane & 7) : 8 * (2 * warp + (lane >> 4)) + (lane & 7)), kc(D == 128 ? lane >> 3 : (lane >> 3) & 1) {}
+};
+
+// 128 tokens' values to the operand, by a group: a warp takes groups of 8 tokens.  Matrix p of the load is the 16-byte piece p of the tokens'
+// rows: the lane gets half-word 8 p + lane / 4 of tokens 2 (lane % 4) and the next one, all of one group of dims.  True: some are not finite.
+template <class F, int D>
+__device__ __forceinline__ bool put_values(unsigned char* v, const unsigned char* codes, int* bad, int left_of_step, int warp, int lane)
+{
+    constexpr int J = F::J, kHalf = F::kBytes / 2;
+    const int vh = lane >> 2, vp2 = 2 * (lane & 3), vgroup = 32 * (vh % J) * F::NG / D;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int vt = warp + 8 * i, r0 = 8 * (vt & 1);
+        const unsigned char* tile = codes + (vt >> 1) * kHalf;
+        const int left = left_of_step - 8 * vt - vp2;                                            // tokens behind the lane's first
+        // lane l gives the address of row l % 8 of matrix l / 8 (at D = 64, two matrices: lanes 16 .. 31 repeat)
+        const int lr = r0 + (lane & 7), lp = (lane >> 3) & (J - 1);
+        const int stored = D == 128 ? lp ^ (((lr >> 1) & 1) << 1) : lp;
+        const uint32_t from = smem_u32(tile + lr * (D / 2) + 16 * piece_of<D>(lr, stored, true));
+        uint32_t w[J];
+        if constexpr (J == 4)
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+        else
+            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
+        __half2 pa = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2, vgroup) - F::kVal);
+        __half2 pb = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2 + 1, vgroup) - F::kVal);
+        if (left < 0) pa = h2_of(0);                                                             // behind the last token: whatever the page holds
+        if (left < 1) pb = h2_of(0);
+        const __half2 zero = __hfma2(pa, h2_of(0), __hmul2(pb, h2_of(0)));                       // NaN if one of them is not finite
+        if (!__hbeq2(zero, zero)) {
+            found = true;
+            if (!finite2(pa)) {
+                pa = h2_of(0);
+                atomicOr(&bad[8 * vt + vp2], 1 << vgroup);
+            }
+            if (!finite2(pb)) {
+                pb = h2_of(0);
+                atomicOr(&bad[8 * vt + vp2 + 1], 1 << vgroup);
+            }
+        }
+        const __half2 s = __lows2half2(pa, pb), m = __highs2half2(pa, pb);
+#pragma unroll
+        for (int q = 0; q < J; ++q) {
+            __half2 n[4];
+            codes8(w[q], n);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) *reinterpret_cast<__half2*>(v + operand_at(D, 32 * q + 8 * d + vh, vt) + 2 * vp2) = __hfma2(n[d], s, m);
         }
     }
-    copies_landed();
-    workers_sync<kWorkers>();
-    put_k();
-    written(k_bar, lane);
-    workers_sync<kWorkers>();                                                                    // the keys' codes have been read
-    if (T == 2 && steps > 1) fetch_k(1);
+    return found;
+}
 
-    // ---- the row of this thread in the softmax, and its half of the columns
-    const int row = 32 * (warp & 3) + lane, half = (warp >> 2) & 1, slot = mine * kRows + row;
-    const uint32_t at_s = tmem + 256 * mine + ((uint32_t)(32 * (warp & 3)) << 16), at_o = at_s + kTokens + half * (D / 2);
-    const uint32_t s_bar = smem_u32(&sm.s_done[mine]), p_bar = smem_u32(&sm.p_ready[mine]);
-    const int sees = pos + min((int)((row0 + slot) / a.share), last_i);                         // last token it sees (rows behind the last: as that one)
-    const int first_sees = pos + first_i;
-    // (the sign of a negative scale goes into the scores, so that `unit` is positive; a scale of zero makes them zero)
-    const float unit = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2), sign = a.scale_log2 == 0.f ? 0.f : a.scale_log2 < 0.f ? -1.f : 1.f;
-    const uint64_t unit2 = pair(unit, unit);
-    float ref = -INFINITY;
-    uint64_t sum2 = pair(0.f, 0.f);
-    int nan_groups = 0;
-    for (int step = 0; step < steps; ++step) {
-        const bool found = put_v(step);                                                          // (P V of the step before is over)
-        written(v_bar, lane);
-        if (T == 1 && step + 1 < steps) fetch_k(step + 1);
-        if (tid < kTilesOf) look(step + 2);
-        ok = ok && mbar_wait(s_bar, step & 1, &sm.abort_flag, kWaitNs);
-        tc_fence_after_sync();
-        const uint64_t pages = *reinterpret_cast<const uint64_t*>(sm.page_ok[step & 3]);
-        const bool masked = (step + 1) * kTokens - 1 > first_sees || pages != 0x0101010101010101ull;
+// A row tile's queries to the operand, by its group, rotated as the decode kernel does and in the order of the keys' dims.  Adjacent lanes
+// take adjacent words of a row (two threads a row, each with half of its words, took 258 us instead of 106 for 8 x 512 rotated queries).
+template <int D>
+__device__ __forceinline__ void put_queries(const PromptArgs& a, const Task& w, unsigned char* q, long long first, int tid)
+{
+    constexpr int kWords = D / 8, kAtOnce = kGroup / kWords;                                     // rows at once
+    const int word = tid % kWords, i0 = (int)(first / a.share), h0 = (int)(first % a.share);
+    const __half* from = a.qkv + ((long long)w.b * a.seq + i0) * a.stride + (long long)w.kvh * a.share * D;
+    const int left = (int)min(w.rows - first, (long long)kRows);
+#pragma unroll 4
+    for (int r = tid / kWords; r < kRows; r += kAtOnce) {
+        const int i = (h0 + r) / a.share, h = h0 + r - i * a.share;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r < left) load_rotated<D>(from + i * a.stride + h * D, word, a.cos, a.sin, w.pos + i0 + i, x);
+        *reinterpret_cast<uint4*>(q + operand_at(kRows, r, word)) =
+            make_uint4(h2_bits(__floats2half2_rn(x[0], x[4])), h2_bits(__floats2half2_rn(x[1], x[5])), h2_bits(__floats2half2_rn(x[2], x[6])),
+                       h2_bits(__floats2half2_rn(x[3], x[7])));
+    }
+}
+
+// The two products of a step, by one warp.
+template <int D>
+__device__ __forceinline__ void issue_s(uint32_t s, uint64_t q_desc, uint64_t k_desc, uint32_t done)
+{
+    tc_fence_after_sync();
+    __syncwarp();
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t at = (uint64_t)((kk >> 2) * (kRows * 128 / 16) + 2 * (kk & 3));
+        if (elect_one()) mma_f16_ss(s, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
+    }
+    if (elect_one()) tc_commit(done);
+    __syncwarp();
+}
+template <int D>
+__device__ __forceinline__ void issue_pv(uint32_t s, uint64_t v_desc, bool first, uint32_t done)
+{
+    tc_fence_after_sync();
+    __syncwarp();
+#pragma unroll
+    for (int kk = 0; kk < kTokens / 16; ++kk) {
+        // P of tokens 0 .. 63 stands in columns 0 .. 31, of tokens 64 .. 127 in columns 64 .. 95
+        const uint64_t at = (uint64_t)((kk >> 2) * (D * 128 / 16) + 2 * (kk & 3));
+        if (elect_one()) mma_f16_ts(s + kTokens, s + (kk >> 2) * 64 + (kk & 3) * 8, v_desc + at, idesc_f16_m128(D), !first || kk > 0);
+    }
+    if (elect_one()) tc_commit(done);
+    __syncwarp();
+}
+
+// A thread's row in the softmax, and its half of the columns.
+template <class F, int D>
+struct Row {
+    float* swap;                                  // [2][rows of the CTA]: what the two threads of a row tell each other
+    int swap_rows, slot, half, barrier;
+    uint32_t at_s, at_o;
+    int sees;                                     // last token it sees (rows behind the last: as that one)
+    float unit, sign, ref;
+    uint64_t sum2;
+    int nan_groups;
+    __device__ __forceinline__ Row(const PromptArgs& a, const Task& w, float* swap_, int swap_rows_, int tile, int warp, int lane, uint32_t tmem)
+        : swap(swap_), swap_rows(swap_rows_), ref(-INFINITY), nan_groups(0)
+    {
+        const int row = 32 * (warp & 3) + lane;
+        half = (warp >> 2) & 1;
+        slot = tile * kRows + row;
+        barrier = 1 + tile * 4 + (warp & 3);
+        at_s = tmem + 256 * tile + ((uint32_t)(32 * (warp & 3)) << 16);
+        at_o = at_s + kTokens + half * (D / 2);
+        sees = w.pos + min((int)((w.row0 + slot) / a.share), w.last_i);
+        // (the sign of a negative scale goes into the scores, so that `unit` is positive; a scale of zero makes them zero)
+        unit = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+        sign = a.scale_log2 == 0.f ? 0.f : a.scale_log2 < 0.f ? -1.f : 1.f;
+        sum2 = pair(0.f, 0.f);
+    }
+    // S of a step becomes P
+    __device__ __forceinline__ void softmax(const Task& w, int step, uint64_t pages)
+    {
+        const bool masked = (step + 1) * kTokens - 1 > w.first_sees || pages != 0x0101010101010101ull;
         const int from = step * kTokens + 64 * half;                                             // the thread's first token
         uint32_t s[32];
         auto fetch = [&](int c) {                                                                // scores of 32 tokens
@@ -483,9 +408,9 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
             top = fmaxf(t0, t1);
         }
         // both threads of a row move the reference alike
-        sm.swap[half][slot] = top;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + mine * 4 + (warp & 3)) : "memory");
-        top = fmaxf(top, sm.swap[half ^ 1][slot]) * unit;
+        swap[half * swap_rows + slot] = top;
+        meet(barrier, 64);
+        top = fmaxf(top, swap[(half ^ 1) * swap_rows + slot]) * unit;
         const bool move = top - ref > 8.f;                                                       // (from minus infinity as well; not with nothing seen)
         if (__any_sync(0xffffffffu, move)) {
             const float to = move ? top : ref, keep = ref == -INFINITY ? 0.f : ex2(ref - to);
@@ -505,7 +430,7 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
             }
         }
         const float shift = ref == -INFINITY ? 0.f : -ref;                                       // nothing seen yet: weights 0
-        const uint64_t shift2 = pair(shift, shift);
+        const uint64_t unit2 = pair(unit, unit), shift2 = pair(shift, shift);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             if (c == 1) fetch(1);                                                                // (again: 64 at a time are too many registers)
@@ -520,97 +445,394 @@ __global__ void __launch_bounds__(256 * T + 32, T == 1 ? 2 : 1) prompt_kernel(co
             tmem_st_32x32b_x16(at_s + 64 * half + 16 * c, p);                                    // over columns that this thread has read
         }
         tmem_wait_st();
-        written(p_bar, lane);
-        copies_landed();
-        if (workers_any<kWorkers>(found)) {
-            // rows that see a value that is not finite
+    }
+    // the values of a step that are not finite
+    __device__ __forceinline__ void mind(const int* bad, int step, uint64_t pages)
+    {
 #pragma unroll 1
-            for (int i = 0; i < 64; ++i) {
-                const int t = from + i;
-                if (t <= sees && (pages >> (8 * ((64 * half + i) >> 4)) & 1)) nan_groups |= sm.bad[64 * half + i];
-            }
-            workers_sync<kWorkers>();
-            if (tid < kTokens) sm.bad[tid] = 0;
+        for (int i = 64 * half; i < 64 * half + 64; ++i)
+            if (step * kTokens + i <= sees && (pages >> (8 * (i >> 4)) & 1)) nan_groups |= bad[i];
+    }
+    // out = O / sum; swap_bad [rows of the CTA]
+    __device__ __forceinline__ void finish(const PromptArgs& a, const Task& w, int* swap_bad)
+    {
+        const float2 sums = unpair(sum2);
+        float sum = sums.x + sums.y;
+        meet(barrier, 64);                                                                       // (the last step's exchange is over)
+        swap[half * swap_rows + slot] = sum;
+        if (half) swap_bad[slot] = nan_groups;
+        meet(barrier, 64);
+        sum += swap[(half ^ 1) * swap_rows + slot];
+        if (!half) {
+            nan_groups |= swap_bad[slot];
+            swap_bad[slot] = nan_groups;
         }
-        if (step + 1 < steps) {
-            load_codes(sm.v_codes[0], step + 1, kHalf);                                             // (everybody has read the codes of this step)
-            put_k();                                                                             // (S of this step is over in all row tiles)
-            written(k_bar, lane);
-            if (tid < kTilesOf) note(step + 2);
-            copies_landed();
-            workers_sync<kWorkers>();
-            if (T == 2 && step + 2 < steps) fetch_k(step + 2);
+        meet(barrier, 64);
+        nan_groups = swap_bad[slot];
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const long long f = w.row0 + slot;
+        __half* to = a.out + ((long long)w.b * a.seq + (int)(f / a.share)) * a.heads * D + (w.kvh * a.share + (int)(f % a.share)) * D;
+        // columns of this half: pieces p = half D/64 .. of half-words, 32 columns each; 32/J adjacent dims of each 32 stand in a piece
+        constexpr int J = F::J;
 #pragma unroll
-            for (int t = 0; t < T; ++t) ok = ok && mbar_wait(smem_u32(&sm.pv_done[t]), step & 1, &sm.abort_flag, kWaitNs);
+        for (int c = 0; c < D / 64; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(at_o + 32 * c, o);
+            tmem_wait_ld();
+            if (f >= w.rows) continue;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float mul = nan_groups >> (32 * j * F::NG / D) & 1 ? __int_as_float(0x7fffffff) : inv;
+                __half* dims = to + 32 * j + (half * (D / 64) + c) * (32 / J);
+#pragma unroll
+                for (int r = 0; r < 8 / J; r += 2) {                                             // half-words r J + j of the piece: four dims each
+                    uint32_t h[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = (r + i / 2) * J + j + 16 * (i % 2);
+                        h[i] = h2_bits(__floats2half2_rn(__uint_as_float(o[at]) * mul, __uint_as_float(o[at + 8]) * mul));
+                    }
+                    *reinterpret_cast<uint4*>(dims + 4 * r) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            }
+        }
+    }
+};
+
+// ---- one row tile ------------------------------------------------------------------------------------------------------------------
+template <int D, int half_tile>
+struct SingleSmem {
+    alignas(1024) unsigned char q[kRows * D * 2], k[kTokens * D * 2], v[kTokens * D * 2];
+    alignas(16) unsigned char v_codes[kTilesOf * half_tile];                                     // (the keys' come through registers, or two CTAs would not fit)
+    Places places;
+    uint64_t s_done, pv_done;                     // products over
+    uint64_t k_ready, v_ready, p_ready;           // operands written
+    uint32_t tmem;
+    int abort_flag, any_bad;
+    int bad[kTokens];                             // groups of a token's value that are not finite
+    float swap[2 * kRows];
+    int swap_bad[kRows];
+};
+
+template <class F, int D>
+__global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs a)
+{
+    constexpr int NG = F::NG;
+    constexpr uint32_t kTmemCols = 256;           // S (then P) in 128 columns, O in the 128 behind them
+    extern __shared__ unsigned char raw[];
+    using S = SingleSmem<D, F::kBytes / 2>;
+    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    Task w;
+    if (!w.take(a, 1)) return;
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        mbar_init(smem_u32(&sm.s_done), 1);
+        mbar_init(smem_u32(&sm.pv_done), 1);
+        mbar_init(smem_u32(&sm.k_ready), 8);
+        mbar_init(smem_u32(&sm.v_ready), 8);
+        mbar_init(smem_u32(&sm.p_ready), 8);
+        sm.abort_flag = 0;
+        sm.any_bad = 0;
+    }
+    mbar_fence_init();
+    if (tid < kTokens) sm.bad[tid] = 0;
+    Lookup<F> lookup(a, w);
+    if (tid < kTilesOf)
+        for (int i = 0; i < 2; ++i) {
+            lookup.look(w, i, tid);
+            lookup.note(a, w, sm.places, i, tid);
+        }
+    __syncthreads();
+    const uint32_t tmem = sm.tmem, s_bar = smem_u32(&sm.s_done), pv_bar = smem_u32(&sm.pv_done), k_bar = smem_u32(&sm.k_ready),
+                   v_bar = smem_u32(&sm.v_ready), p_bar = smem_u32(&sm.p_ready);
+    bool ok = true;
+    auto wait = [&](uint32_t bar, int step) { ok = ok && mbar_wait(bar, step & 1, &sm.abort_flag, kWaitNs); };
+
+    if (warp == 8) {
+        // ---- the products.  P stands where S stood: S of a step is issued when P V of the step before is over
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q)), k_desc = smem_desc_sw128(smem_u32(sm.k)), v_desc = smem_desc_sw128(smem_u32(sm.v));
+        for (int step = 0; step < w.steps; ++step) {
+            wait(k_bar, step);
+            if (step > 0) wait(pv_bar, step - 1);
+            issue_s<D>(tmem, q_desc, k_desc, s_bar);
+            wait(v_bar, step);
+            wait(p_bar, step);
+            issue_pv<D>(tmem, v_desc, step == 0, pv_bar);
+        }
+        wait(pv_bar, w.steps - 1);
+        if (!ok && lane == 0) atomicExch(a.error, 1);
+        __syncthreads();                                                                         // the workers have read O
+        tmem_dealloc(tmem, kTmemCols);
+        return;
+    }
+
+    const KeyPlace<D> key(warp, lane);
+    constexpr int kPieces = KeyPlace<D>::kPieces;
+    uint4 kw[kPieces];
+    __half2 kp[kPieces][NG];
+    auto fetch_k = [&](int step) {
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int row = key.row + 64 * k;
+            const unsigned char* tile = sm.places.tile[step & 7][row >> 4];
+            kw[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) kp[k][g] = h2_of(0);
+            if (tile) {
+                kw[k] = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * key.kc);
+                load_params<NG>(tile + F::key_par(row & 15, 0), kp[k]);
+            }
+        }
+    };
+    auto put_k = [&]() {
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) put_key_piece<F, D>(sm.k, key.row + 64 * k, key.kc, kw[k], kp[k]);
+        written(k_bar, lane);
+    };
+    fetch_k(0);
+    load_codes<F, D>(sm.v_codes, sm.places, 0, true, tid, a.c.pool);
+    put_queries<D>(a, w, sm.q, w.row0, tid);
+    put_k();
+    copies_landed();
+    meet(9, kGroup);
+    Row<F, D> row(a, w, sm.swap, kRows, 0, warp, lane, tmem);
+    for (int step = 0; step < w.steps; ++step) {
+        // (P V of the step before is over)
+        if (put_values<F, D>(sm.v, sm.v_codes, sm.bad, w.last - step * kTokens, warp, lane)) sm.any_bad = 1;
+        written(v_bar, lane);
+        if (step + 1 < w.steps) fetch_k(step + 1);
+        if (tid < kTilesOf) lookup.look(w, step + 2, tid);
+        wait(s_bar, step);
+        tc_fence_after_sync();
+        const uint64_t pages = *reinterpret_cast<const uint64_t*>(sm.places.page_ok[step & 7]);
+        row.softmax(w, step, pages);
+        written(p_bar, lane);
+        meet(9, kGroup);                                                                         // everybody has read this step's codes
+        if (sm.any_bad) {
+            row.mind(sm.bad, step, pages);
+            meet(9, kGroup);
+            if (tid < kTokens) sm.bad[tid] = 0;
+            if (tid == 0) sm.any_bad = 0;
+        }
+        if (step + 1 < w.steps) {
+            load_codes<F, D>(sm.v_codes, sm.places, step + 1, true, tid, a.c.pool);
+            put_k();                                                                             // (S of this step is over)
+            if (tid < kTilesOf) lookup.note(a, w, sm.places, step + 2, tid);
+            copies_landed();
+            meet(9, kGroup);
+            wait(pv_bar, step);
             tc_fence_after_sync();
         }
     }
-    ok = ok && mbar_wait(smem_u32(&sm.pv_done[mine]), (steps - 1) & 1, &sm.abort_flag, kWaitNs);
+    wait(pv_bar, w.steps - 1);
     tc_fence_after_sync();
     if (!ok && lane == 0) atomicExch(a.error, 1);
-
-    // ---- out = O / sum
-    const float2 sums = unpair(sum2);
-    float sum = sums.x + sums.y;
-    sm.swap[half][slot] = sum;
-    if (half) sm.swap_bad[slot] = nan_groups;
-    workers_sync<kWorkers>();
-    sum += sm.swap[half ^ 1][slot];
-    if (!half) {
-        nan_groups |= sm.swap_bad[slot];
-        sm.swap_bad[slot] = nan_groups;
-    }
-    workers_sync<kWorkers>();
-    nan_groups = sm.swap_bad[slot];
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const long long f = row0 + slot;
-    __half* to = a.out + ((long long)b * a.seq + (int)(f / a.share)) * a.heads * D + (kvh * a.share + (int)(f % a.share)) * D;
-    // columns of this half: pieces p = half D/64 .. of half-words, 32 columns each; 32/J adjacent dims of each 32 stand in a piece
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(at_o + 32 * c, o);
-        tmem_wait_ld();
-        if (f >= rows) continue;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const float mul = nan_groups >> (32 * j * NG / D) & 1 ? __int_as_float(0x7fffffff) : inv;
-            __half* dims = to + 32 * j + (half * (D / 64) + c) * (32 / J);
-#pragma unroll
-            for (int r = 0; r < 8 / J; r += 2) {                                                 // half-words r J + j of the piece: four dims each
-                uint32_t h[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = (r + i / 2) * J + j + 16 * (i % 2);
-                    h[i] = h2_bits(__floats2half2_rn(__uint_as_float(o[at]) * mul, __uint_as_float(o[at + 8]) * mul));
-                }
-                *reinterpret_cast<uint4*>(dims + 4 * r) = make_uint4(h[0], h[1], h[2], h[3]);
-            }
-        }
-    }
+    row.finish(a, w, sm.swap_bad);
     tc_fence_before_sync();
     __syncthreads();
 }
 
-template <class F, int D, int T>
-int launch_prompt_as(PromptArgs& a, long long rows, int batch, cudaStream_t st)
+// ---- two row tiles that take turns ---------------------------------------------------------------------------------------------------
+template <int D, int half_tile>
+struct PairSmem {
+    alignas(1024) unsigned char q[2][kRows * D * 2], k[2][kTokens * D * 2], v[2][kTokens * D * 2];   // k, v: by step modulo 2
+    alignas(16) unsigned char codes[2][kTilesOf * half_tile];                                    // of the values (first group), of the keys
+    Places places[2];                             // the groups' own
+    uint64_t s_done[2], pv_done[2];               // products over, by row tile
+    uint64_t p_ready[2];                          // ... P written
+    uint64_t k_ready[2], v_ready[2];              // operands written, by step modulo 2
+    uint32_t tmem;
+    int abort_flag, any_bad[4];                   // by step modulo 4
+    int bad[4][kTokens];                          // groups of a token's value that are not finite
+    float swap[2 * 2 * kRows];
+    int swap_bad[2 * kRows];
+};
+
+template <class F, int D>
+__global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptArgs a)
 {
-    static int configured[64] = {0};   // benign race: the attribute call is idempotent
-    const int smem = (int)sizeof(Smem<D, F::kBytes / 2, T>) + 1024;
-    static_assert(sizeof(Smem<D, F::kBytes / 2, T>) + 1024 <= (T == 1 ? 115712 : 232448), "fits the SM");
+    constexpr int NG = F::NG, kHalf = F::kBytes / 2;
+    constexpr uint32_t kTmemCols = 512;           // a row tile's S (then P) in 128 columns, O in the 128 behind them
+    extern __shared__ unsigned char raw[];
+    using S = PairSmem<D, kHalf>;
+    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Task w;
+    if (!w.take(a, 2)) return;
+    if (warp == 16) {
+        tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
+        tmem_relinquish();
+    }
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(smem_u32(&sm.s_done[t]), 1);
+            mbar_init(smem_u32(&sm.pv_done[t]), 1);
+            mbar_init(smem_u32(&sm.p_ready[t]), 8);
+            mbar_init(smem_u32(&sm.k_ready[t]), 8);
+            mbar_init(smem_u32(&sm.v_ready[t]), 8);
+        }
+        sm.abort_flag = 0;
+    }
+    mbar_fence_init();
+    for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 32) sm.bad[0][i] = 0;
+    if (threadIdx.x < 4) sm.any_bad[threadIdx.x] = 0;
+    const int mine = warp >> 3, tid = threadIdx.x & (kGroup - 1), gwarp = warp & 7;              // the worker's row tile, its place in the group
+    Lookup<F> lookup(a, w);
+    if (mine < 2 && tid < kTilesOf)
+        for (int i = 0; i < 2; ++i) {
+            lookup.look(w, i, tid);
+            lookup.note(a, w, sm.places[mine], i, tid);
+        }
+    __syncthreads();
+    const uint32_t tmem = sm.tmem;
+    bool ok = true;
+    auto wait = [&](uint64_t& bar, int phase) { ok = ok && mbar_wait(smem_u32(&bar), phase & 1, &sm.abort_flag, kWaitNs); };
+
+    if (warp == 16) {
+        // ---- the products, in the order in which the groups take turns: P V of the first row tile, its next S, then the second's.  P stands
+        // where S stood: S of a step is issued when P V of the step before is over
+        uint64_t q_desc[2], k_desc[2], v_desc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            q_desc[t] = smem_desc_sw128(smem_u32(sm.q[t]));
+            k_desc[t] = smem_desc_sw128(smem_u32(sm.k[t]));
+            v_desc[t] = smem_desc_sw128(smem_u32(sm.v[t]));
+        }
+        wait(sm.k_ready[0], 0);
+        wait(sm.v_ready[0], 0);                                                                  // (with it the first group's queries)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) issue_s<D>(tmem + 256 * t, q_desc[t], k_desc[0], smem_u32(&sm.s_done[t]));
+        for (int step = 0; step < w.steps; ++step) {
+            const int now = step & 1, next = now ^ 1;
+            if (step > 0) wait(sm.v_ready[now], step >> 1);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                wait(sm.p_ready[t], step);
+                issue_pv<D>(tmem + 256 * t, v_desc[now], step == 0, smem_u32(&sm.pv_done[t]));
+                if (step + 1 < w.steps) {
+                    if (t == 0) wait(sm.k_ready[next], (step + 1) >> 1);
+                    wait(sm.pv_done[t], step);
+                    issue_s<D>(tmem + 256 * t, q_desc[t], k_desc[next], smem_u32(&sm.s_done[t]));
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) wait(sm.pv_done[t], w.steps - 1);
+        if (!ok && lane == 0) atomicExch(a.error, 1);
+        __syncthreads();                                                                         // the workers have read O
+        tmem_dealloc(tmem, kTmemCols);
+        return;
+    }
+
+    // ---- the groups: the first unpacks values, the second keys
+    Places& places = sm.places[mine];
+    unsigned char* codes = sm.codes[mine];
+    auto unpack = [&](int step, bool clear) {                                                    // into the buffer of step modulo 2
+        if (mine == 0) {
+            int* bad = sm.bad[step & 3];
+            if (clear) {
+                if (tid < kTokens) bad[tid] = 0;
+                if (tid == 0) sm.any_bad[step & 3] = 0;
+                meet(9, kGroup);
+            }
+            if (put_values<F, D>(sm.v[step & 1], codes, bad, w.last - step * kTokens, gwarp, lane)) sm.any_bad[step & 3] = 1;
+            written(smem_u32(&sm.v_ready[step & 1]), lane);
+        } else {
+            const KeyPlace<D> key(gwarp, lane);
+#pragma unroll
+            for (int k = 0; k < KeyPlace<D>::kPieces; ++k) {
+                const int row = key.row + 64 * k;
+                const unsigned char* tile = codes + (row >> 4) * kHalf;
+                __half2 par[NG];
+                load_params<NG>(tile + F::key_par(row & 15, 0), par);
+                put_key_piece<F, D>(sm.k[step & 1], row, key.kc, *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * piece_of<D>(row & 15, key.kc, false)), par);
+            }
+            written(smem_u32(&sm.k_ready[step & 1]), lane);
+        }
+    };
+    // the next step's codes, once this group has read the last ones; then where the tiles of the step after it stand
+    auto advance = [&](int step) {
+        if (tid < kTilesOf) lookup.note(a, w, places, step + 1, tid);
+        meet(9 + mine, kGroup);
+        if (step < w.steps) load_codes<F, D>(codes, places, step, mine == 0, tid, a.c.pool);
+        if (tid < kTilesOf) lookup.look(w, step + 2, tid);
+    };
+    auto unpack_next = [&](int step) {                                                           // what `advance` fetched
+        // (marks of four steps before: both row tiles have minded them.  Looked at before the barrier, behind which new ones are set)
+        const bool clear = mine == 0 && sm.any_bad[step & 3];
+        copies_landed();
+        meet(9 + mine, kGroup);
+        unpack(step, clear);
+        advance(step + 1);
+    };
+    load_codes<F, D>(codes, places, 0, mine == 0, tid, a.c.pool);
+    if (tid < kTilesOf) lookup.look(w, 2, tid);
+    put_queries<D>(a, w, sm.q[mine], w.row0 + mine * kRows, tid);
+    unpack_next(0);
+    Row<F, D> row(a, w, sm.swap, 2 * kRows, mine, gwarp, lane, tmem);
+    for (int step = 0; step < w.steps; ++step) {
+        // the second group unpacks first: the keys of the next step, whose buffer S of the step before has left
+        if (mine == 1 && step + 1 < w.steps) unpack_next(step + 1);                              // (products are over in the order of their issue)
+        wait(sm.s_done[mine], step);
+        tc_fence_after_sync();
+        if (step > 0 && sm.any_bad[(step - 1) & 3]) row.mind(sm.bad[(step - 1) & 3], step - 1, *reinterpret_cast<const uint64_t*>(places.page_ok[(step - 1) & 7]));
+        row.softmax(w, step, *reinterpret_cast<const uint64_t*>(places.page_ok[step & 7]));
+        // the first group unpacks afterwards: the values of the next step, whose buffer P V of the step before has left.  (Waited for before
+        // this step's P is announced: behind it the barrier could be two phases on.)
+        if (mine == 0 && step > 0) wait(sm.pv_done[1], step - 1);
+        written(smem_u32(&sm.p_ready[mine]), lane);
+        if (mine == 0 && step + 1 < w.steps) unpack_next(step + 1);
+    }
+    wait(sm.pv_done[mine], w.steps - 1);
+    tc_fence_after_sync();
+    if (!ok && lane == 0) atomicExch(a.error, 1);
+    if (sm.any_bad[(w.steps - 1) & 3])
+        row.mind(sm.bad[(w.steps - 1) & 3], w.steps - 1, *reinterpret_cast<const uint64_t*>(places.page_ok[(w.steps - 1) & 7]));
+    row.finish(a, w, sm.swap_bad);
+    tc_fence_before_sync();
+    __syncthreads();
+}
+
+template <class K>
+int launch_prompt_as(K kernel, int (&configured)[64], int smem, int tiles, PromptArgs& a, long long rows, int batch, cudaStream_t st)
+{
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return record_cuda_error(e);
-    if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(prompt_kernel<F, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (dev >= 64 || !configured[dev]) {               // benign race: the attribute call is idempotent
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return record_cuda_error(e);
         if (dev < 64) configured[dev] = 1;
     }
-    a.blocks = (int)((rows + T * kRows - 1) / (T * kRows));
-    prompt_kernel<F, D, T><<<dim3(a.blocks, a.c.kv_heads, batch), 256 * T + 32, smem, st>>>(a);
+    a.blocks = (int)((rows + tiles * kRows - 1) / (tiles * kRows));
+    kernel<<<dim3(a.blocks, a.c.kv_heads, batch), tiles * kGroup + 32, smem, st>>>(a);
     count_launch();
     e = cudaGetLastError();
     return e == cudaSuccess ? W4A16_OK : record_cuda_error(e);
+}
+
+template <class F, int D>
+int launch_prompt(PromptArgs& a, long long rows, int batch, cudaStream_t st)
+{
+    // (at 64 dims a step of K and V costs half as much, and two CTAs that wait for each other's products do better: 243 / 265 us for
+    // 2 x 2048 queries behind 1000 tokens, 32 heads on 8, before the row tiles took turns)
+    if constexpr (D == 128) {
+        if (rows > kRows) {
+            using S = PairSmem<D, F::kBytes / 2>;
+            static_assert(sizeof(S) + 1024 <= 232448, "fits the SM");
+            static int configured[64] = {0};
+            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, 2, a, rows, batch, st);
+        }
+    }
+    using S = SingleSmem<D, F::kBytes / 2>;
+    static_assert(sizeof(S) + 1024 <= 115712, "two fit the SM");
+    static int configured[64] = {0};
+    return launch_prompt_as(single_kernel<F, D>, configured, (int)sizeof(S) + 1024, 1, a, rows, batch, st);
 }
 
 }  // namespace
@@ -648,11 +870,6 @@ extern "C" int w4a16_kv4_attention(const void* qkv, const void* pool, const void
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        // (at 64 dims a tile of K and V costs half as much, and two CTAs that wait for each other's products do better: 243 / 265 us for
-        // 2 x 2048 queries behind 1000 tokens, 32 heads on 8; at 128 dims 1014 / 788 us for 4096 behind 4096)
-        if constexpr (F::NW == 16) {
-            if (rows > kRows) return launch_prompt_as<F, 128, 2>(a, rows, batch, (cudaStream_t)stream);
-        }
-        return launch_prompt_as<F, F::NW * 8, 1>(a, rows, batch, (cudaStream_t)stream);
+        return launch_prompt<F, F::NW * 8>(a, rows, batch, (cudaStream_t)stream);
     });
 }
