@@ -126,8 +126,20 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
           "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }      // this thread's
-// barriers of `threads` worker threads: 1 to 8 are the pairs of warps that share rows, 9 and 10 the row tiles'
+// barriers of `threads` worker threads: 1 to 8 are the pairs of warps that share rows
 __device__ __forceinline__ void meet(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t at, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+// the loads so far are over; s, of one of them, is not used before
+__device__ __forceinline__ void tmem_landed(uint32_t (&s)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(s[0]), "+r"(s[1]), "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7]), "+r"(s[8]), "+r"(s[9]), "+r"(s[10]),
+                   "+r"(s[11]), "+r"(s[12]), "+r"(s[13]), "+r"(s[14]), "+r"(s[15])::"memory");
+}
 // the warp's operand writes of either kind, made visible to the products, and its arrival
 __device__ __forceinline__ void written(uint32_t bar, int lane)
 {
@@ -143,7 +155,6 @@ __device__ __forceinline__ int operand_at(int rows, int r, int c) { return (c >>
 // What a CTA works on: `tiles` row tiles of one (batch row, key/value head).
 struct Task {
     int b, kvh, pos, last, steps; // last: the last token that any of its rows sees
-    int first_sees;               // ... and that its first row sees
     int last_i;
     long long rows, row0;         // rows there are, its first
     __device__ __forceinline__ bool take(const PromptArgs& a, int tiles)
@@ -162,40 +173,36 @@ struct Task {
         if (row0 >= rows) return false;
         last_i = (int)(min(row0 + tiles * kRows, rows) - 1) / a.share;
         last = pos + last_i;
-        first_sees = pos + (int)(row0 / a.share);
         steps = last / kTokens + 1;
         return true;
     }
 };
 
-// Where the 16-token tiles of the steps stand, by step modulo 8: looked up by threads 0 .. 7 of a row tile's group, two steps ahead.
-struct Places {
-    const unsigned char* tile[8][kTilesOf];       // null: behind the last token, or no page
-    unsigned char page_ok[8][kTilesOf];           // 0: a page is needed and is none of the pool
-};
+// A warp's 16-token tile of the steps: the page's number is fetched a step before the tile's place is needed.
 template <class F>
 struct Lookup {
     const int* ids;
     const unsigned char* head;
-    int tshift, next_id;
-    __device__ __forceinline__ Lookup(const PromptArgs& a, const Task& w) : tshift(a.c.page_shift - 4), next_id(-1)
+    long long page_bytes;
+    int tshift, last, pages, id, warp;            // id: of the step that was looked up
+    __device__ __forceinline__ Lookup(const PromptArgs& a, const Task& w, int warp_)
+        : ids(a.c.table + (size_t)w.b * a.c.width), head(a.c.pool + ((size_t)w.kvh << (a.c.page_shift - 4)) * F::kBytes), page_bytes(a.page_bytes),
+          tshift(a.c.page_shift - 4), last(w.last >> 4), pages(a.c.pages), warp(warp_)
     {
-        ids = a.c.table + (size_t)w.b * a.c.width;
-        head = a.c.pool + ((size_t)w.kvh << tshift) * F::kBytes;
+        look(0);
     }
-    __device__ __forceinline__ void look(const Task& w, int step, int i)
+    __device__ __forceinline__ void look(int step)
     {
-        const int t16 = step * kTilesOf + i;
-        next_id = t16 <= w.last >> 4 ? ids[t16 >> tshift] : -1;
+        const int t16 = step * kTilesOf + warp;
+        id = t16 <= last ? ids[t16 >> tshift] : 0;
     }
-    __device__ __forceinline__ void note(const PromptArgs& a, const Task& w, Places& p, int step, int i) const
+    // the tile; null: behind the last token, or no page
+    __device__ __forceinline__ const unsigned char* tile(int step) const
     {
-        const int t16 = step * kTilesOf + i;
-        const bool needed = t16 <= w.last >> 4, there = needed && (unsigned)next_id < (unsigned)a.c.pages;
-        p.tile[step & 7][i] = there ? head + next_id * a.page_bytes + (t16 & ((1 << tshift) - 1)) * F::kBytes : nullptr;
-        p.page_ok[step & 7][i] = there || !needed;
-        if (needed && !there) atomicExch(a.error, kErrPage);
+        const int t16 = step * kTilesOf + warp;
+        return t16 <= last && (unsigned)id < (unsigned)pages ? head + id * page_bytes + (t16 & ((1 << tshift) - 1)) * F::kBytes : nullptr;
     }
+    __device__ __forceinline__ bool fails(const unsigned char* tile, int step) const { return !tile && step * kTilesOf + warp <= last; }
 };
 
 // A code row's 16-byte pieces change places on their way to shared memory, so that the eight rows that are read together stand on different
@@ -205,22 +212,21 @@ __device__ __forceinline__ int piece_of(int row, int piece, bool values)
 {
     return D == 128 ? piece ^ (values ? (row >> 2) & 1 : (row >> 1) & 3) : piece ^ ((row >> 2) & 1);
 }
-// The keys' or the values' halves of a step's tiles to shared memory, by a row tile's group.
+// The keys' or the values' half of a warp's tile to shared memory.
 template <class F, int D>
-__device__ __forceinline__ void load_codes(unsigned char* to, const Places& p, int step, bool values, int tid, const unsigned char* any)
+__device__ __forceinline__ void load_codes(unsigned char* to, const unsigned char* tile, bool values, int lane, const unsigned char* any)
 {
-    constexpr int kHalf = F::kBytes / 2, kPieces = kHalf / 16, kRowPieces = D / 32;              // of a tile, of a code row
+    constexpr int kHalf = F::kBytes / 2, kPieces = kHalf / 16, kRowPieces = D / 32;              // of a half, of a code row
     static_assert(F::kVal == kHalf, "keys and values are halves of a tile");
+    const unsigned char* from = tile ? tile + (values ? kHalf : 0) : any;
 #pragma unroll
-    for (int i = 0; i < (kTilesOf * kPieces + kGroup - 1) / kGroup; ++i) {
-        const int at = tid + i * kGroup;
-        if (at >= kTilesOf * kPieces) break;
-        const unsigned char* tile = p.tile[step & 7][at / kPieces];
-        const int piece = at % kPieces, row = piece / kRowPieces;
+    for (int i = 0; i < (kPieces + 31) / 32; ++i) {
+        const int piece = lane + 32 * i, row = piece / kRowPieces;
         const int there = row < kTile ? row * kRowPieces + piece_of<D>(row, piece % kRowPieces, values) : piece;
         // (a tile that is none is filled with zeros: its values are 0, its keys are hidden)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                     ::"r"(smem_u32(to) + (at - piece + there) * 16), "l"(tile ? tile + (values ? kHalf : 0) + piece * 16 : any), "r"(tile ? 16 : 0) : "memory");
+        if (piece < kPieces)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                         ::"r"(smem_u32(to) + there * 16), "l"(tile ? from + piece * 16 : any), "r"(tile ? 16 : 0) : "memory");
     }
 }
 
@@ -240,64 +246,90 @@ __device__ __forceinline__ void put_key_piece(unsigned char* k, int row, int kc,
                                                                                h2_bits(__hfma2(n[2], s, m)), h2_bits(__hfma2(n[3], s, m)));
     }
 }
-// The keys a thread of a group takes: rows kt0 and (D = 128) kt0 + 64; eight lanes take eight rows, so that their stores fall on different banks.
+// The keys a lane takes of its warp's tile: rows `row` and (D = 128) row + 8; eight lanes take eight rows, so that their stores fall on
+// different banks.
 template <int D>
 struct KeyPlace {
     static constexpr int kPieces = D / 64;
     int row, kc;
-    __device__ __forceinline__ KeyPlace(int warp, int lane)
-        : row(D == 128 ? 8 * warp + (lane & 7) : 8 * (2 * warp + (lane >> 4)) + (lane & 7)), kc(D == 128 ? lane >> 3 : (lane >> 3) & 1) {}
+    __device__ __forceinline__ KeyPlace(int lane) : row(D == 128 ? lane & 7 : 8 * (lane >> 4) + (lane & 7)), kc(D == 128 ? lane >> 3 : (lane >> 3) & 1) {}
 };
 
-// 128 tokens' values to the operand, by a group: a warp takes groups of 8 tokens.  Matrix p of the load is the 16-byte piece p of the tokens'
-// rows: the lane gets half-word 8 p + lane / 4 of tokens 2 (lane % 4) and the next one, all of one group of dims.  True: some are not finite.
+// A tile's values to the operand, by a warp.  Matrix p of the loads is the 16-byte piece p of eight tokens' rows: the lane gets half-word
+// 8 p + lane / 4 of tokens 2 (lane % 4) and the next one, all of one group of dims.  `left`: tokens of the tile behind its first; bad: of the
+// tile's tokens.  True: some are not finite.
 template <class F, int D>
-__device__ __forceinline__ bool put_values(unsigned char* v, const unsigned char* codes, int* bad, int left_of_step, int warp, int lane)
+__device__ __forceinline__ bool put_values(unsigned char* v, const unsigned char* tile, int* bad, int left, int warp, int lane)
 {
-    constexpr int J = F::J, kHalf = F::kBytes / 2;
+    constexpr int J = F::J;
     const int vh = lane >> 2, vp2 = 2 * (lane & 3), vgroup = 32 * (vh % J) * F::NG / D;
-    bool found = false;
+    uint32_t w[2][J];
+    __half2 par[2][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int vt = warp + 8 * i, r0 = 8 * (vt & 1);
-        const unsigned char* tile = codes + (vt >> 1) * kHalf;
-        const int left = left_of_step - 8 * vt - vp2;                                            // tokens behind the lane's first
+    for (int i = 0; i < 2; ++i) {                                                                // tokens 8 i .. 8 i + 7
         // lane l gives the address of row l % 8 of matrix l / 8 (at D = 64, two matrices: lanes 16 .. 31 repeat)
-        const int lr = r0 + (lane & 7), lp = (lane >> 3) & (J - 1);
+        const int lr = 8 * i + (lane & 7), lp = (lane >> 3) & (J - 1);
         const int stored = D == 128 ? lp ^ (((lr >> 1) & 1) << 1) : lp;
         const uint32_t from = smem_u32(tile + lr * (D / 2) + 16 * piece_of<D>(lr, stored, true));
-        uint32_t w[J];
         if constexpr (J == 4)
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+                         : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3]) : "r"(from) : "memory");
         else
-            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
-        __half2 pa = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2, vgroup) - F::kVal);
-        __half2 pb = *reinterpret_cast<const __half2*>(tile + F::val_par(r0 + vp2 + 1, vgroup) - F::kVal);
-        if (left < 0) pa = h2_of(0);                                                             // behind the last token: whatever the page holds
-        if (left < 1) pb = h2_of(0);
-        const __half2 zero = __hfma2(pa, h2_of(0), __hmul2(pb, h2_of(0)));                       // NaN if one of them is not finite
-        if (!__hbeq2(zero, zero)) {
-            found = true;
-            if (!finite2(pa)) {
-                pa = h2_of(0);
-                atomicOr(&bad[8 * vt + vp2], 1 << vgroup);
-            }
-            if (!finite2(pb)) {
-                pb = h2_of(0);
-                atomicOr(&bad[8 * vt + vp2 + 1], 1 << vgroup);
-            }
+            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w[i][0]), "=r"(w[i][1]) : "r"(from) : "memory");
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            par[i][t] = *reinterpret_cast<const __half2*>(tile + F::val_par(8 * i + vp2 + t, vgroup) - F::kVal);
+            if (left < 8 * i + vp2 + t) par[i][t] = h2_of(0);                                    // behind the last token: whatever the page holds
         }
-        const __half2 s = __lows2half2(pa, pb), m = __highs2half2(pa, pb);
+    }
+    // NaN if one of them is not finite
+    const __half2 zero = __hfma2(par[0][0], h2_of(0), __hfma2(par[0][1], h2_of(0), __hfma2(par[1][0], h2_of(0), __hmul2(par[1][1], h2_of(0)))));
+    const bool found = !__hbeq2(zero, zero);
+    if (found) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (!finite2(par[i][t])) {
+                    par[i][t] = h2_of(0);
+                    atomicOr(&bad[8 * i + vp2 + t], 1 << vgroup);
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __half2 s = __lows2half2(par[i][0], par[i][1]), m = __highs2half2(par[i][0], par[i][1]);
 #pragma unroll
         for (int q = 0; q < J; ++q) {
             __half2 n[4];
-            codes8(w[q], n);
+            codes8(w[i][q], n);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) *reinterpret_cast<__half2*>(v + operand_at(D, 32 * q + 8 * d + vh, vt) + 2 * vp2) = __hfma2(n[d], s, m);
+            for (int d = 0; d < 4; ++d)
+                *reinterpret_cast<__half2*>(v + operand_at(D, 32 * q + 8 * d + vh, 2 * warp + i) + 2 * vp2) = __hfma2(n[d], s, m);
         }
     }
     return found;
+}
+
+// Marks of values that are not finite, by step modulo 4: a warp writes those of its tile when it unpacks the step (by then every row has
+// looked at those of four steps before), the rows look at them when the step's products are over.
+struct Marks {
+    unsigned char any[4][8];                      // a warp's tile has some
+    unsigned char page_ok[4][8];                  // 0: it stands on a page that is needed and is none of the pool
+    int bad[4][kTokens];                          // groups of a token's value that are not finite
+    __device__ __forceinline__ uint64_t pages(int step) const { return *reinterpret_cast<const uint64_t*>(page_ok[step & 3]); }
+    __device__ __forceinline__ bool some(int step) const { return *reinterpret_cast<const uint64_t*>(any[step & 3]) != 0; }
+};
+template <class F, int D>
+__device__ __forceinline__ void put_values_of(Marks& marks, unsigned char* v, const unsigned char* codes, const Task& w, int step, int warp, int lane)
+{
+    int* bad = &marks.bad[step & 3][kTile * warp];
+    if (marks.any[step & 3][warp]) {
+        if (lane < kTile) bad[lane] = 0;
+        __syncwarp();
+    }
+    const bool found = put_values<F, D>(v, codes, bad, w.last - step * kTokens - kTile * warp, warp, lane);
+    const int any = __any_sync(0xffffffffu, found);
+    if (lane == 0) marks.any[step & 3][warp] = (unsigned char)any;
 }
 
 // A row tile's queries to the operand, by its group, rotated as the decode kernel does and in the order of the keys' dims.  Adjacent lanes
@@ -355,7 +387,7 @@ struct Row {
     float* swap;                                  // [2][rows of the CTA]: what the two threads of a row tell each other
     int swap_rows, slot, half, barrier;
     uint32_t at_s, at_o;
-    int sees;                                     // last token it sees (rows behind the last: as that one)
+    int sees, first;                              // last token it sees (rows behind the last: as that one), that the tile's first row sees
     float unit, sign, ref;
     uint64_t sum2;
     int nan_groups;
@@ -369,41 +401,44 @@ struct Row {
         at_s = tmem + 256 * tile + ((uint32_t)(32 * (warp & 3)) << 16);
         at_o = at_s + kTokens + half * (D / 2);
         sees = w.pos + min((int)((w.row0 + slot) / a.share), w.last_i);
+        first = w.pos + (int)((w.row0 + tile * kRows) / a.share);
         // (the sign of a negative scale goes into the scores, so that `unit` is positive; a scale of zero makes them zero)
         unit = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
         sign = a.scale_log2 == 0.f ? 0.f : a.scale_log2 < 0.f ? -1.f : 1.f;
         sum2 = pair(0.f, 0.f);
     }
-    // S of a step becomes P
-    __device__ __forceinline__ void softmax(const Task& w, int step, uint64_t pages)
+    // S of a step becomes P; 16 scores at a time, the next ones on their way
+    __device__ __forceinline__ void softmax(int step, uint64_t pages)
     {
-        const bool masked = (step + 1) * kTokens - 1 > w.first_sees || pages != 0x0101010101010101ull;
-        const int from = step * kTokens + 64 * half;                                             // the thread's first token
-        uint32_t s[32];
-        auto fetch = [&](int c) {                                                                // scores of 32 tokens
-            tmem_ld_32x32b_x32(at_s + 64 * half + 32 * c, s);
-            tmem_wait_ld();
+        const bool masked = (step + 1) * kTokens - 1 > first || pages != 0x0101010101010101ull;
+        const int seen = sees - step * kTokens - 64 * half;                                      // the last of the thread's tokens that the row sees
+        const uint32_t ok4 = (uint32_t)(pages >> (32 * half));
+        auto ask = [&](int c, uint32_t (&s)[16]) { tmem_ld_32x32b_x16(at_s + 64 * half + 16 * c, s); };
+        auto take = [&](int c, uint32_t (&s)[16]) {
+            tmem_landed(s);
             if (sign != 1.f) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * sign);
+                for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * sign);
             }
             if (masked) {
-                const int seen = sees - (from + 32 * c);
-                const uint32_t p0 = (uint32_t)(pages >> (8 * (4 * half + 2 * c))) & 1, p1 = (uint32_t)(pages >> (8 * (4 * half + 2 * c + 1))) & 1;
+                const int last = ok4 >> (8 * c) & 1 ? seen - 16 * c : -1;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i > seen || !(i < 16 ? p0 : p1)) s[i] = 0xff800000u;
+                for (int i = 0; i < 16; ++i)
+                    if (i > last) s[i] = 0xff800000u;
             }
         };
+        uint32_t s[2][16];
         float top = -INFINITY;
+        ask(3, s[1]);
 #pragma unroll
-        for (int c = 1; c >= 0; --c) {
-            fetch(c);
+        for (int c = 3; c >= 0; --c) {
+            take(c, s[c & 1]);
+            ask(c > 0 ? c - 1 : 1, s[(c & 1) ^ 1]);                                              // (at last, the second sixteen for the weights)
             float t0 = top, t1 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                t0 = max3(t0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                t1 = max3(t1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+            for (int i = 0; i < 16; i += 4) {
+                t0 = max3(t0, __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
+                t1 = max3(t1, __uint_as_float(s[c & 1][i + 2]), __uint_as_float(s[c & 1][i + 3]));
             }
             top = fmaxf(t0, t1);
         }
@@ -432,23 +467,29 @@ struct Row {
         const float shift = ref == -INFINITY ? 0.f : -ref;                                       // nothing seen yet: weights 0
         const uint64_t unit2 = pair(unit, unit), shift2 = pair(shift, shift);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (c == 1) fetch(1);                                                                // (again: 64 at a time are too many registers)
-            uint32_t p[16];
+        for (int c = 0; c < 4; ++c) {
+            if (c > 0) {
+                take(c, s[c & 1]);
+                if (c < 3) ask(c + 1, s[(c & 1) ^ 1]);
+            }
+            uint32_t p[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 x = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), unit2, shift2));
+            for (int i = 0; i < 8; ++i) {
+                const float2 x = unpair(fma2(pair(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), unit2, shift2));
                 const float p0 = ex2(x.x), p1 = ex2(x.y);
                 sum2 = add2(sum2, pair(p0, p1));
                 p[i] = h2_bits(__floats2half2_rn(p0, p1));
             }
-            tmem_st_32x32b_x16(at_s + 64 * half + 16 * c, p);                                    // over columns that this thread has read
+            tmem_st_32x32b_x8(at_s + 64 * half + 8 * c, p);                                      // over columns that this thread has read
         }
         tmem_wait_st();
     }
     // the values of a step that are not finite
-    __device__ __forceinline__ void mind(const int* bad, int step, uint64_t pages)
+    __device__ __forceinline__ void mind(const Marks& marks, int step)
     {
+        if (!marks.some(step)) return;
+        const uint64_t pages = marks.pages(step);
+        const int* bad = marks.bad[step & 3];
 #pragma unroll 1
         for (int i = 64 * half; i < 64 * half + 64; ++i)
             if (step * kTokens + i <= sees && (pages >> (8 * (i >> 4)) & 1)) nan_groups |= bad[i];
@@ -504,12 +545,11 @@ template <int D, int half_tile>
 struct SingleSmem {
     alignas(1024) unsigned char q[kRows * D * 2], k[kTokens * D * 2], v[kTokens * D * 2];
     alignas(16) unsigned char v_codes[kTilesOf * half_tile];                                     // (the keys' come through registers, or two CTAs would not fit)
-    Places places;
+    Marks marks;
     uint64_t s_done, pv_done;                     // products over
     uint64_t k_ready, v_ready, p_ready;           // operands written
     uint32_t tmem;
-    int abort_flag, any_bad;
-    int bad[kTokens];                             // groups of a token's value that are not finite
+    int abort_flag;
     float swap[2 * kRows];
     int swap_bad[kRows];
 };
@@ -536,16 +576,11 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
         mbar_init(smem_u32(&sm.v_ready), 8);
         mbar_init(smem_u32(&sm.p_ready), 8);
         sm.abort_flag = 0;
-        sm.any_bad = 0;
     }
     mbar_fence_init();
-    if (tid < kTokens) sm.bad[tid] = 0;
-    Lookup<F> lookup(a, w);
-    if (tid < kTilesOf)
-        for (int i = 0; i < 2; ++i) {
-            lookup.look(w, i, tid);
-            lookup.note(a, w, sm.places, i, tid);
-        }
+    for (int i = tid; i < 4 * kTokens; i += kGroup + 32) sm.marks.bad[0][i] = 0;
+    if (tid < 4 * 8) sm.marks.any[0][tid] = 0;
+    Lookup<F> lookup(a, w, warp);
     __syncthreads();
     const uint32_t tmem = sm.tmem, s_bar = smem_u32(&sm.s_done), pv_bar = smem_u32(&sm.pv_done), k_bar = smem_u32(&sm.k_ready),
                    v_bar = smem_u32(&sm.v_ready), p_bar = smem_u32(&sm.p_ready);
@@ -570,67 +605,63 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
         return;
     }
 
-    const KeyPlace<D> key(warp, lane);
-    constexpr int kPieces = KeyPlace<D>::kPieces;
+    // ---- the workers: each warp unpacks a tile of the step, its keys by way of registers
+    const KeyPlace<D> key(lane);
+    constexpr int kPieces = KeyPlace<D>::kPieces, kHalf = F::kBytes / 2;
+    unsigned char* codes = sm.v_codes + warp * kHalf;
     uint4 kw[kPieces];
     __half2 kp[kPieces][NG];
-    auto fetch_k = [&](int step) {
+    bool page_fails = false;
+    auto fetch = [&](int step) {
+        const unsigned char* tile = lookup.tile(step);
+        page_fails = lookup.fails(tile, step);
+        load_codes<F, D>(codes, tile, true, lane, a.c.pool);
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
-            const int row = key.row + 64 * k;
-            const unsigned char* tile = sm.places.tile[step & 7][row >> 4];
             kw[k] = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int g = 0; g < NG; ++g) kp[k][g] = h2_of(0);
             if (tile) {
-                kw[k] = *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * key.kc);
-                load_params<NG>(tile + F::key_par(row & 15, 0), kp[k]);
+                kw[k] = *reinterpret_cast<const uint4*>(tile + (key.row + 8 * k) * (D / 2) + 16 * key.kc);
+                load_params<NG>(tile + F::key_par(key.row + 8 * k, 0), kp[k]);
             }
         }
+        lookup.look(step + 1);
     };
-    auto put_k = [&]() {
+    auto put_keys = [&](int step) {
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) put_key_piece<F, D>(sm.k, key.row + 64 * k, key.kc, kw[k], kp[k]);
+        for (int k = 0; k < kPieces; ++k) put_key_piece<F, D>(sm.k, kTile * warp + key.row + 8 * k, key.kc, kw[k], kp[k]);
+        if (lane == 0) {
+            sm.marks.page_ok[step & 3][warp] = !page_fails;
+            if (page_fails) atomicExch(a.error, kErrPage);
+        }
         written(k_bar, lane);
     };
-    fetch_k(0);
-    load_codes<F, D>(sm.v_codes, sm.places, 0, true, tid, a.c.pool);
+    fetch(0);
     put_queries<D>(a, w, sm.q, w.row0, tid);
-    put_k();
-    copies_landed();
-    meet(9, kGroup);
+    put_keys(0);
     Row<F, D> row(a, w, sm.swap, kRows, 0, warp, lane, tmem);
     for (int step = 0; step < w.steps; ++step) {
-        // (P V of the step before is over)
-        if (put_values<F, D>(sm.v, sm.v_codes, sm.bad, w.last - step * kTokens, warp, lane)) sm.any_bad = 1;
+        copies_landed();
+        __syncwarp();
+        put_values_of<F, D>(sm.marks, sm.v, codes, w, step, warp, lane);                         // (P V of the step before is over)
         written(v_bar, lane);
-        if (step + 1 < w.steps) fetch_k(step + 1);
-        if (tid < kTilesOf) lookup.look(w, step + 2, tid);
+        if (step + 1 < w.steps) fetch(step + 1);
         wait(s_bar, step);
         tc_fence_after_sync();
-        const uint64_t pages = *reinterpret_cast<const uint64_t*>(sm.places.page_ok[step & 7]);
-        row.softmax(w, step, pages);
+        row.softmax(step, sm.marks.pages(step));
         written(p_bar, lane);
-        meet(9, kGroup);                                                                         // everybody has read this step's codes
-        if (sm.any_bad) {
-            row.mind(sm.bad, step, pages);
-            meet(9, kGroup);
-            if (tid < kTokens) sm.bad[tid] = 0;
-            if (tid == 0) sm.any_bad = 0;
-        }
         if (step + 1 < w.steps) {
-            load_codes<F, D>(sm.v_codes, sm.places, step + 1, true, tid, a.c.pool);
-            put_k();                                                                             // (S of this step is over)
-            if (tid < kTilesOf) lookup.note(a, w, sm.places, step + 2, tid);
-            copies_landed();
-            meet(9, kGroup);
+            put_keys(step + 1);                                                                  // (S of this step is over)
             wait(pv_bar, step);
             tc_fence_after_sync();
+            row.mind(sm.marks, step);
         }
     }
     wait(pv_bar, w.steps - 1);
     tc_fence_after_sync();
     if (!ok && lane == 0) atomicExch(a.error, 1);
+    row.mind(sm.marks, w.steps - 1);
     row.finish(a, w, sm.swap_bad);
     tc_fence_before_sync();
     __syncthreads();
@@ -641,13 +672,12 @@ template <int D, int half_tile>
 struct PairSmem {
     alignas(1024) unsigned char q[2][kRows * D * 2], k[2][kTokens * D * 2], v[2][kTokens * D * 2];   // k, v: by step modulo 2
     alignas(16) unsigned char codes[2][kTilesOf * half_tile];                                    // of the values (first group), of the keys
-    Places places[2];                             // the groups' own
+    Marks marks;
     uint64_t s_done[2], pv_done[2];               // products over, by row tile
     uint64_t p_ready[2];                          // ... P written
     uint64_t k_ready[2], v_ready[2];              // operands written, by step modulo 2
     uint32_t tmem;
-    int abort_flag, any_bad[4];                   // by step modulo 4
-    int bad[4][kTokens];                          // groups of a token's value that are not finite
+    int abort_flag;
     float swap[2 * 2 * kRows];
     int swap_bad[2 * kRows];
 };
@@ -679,15 +709,10 @@ __global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptAr
         sm.abort_flag = 0;
     }
     mbar_fence_init();
-    for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 32) sm.bad[0][i] = 0;
-    if (threadIdx.x < 4) sm.any_bad[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 32) sm.marks.bad[0][i] = 0;
+    if (threadIdx.x < 4 * 8) sm.marks.any[0][threadIdx.x] = 0;
     const int mine = warp >> 3, tid = threadIdx.x & (kGroup - 1), gwarp = warp & 7;              // the worker's row tile, its place in the group
-    Lookup<F> lookup(a, w);
-    if (mine < 2 && tid < kTilesOf)
-        for (int i = 0; i < 2; ++i) {
-            lookup.look(w, i, tid);
-            lookup.note(a, w, sm.places[mine], i, tid);
-        }
+    Lookup<F> lookup(a, w, gwarp);
     __syncthreads();
     const uint32_t tmem = sm.tmem;
     bool ok = true;
@@ -729,70 +754,59 @@ __global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptAr
         return;
     }
 
-    // ---- the groups: the first unpacks values, the second keys
-    Places& places = sm.places[mine];
-    unsigned char* codes = sm.codes[mine];
-    auto unpack = [&](int step, bool clear) {                                                    // into the buffer of step modulo 2
+    // ---- the groups: the first unpacks values, the second keys, each warp a tile of the step
+    unsigned char* codes = sm.codes[mine] + gwarp * kHalf;
+    const KeyPlace<D> key(lane);
+    bool page_fails = false;
+    auto fetch = [&](int step) {                                                                 // the step's codes, and the page of the one behind it
+        const unsigned char* tile = lookup.tile(step);
+        page_fails = lookup.fails(tile, step);
+        load_codes<F, D>(codes, tile, mine == 0, lane, a.c.pool);
+        lookup.look(step + 1);
+    };
+    auto unpack = [&](int step) {                                                                // what was fetched, into the buffer of step modulo 2
+        copies_landed();
+        __syncwarp();
         if (mine == 0) {
-            int* bad = sm.bad[step & 3];
-            if (clear) {
-                if (tid < kTokens) bad[tid] = 0;
-                if (tid == 0) sm.any_bad[step & 3] = 0;
-                meet(9, kGroup);
-            }
-            if (put_values<F, D>(sm.v[step & 1], codes, bad, w.last - step * kTokens, gwarp, lane)) sm.any_bad[step & 3] = 1;
+            put_values_of<F, D>(sm.marks, sm.v[step & 1], codes, w, step, gwarp, lane);
             written(smem_u32(&sm.v_ready[step & 1]), lane);
         } else {
-            const KeyPlace<D> key(gwarp, lane);
 #pragma unroll
             for (int k = 0; k < KeyPlace<D>::kPieces; ++k) {
-                const int row = key.row + 64 * k;
-                const unsigned char* tile = codes + (row >> 4) * kHalf;
+                const int r = key.row + 8 * k;
                 __half2 par[NG];
-                load_params<NG>(tile + F::key_par(row & 15, 0), par);
-                put_key_piece<F, D>(sm.k[step & 1], row, key.kc, *reinterpret_cast<const uint4*>(tile + (row & 15) * (D / 2) + 16 * piece_of<D>(row & 15, key.kc, false)), par);
+                load_params<NG>(codes + F::key_par(r, 0), par);
+                put_key_piece<F, D>(sm.k[step & 1], kTile * gwarp + r, key.kc, *reinterpret_cast<const uint4*>(codes + r * (D / 2) + 16 * piece_of<D>(r, key.kc, false)), par);
+            }
+            if (lane == 0) {
+                sm.marks.page_ok[step & 3][gwarp] = !page_fails;
+                if (page_fails) atomicExch(a.error, kErrPage);
             }
             written(smem_u32(&sm.k_ready[step & 1]), lane);
         }
+        if (step + 1 < w.steps) fetch(step + 1);
     };
-    // the next step's codes, once this group has read the last ones; then where the tiles of the step after it stand
-    auto advance = [&](int step) {
-        if (tid < kTilesOf) lookup.note(a, w, places, step + 1, tid);
-        meet(9 + mine, kGroup);
-        if (step < w.steps) load_codes<F, D>(codes, places, step, mine == 0, tid, a.c.pool);
-        if (tid < kTilesOf) lookup.look(w, step + 2, tid);
-    };
-    auto unpack_next = [&](int step) {                                                           // what `advance` fetched
-        // (marks of four steps before: both row tiles have minded them.  Looked at before the barrier, behind which new ones are set)
-        const bool clear = mine == 0 && sm.any_bad[step & 3];
-        copies_landed();
-        meet(9 + mine, kGroup);
-        unpack(step, clear);
-        advance(step + 1);
-    };
-    load_codes<F, D>(codes, places, 0, mine == 0, tid, a.c.pool);
-    if (tid < kTilesOf) lookup.look(w, 2, tid);
+    fetch(0);
     put_queries<D>(a, w, sm.q[mine], w.row0 + mine * kRows, tid);
-    unpack_next(0);
+    unpack(0);
     Row<F, D> row(a, w, sm.swap, 2 * kRows, mine, gwarp, lane, tmem);
     for (int step = 0; step < w.steps; ++step) {
         // the second group unpacks first: the keys of the next step, whose buffer S of the step before has left
-        if (mine == 1 && step + 1 < w.steps) unpack_next(step + 1);                              // (products are over in the order of their issue)
+        if (mine == 1 && step + 1 < w.steps) unpack(step + 1);                                   // (products are over in the order of their issue)
         wait(sm.s_done[mine], step);
         tc_fence_after_sync();
-        if (step > 0 && sm.any_bad[(step - 1) & 3]) row.mind(sm.bad[(step - 1) & 3], step - 1, *reinterpret_cast<const uint64_t*>(places.page_ok[(step - 1) & 7]));
-        row.softmax(w, step, *reinterpret_cast<const uint64_t*>(places.page_ok[step & 7]));
+        if (step > 0) row.mind(sm.marks, step - 1);
+        row.softmax(step, sm.marks.pages(step));
         // the first group unpacks afterwards: the values of the next step, whose buffer P V of the step before has left.  (Waited for before
         // this step's P is announced: behind it the barrier could be two phases on.)
         if (mine == 0 && step > 0) wait(sm.pv_done[1], step - 1);
         written(smem_u32(&sm.p_ready[mine]), lane);
-        if (mine == 0 && step + 1 < w.steps) unpack_next(step + 1);
+        if (mine == 0 && step + 1 < w.steps) unpack(step + 1);
     }
     wait(sm.pv_done[mine], w.steps - 1);
     tc_fence_after_sync();
     if (!ok && lane == 0) atomicExch(a.error, 1);
-    if (sm.any_bad[(w.steps - 1) & 3])
-        row.mind(sm.bad[(w.steps - 1) & 3], w.steps - 1, *reinterpret_cast<const uint64_t*>(places.page_ok[(w.steps - 1) & 7]));
+    row.mind(sm.marks, w.steps - 1);
     row.finish(a, w, sm.swap_bad);
     tc_fence_before_sync();
     __syncthreads();
