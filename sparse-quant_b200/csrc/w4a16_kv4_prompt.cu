@@ -683,7 +683,7 @@ struct PairSmem {
 };
 
 template <class F, int D>
-__global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptArgs a)
+__global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptArgs a)
 {
     constexpr int NG = F::NG, kHalf = F::kBytes / 2;
     constexpr uint32_t kTmemCols = 512;           // a row tile's S (then P) in 128 columns, O in the 128 behind them
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptAr
         sm.abort_flag = 0;
     }
     mbar_fence_init();
-    for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 32) sm.marks.bad[0][i] = 0;
+    for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 128) sm.marks.bad[0][i] = 0;
     if (threadIdx.x < 4 * 8) sm.marks.any[0][threadIdx.x] = 0;
     const int mine = warp >> 3, tid = threadIdx.x & (kGroup - 1), gwarp = warp & 7;              // the worker's row tile, its place in the group
     Lookup<F> lookup(a, w, gwarp);
@@ -718,7 +718,12 @@ __global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptAr
     bool ok = true;
     auto wait = [&](uint64_t& bar, int phase) { ok = ok && mbar_wait(smem_u32(&bar), phase & 1, &sm.abort_flag, kWaitNs); };
 
-    if (warp == 16) {
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp > 16) {
+            __syncthreads();
+            return;
+        }
         // ---- the products, in the order in which the groups take turns: P V of the first row tile, its next S, then the second's.  P stands
         // where S stood: S of a step is issued when P V of the step before is over
         uint64_t q_desc[2], k_desc[2], v_desc[2];
@@ -754,6 +759,7 @@ __global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptAr
         return;
     }
 
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");  // the workers take what the products' warps leave: 16 x 104 + 4 x 56 of 20 x 96
     // ---- the groups: the first unpacks values, the second keys, each warp a tile of the step
     unsigned char* codes = sm.codes[mine] + gwarp * kHalf;
     const KeyPlace<D> key(lane);
@@ -813,7 +819,7 @@ __global__ void __launch_bounds__(2 * kGroup + 32, 1) pair_kernel(const PromptAr
 }
 
 template <class K>
-int launch_prompt_as(K kernel, int (&configured)[64], int smem, int tiles, PromptArgs& a, long long rows, int batch, cudaStream_t st)
+int launch_prompt_as(K kernel, int (&configured)[64], int smem, int tiles, int threads, PromptArgs& a, long long rows, int batch, cudaStream_t st)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -824,7 +830,7 @@ int launch_prompt_as(K kernel, int (&configured)[64], int smem, int tiles, Promp
         if (dev < 64) configured[dev] = 1;
     }
     a.blocks = (int)((rows + tiles * kRows - 1) / (tiles * kRows));
-    kernel<<<dim3(a.blocks, a.c.kv_heads, batch), tiles * kGroup + 32, smem, st>>>(a);
+    kernel<<<dim3(a.blocks, a.c.kv_heads, batch), threads, smem, st>>>(a);
     count_launch();
     e = cudaGetLastError();
     return e == cudaSuccess ? W4A16_OK : record_cuda_error(e);
@@ -840,13 +846,13 @@ int launch_prompt(PromptArgs& a, long long rows, int batch, cudaStream_t st)
             using S = PairSmem<D, F::kBytes / 2>;
             static_assert(sizeof(S) + 1024 <= 232448, "fits the SM");
             static int configured[64] = {0};
-            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, 2, a, rows, batch, st);
+            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, 2, 2 * kGroup + 128, a, rows, batch, st);
         }
     }
     using S = SingleSmem<D, F::kBytes / 2>;
     static_assert(sizeof(S) + 1024 <= 115712, "two fit the SM");
     static int configured[64] = {0};
-    return launch_prompt_as(single_kernel<F, D>, configured, (int)sizeof(S) + 1024, 1, a, rows, batch, st);
+    return launch_prompt_as(single_kernel<F, D>, configured, (int)sizeof(S) + 1024, 1, kGroup + 32, a, rows, batch, st);
 }
 
 }  // namespace
