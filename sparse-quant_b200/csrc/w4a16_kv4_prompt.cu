@@ -255,6 +255,19 @@ struct KeyPlace {
     __device__ __forceinline__ KeyPlace(int lane) : row(D == 128 ? lane & 7 : 8 * (lane >> 4) + (lane & 7)), kc(D == 128 ? lane >> 3 : (lane >> 3) & 1) {}
 };
 
+template <class F, int D>
+__device__ __forceinline__ void put_keys(unsigned char* k, const unsigned char* codes, int warp, int lane)
+{
+    const KeyPlace<D> key(lane);
+#pragma unroll
+    for (int i = 0; i < KeyPlace<D>::kPieces; ++i) {
+        const int r = key.row + 8 * i;
+        __half2 par[F::NG];
+        load_params<F::NG>(codes + F::key_par(r, 0), par);
+        put_key_piece<F, D>(k, kTile * warp + r, key.kc, *reinterpret_cast<const uint4*>(codes + r * (D / 2) + 16 * piece_of<D>(r, key.kc, false)), par);
+    }
+}
+
 // A tile's values to the operand, by a warp.  Matrix p of the loads is the 16-byte piece p of eight tokens' rows: the lane gets half-word
 // 8 p + lane / 4 of tokens 2 (lane % 4) and the next one, all of one group of dims.  `left`: tokens of the tile behind its first; bad: of the
 // tile's tokens.  True: some are not finite.
@@ -544,7 +557,7 @@ struct Row {
 template <int D, int half_tile>
 struct SingleSmem {
     alignas(1024) unsigned char q[kRows * D * 2], k[kTokens * D * 2], v[kTokens * D * 2];
-    alignas(16) unsigned char v_codes[kTilesOf * half_tile];                                     // (the keys' come through registers, or two CTAs would not fit)
+    alignas(16) unsigned char codes[kTilesOf * half_tile];                                       // of keys and values in turn, or two CTAs would not fit
     Marks marks;
     uint64_t s_done, pv_done;                     // products over
     uint64_t k_ready, v_ready, p_ready;           // operands written
@@ -557,7 +570,7 @@ struct SingleSmem {
 template <class F, int D>
 __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs a)
 {
-    constexpr int NG = F::NG;
+    constexpr int kHalf = F::kBytes / 2;
     constexpr uint32_t kTmemCols = 256;           // S (then P) in 128 columns, O in the 128 behind them
     extern __shared__ unsigned char raw[];
     using S = SingleSmem<D, F::kBytes / 2>;
@@ -605,41 +618,30 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
         return;
     }
 
-    // ---- the workers: each warp unpacks a tile of the step, its keys by way of registers
-    const KeyPlace<D> key(lane);
-    constexpr int kPieces = KeyPlace<D>::kPieces, kHalf = F::kBytes / 2;
-    unsigned char* codes = sm.v_codes + warp * kHalf;
-    uint4 kw[kPieces];
-    __half2 kp[kPieces][NG];
-    bool page_fails = false;
-    auto fetch = [&](int step) {
-        const unsigned char* tile = lookup.tile(step);
-        page_fails = lookup.fails(tile, step);
-        load_codes<F, D>(codes, tile, true, lane, a.c.pool);
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            kw[k] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) kp[k][g] = h2_of(0);
-            if (tile) {
-                kw[k] = *reinterpret_cast<const uint4*>(tile + (key.row + 8 * k) * (D / 2) + 16 * key.kc);
-                load_params<NG>(tile + F::key_par(key.row + 8 * k, 0), kp[k]);
-            }
+    // ---- the workers: each warp unpacks a tile of the step
+    unsigned char* codes = sm.codes + warp * kHalf;
+    const unsigned char* tile = nullptr;
+    auto fetch = [&](int step) {                                                                 // the keys' codes, and the page of the step behind
+        tile = lookup.tile(step);
+        load_codes<F, D>(codes, tile, false, lane, a.c.pool);
+        if (tile && lane * 128 < kHalf) asm volatile("prefetch.global.L2 [%0];" ::"l"(tile + kHalf + lane * 128));
+        if (lane == 0) {
+            const bool fails = lookup.fails(tile, step);
+            sm.marks.page_ok[step & 3][warp] = !fails;
+            if (fails) atomicExch(a.error, kErrPage);
         }
         lookup.look(step + 1);
     };
-    auto put_keys = [&](int step) {
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k) put_key_piece<F, D>(sm.k, kTile * warp + key.row + 8 * k, key.kc, kw[k], kp[k]);
-        if (lane == 0) {
-            sm.marks.page_ok[step & 3][warp] = !page_fails;
-            if (page_fails) atomicExch(a.error, kErrPage);
-        }
+    auto unpack_keys = [&]() {
+        copies_landed();
+        __syncwarp();
+        put_keys<F, D>(sm.k, codes, warp, lane);
         written(k_bar, lane);
+        load_codes<F, D>(codes, tile, true, lane, a.c.pool);
     };
     fetch(0);
     put_queries<D>(a, w, sm.q, w.row0, tid);
-    put_keys(0);
+    unpack_keys();
     Row<F, D> row(a, w, sm.swap, kRows, 0, warp, lane, tmem);
     for (int step = 0; step < w.steps; ++step) {
         copies_landed();
@@ -652,7 +654,7 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
         row.softmax(step, sm.marks.pages(step));
         written(p_bar, lane);
         if (step + 1 < w.steps) {
-            put_keys(step + 1);                                                                  // (S of this step is over)
+            unpack_keys();                                                                       // (S of this step is over)
             wait(pv_bar, step);
             tc_fence_after_sync();
             row.mind(sm.marks, step);
@@ -685,7 +687,7 @@ struct PairSmem {
 template <class F, int D>
 __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptArgs a)
 {
-    constexpr int NG = F::NG, kHalf = F::kBytes / 2;
+    constexpr int kHalf = F::kBytes / 2;
     constexpr uint32_t kTmemCols = 512;           // a row tile's S (then P) in 128 columns, O in the 128 behind them
     extern __shared__ unsigned char raw[];
     using S = PairSmem<D, kHalf>;
@@ -762,7 +764,6 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");  // the workers take what the products' warps leave: 16 x 104 + 4 x 56 of 20 x 96
     // ---- the groups: the first unpacks values, the second keys, each warp a tile of the step
     unsigned char* codes = sm.codes[mine] + gwarp * kHalf;
-    const KeyPlace<D> key(lane);
     bool page_fails = false;
     auto fetch = [&](int step) {                                                                 // the step's codes, and the page of the one behind it
         const unsigned char* tile = lookup.tile(step);
@@ -777,13 +778,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
             put_values_of<F, D>(sm.marks, sm.v[step & 1], codes, w, step, gwarp, lane);
             written(smem_u32(&sm.v_ready[step & 1]), lane);
         } else {
-#pragma unroll
-            for (int k = 0; k < KeyPlace<D>::kPieces; ++k) {
-                const int r = key.row + 8 * k;
-                __half2 par[NG];
-                load_params<NG>(codes + F::key_par(r, 0), par);
-                put_key_piece<F, D>(sm.k[step & 1], kTile * gwarp + r, key.kc, *reinterpret_cast<const uint4*>(codes + r * (D / 2) + 16 * piece_of<D>(r, key.kc, false)), par);
-            }
+            put_keys<F, D>(sm.k[step & 1], codes, gwarp, lane);
             if (lane == 0) {
                 sm.marks.page_ok[step & 3][gwarp] = !page_fails;
                 if (page_fails) atomicExch(a.error, kErrPage);
