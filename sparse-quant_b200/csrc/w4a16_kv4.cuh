@@ -125,25 +125,31 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
     }
 }
 
-// Word w (dims 8w .. 8w+7) of a head row at `src` with the rotary embedding of position t ("rotate half"), rounded to fp16 as the
-// fp16 cache holds keys; fp32 products and sum, each rounded.
-template <int D>
-__device__ __forceinline__ uint4 load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t)
+// A word (8 dims) of a head row with the rotary embedding ("rotate half"), rounded to fp16 as the fp16 cache holds keys; fp32 products
+// and sum, each rounded.  y: the word half a row away; sign: -1 in the row's first half.
+__device__ __forceinline__ uint4 rotate(const uint4& x8, const uint4& y8, const uint4& cos8, const uint4& sin8, float sign)
 {
-    uint4 out = *reinterpret_cast<const uint4*>(src + 8 * w);
-    if (!cos) return out;
+    uint4 out;
     float x[8], y[8], c[8], s[8];
-    unpack8(out, x);
-    unpack8(*reinterpret_cast<const uint4*>(src + 8 * (w ^ (D / 16))), y);
-    unpack8(*reinterpret_cast<const uint4*>(cos + (size_t)t * D + 8 * w), c);
-    unpack8(*reinterpret_cast<const uint4*>(sin + (size_t)t * D + 8 * w), s);
-    const float sign = w < D / 16 ? -1.f : 1.f;
+    unpack8(x8, x);
+    unpack8(y8, y);
+    unpack8(cos8, c);
+    unpack8(sin8, s);
     __half2* o = reinterpret_cast<__half2*>(&out);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         o[e] = __floats2half2_rn(__fadd_rn(__fmul_rn(x[2 * e], c[2 * e]), __fmul_rn(sign * y[2 * e], s[2 * e])),
                                  __fadd_rn(__fmul_rn(x[2 * e + 1], c[2 * e + 1]), __fmul_rn(sign * y[2 * e + 1], s[2 * e + 1])));
     return out;
+}
+// Word w (dims 8w .. 8w+7) of a head row at `src`, rotated for position t where there are tables.
+template <int D>
+__device__ __forceinline__ uint4 load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t)
+{
+    const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * w);
+    if (!cos) return x;
+    return rotate(x, *reinterpret_cast<const uint4*>(src + 8 * (w ^ (D / 16))), *reinterpret_cast<const uint4*>(cos + (size_t)t * D + 8 * w),
+                  *reinterpret_cast<const uint4*>(sin + (size_t)t * D + 8 * w), w < D / 16 ? -1.f : 1.f);
 }
 template <int D>
 __device__ __forceinline__ void load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t, float (&x)[8])

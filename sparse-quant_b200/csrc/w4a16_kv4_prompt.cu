@@ -345,23 +345,54 @@ __device__ __forceinline__ void put_values_of(Marks& marks, unsigned char* v, co
     if (lane == 0) marks.any[step & 3][warp] = (unsigned char)any;
 }
 
-// A row tile's queries to the operand, by its group, rotated as the decode kernel does and in the order of the keys' dims.  Adjacent lanes
-// take adjacent words of a row (two threads a row, each with half of its words, took 258 us instead of 106 for 8 x 512 rotated queries).
+// A row tile's queries to the operand, by its group, rotated as the decode kernel does and in the order of the keys' dims.  A thread takes
+// words w and w + D / 16, which rotate into each other; adjacent lanes take adjacent words, and two rows' words are on their way at once (one
+// row after the other, by two threads a row: 14600 cycles before the first product; so: 9500).
 template <int D>
 __device__ __forceinline__ void put_queries(const PromptArgs& a, const Task& w, unsigned char* q, long long first, int tid)
 {
-    constexpr int kWords = D / 8, kAtOnce = kGroup / kWords;                                     // rows at once
-    const int word = tid % kWords, i0 = (int)(first / a.share), h0 = (int)(first % a.share);
-    const __half* from = a.qkv + ((long long)w.b * a.seq + i0) * a.stride + (long long)w.kvh * a.share * D;
-    const int left = (int)min(w.rows - first, (long long)kRows);
-#pragma unroll 4
-    for (int r = tid / kWords; r < kRows; r += kAtOnce) {
-        const int i = (h0 + r) / a.share, h = h0 + r - i * a.share;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (r < left) load_rotated<D>(from + i * a.stride + h * D, word, a.cos, a.sin, w.pos + i0 + i, x);
-        *reinterpret_cast<uint4*>(q + operand_at(kRows, r, word)) =
-            make_uint4(h2_bits(__floats2half2_rn(x[0], x[4])), h2_bits(__floats2half2_rn(x[1], x[5])), h2_bits(__floats2half2_rn(x[2], x[6])),
-                       h2_bits(__floats2half2_rn(x[3], x[7])));
+    constexpr int kHalfWords = D / 16, kApart = kGroup / kHalfWords, kAtOnce = 2;
+    const int word = tid % kHalfWords, i0 = (int)(first / a.share), h0 = (int)(first % a.share);
+    const __half* from = a.qkv + ((long long)w.b * a.seq + i0) * a.stride + (long long)w.kvh * a.share * D + 8 * word;
+    const int left = (int)max(0ll, min(w.rows - first, (long long)kRows));
+    auto put = [&](int r, const uint4& x, int k) {
+        *reinterpret_cast<uint4*>(q + operand_at(kRows, r, word + k * kHalfWords)) =
+            r < left ? make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632))
+                     : make_uint4(0, 0, 0, 0);
+    };
+#pragma unroll 1
+    for (int r0 = tid / kHalfWords; r0 < kRows; r0 += kAtOnce * kApart) {
+        uint4 x[kAtOnce][2], c[kAtOnce][2], s[kAtOnce][2];
+        int i[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int r = min(r0 + u * kApart, max(left - 1, 0));                                // (rows behind the last: as that one, or the first)
+            i[u] = (h0 + r) / a.share;
+            const __half* at = left ? from + i[u] * a.stride + (h0 + r - i[u] * a.share) * D : a.qkv;
+            x[u][0] = *reinterpret_cast<const uint4*>(at);
+            x[u][1] = *reinterpret_cast<const uint4*>(at + D / 2);
+        }
+        if (a.cos) {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const size_t at = (left ? (size_t)(w.pos + i0 + i[u]) * D : 0) + 8 * (word + k * kHalfWords);
+                    c[u][k] = *reinterpret_cast<const uint4*>(a.cos + at);
+                    s[u][k] = *reinterpret_cast<const uint4*>(a.sin + at);
+                }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                put(r0 + u * kApart, rotate(x[u][0], x[u][1], c[u][0], s[u][0], -1.f), 0);
+                put(r0 + u * kApart, rotate(x[u][1], x[u][0], c[u][1], s[u][1], 1.f), 1);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                put(r0 + u * kApart, x[u][0], 0);
+                put(r0 + u * kApart, x[u][1], 1);
+            }
+        }
     }
 }
 
@@ -371,12 +402,14 @@ __device__ __forceinline__ void issue_s(uint32_t s, uint64_t q_desc, uint64_t k_
 {
     tc_fence_after_sync();
     __syncwarp();
+    if (elect_one()) {
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t at = (uint64_t)((kk >> 2) * (kRows * 128 / 16) + 2 * (kk & 3));
-        if (elect_one()) mma_f16_ss(s, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
+        for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t at = (uint64_t)((kk >> 2) * (kRows * 128 / 16) + 2 * (kk & 3));
+            mma_f16_ss(s, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
+        }
+        tc_commit(done);
     }
-    if (elect_one()) tc_commit(done);
     __syncwarp();
 }
 template <int D>
@@ -384,13 +417,15 @@ __device__ __forceinline__ void issue_pv(uint32_t s, uint64_t v_desc, bool first
 {
     tc_fence_after_sync();
     __syncwarp();
+    if (elect_one()) {
 #pragma unroll
-    for (int kk = 0; kk < kTokens / 16; ++kk) {
-        // P of tokens 0 .. 63 stands in columns 0 .. 31, of tokens 64 .. 127 in columns 64 .. 95
-        const uint64_t at = (uint64_t)((kk >> 2) * (D * 128 / 16) + 2 * (kk & 3));
-        if (elect_one()) mma_f16_ts(s + kTokens, s + (kk >> 2) * 64 + (kk & 3) * 8, v_desc + at, idesc_f16_m128(D), !first || kk > 0);
+        for (int kk = 0; kk < kTokens / 16; ++kk) {
+            // P of tokens 0 .. 63 stands in columns 0 .. 31, of tokens 64 .. 127 in columns 64 .. 95
+            const uint64_t at = (uint64_t)((kk >> 2) * (D * 128 / 16) + 2 * (kk & 3));
+            mma_f16_ts(s + kTokens, s + (kk >> 2) * 64 + (kk & 3) * 8, v_desc + at, idesc_f16_m128(D), !first || kk > 0);
+        }
+        tc_commit(done);
     }
-    if (elect_one()) tc_commit(done);
     __syncwarp();
 }
 
@@ -728,28 +763,23 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
         }
         // ---- the products, in the order in which the groups take turns: P V of the first row tile, its next S, then the second's.  P stands
         // where S stood: S of a step is issued when P V of the step before is over
-        uint64_t q_desc[2], k_desc[2], v_desc[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            q_desc[t] = smem_desc_sw128(smem_u32(sm.q[t]));
-            k_desc[t] = smem_desc_sw128(smem_u32(sm.k[t]));
-            v_desc[t] = smem_desc_sw128(smem_u32(sm.v[t]));
-        }
+        constexpr int kOperand = kRows * D * 2 / 16;                                             // q, k and v of two buffers each, one behind the other
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q[0]));
         wait(sm.k_ready[0], 0);
         wait(sm.v_ready[0], 0);                                                                  // (with it the first group's queries)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) issue_s<D>(tmem + 256 * t, q_desc[t], k_desc[0], smem_u32(&sm.s_done[t]));
+        for (int t = 0; t < 2; ++t) issue_s<D>(tmem + 256 * t, q_desc + t * kOperand, q_desc + 2 * kOperand, smem_u32(&sm.s_done[t]));
         for (int step = 0; step < w.steps; ++step) {
             const int now = step & 1, next = now ^ 1;
             if (step > 0) wait(sm.v_ready[now], step >> 1);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 wait(sm.p_ready[t], step);
-                issue_pv<D>(tmem + 256 * t, v_desc[now], step == 0, smem_u32(&sm.pv_done[t]));
+                issue_pv<D>(tmem + 256 * t, q_desc + (4 + now) * kOperand, step == 0, smem_u32(&sm.pv_done[t]));
                 if (step + 1 < w.steps) {
                     if (t == 0) wait(sm.k_ready[next], (step + 1) >> 1);
                     wait(sm.pv_done[t], step);
-                    issue_s<D>(tmem + 256 * t, q_desc[t], k_desc[next], smem_u32(&sm.s_done[t]));
+                    issue_s<D>(tmem + 256 * t, q_desc + t * kOperand, q_desc + (2 + next) * kOperand, smem_u32(&sm.s_done[t]));
                 }
             }
         }
