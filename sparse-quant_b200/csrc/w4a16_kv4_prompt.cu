@@ -14,9 +14,10 @@
 // softmax, eight warps a row tile, and one warp that issues the products (issuing eight takes as long as they run).
 //
 // What bounds it is what the workers can issue, and the exponentials (16 a clock): a step of K and V costs as much to unpack as a row tile's
-// softmax.  For more than 128 rows of 128 dims a CTA has two row tiles (pair_kernel, one CTA an SM), whose warps take turns: while one
+// softmax.  Where there are many row tiles of 128 dims a CTA has two (pair_kernel, one CTA an SM), whose warps take turns: while one
 // row tile is in its softmax the other's warps unpack - the first row tile's the values, the second's the keys, into two buffers each -, and
-// the tensor cores run the products of whichever is ready.  Otherwise (single_kernel) one row tile, two CTAs an SM.
+// the tensor cores run the products of whichever is ready.  Otherwise (single_kernel) one row tile, two CTAs an SM; where there are few, the
+// CTAs of a cluster share the steps of a row tile and join their (reference, sum, O) through each other's shared memory.
 //
 // A value whose group is not finite is multiplied as 0, so that rows that must not see its token stay clean, and the rows that do see it
 // get NaN for that group's dims at the end.
@@ -32,6 +33,8 @@ using namespace sm100;
 constexpr int kRows = 128, kTokens = 128;
 constexpr int kTilesOf = kTokens / kTile;         // 16-token tiles of a step
 constexpr int kGroup = 256;                       // worker threads of a row tile
+constexpr int kMostRanks = 8;                     // of a cluster: the portable size
+constexpr int kLeastSteps = 2;                    // joining a row tile's parts costs about one
 constexpr uint64_t kWaitNs = 400000000ull;        // a product that has not finished by then never will: error word 1
 
 struct PromptArgs {
@@ -44,7 +47,8 @@ struct PromptArgs {
     const __half* sin;
     int* error;
     int seq, heads, share;        // share: query heads of a key/value head
-    int blocks;                   // CTAs of a (batch row, key/value head)
+    int blocks;                   // row tiles (single_kernel; else pairs of them) of a (batch row, key/value head)
+    int batch, ranks, slots;      // ranks: CTAs of a cluster, which may share a row tile's steps; slots: CTAs the GPU holds
     int rope_rows;
     long long stride, page_bytes;
     float scale_log2;             // scale * log2(e)
@@ -155,11 +159,14 @@ __device__ __forceinline__ int operand_at(int rows, int r, int c) { return (c >>
 // What a CTA works on: `tiles` row tiles of one (batch row, key/value head).
 struct Task {
     int b, kvh, pos, last, steps; // last: the last token that any of its rows sees
+    int rank, parts, from, to;    // of a cluster's CTAs the first `parts` have steps, this one from .. to - 1
     int last_i;
     long long rows, row0;         // rows there are, its first
+    // tiles: row tiles of a CTA; kParts: clusters may share their steps
+    template <bool kParts>
     __device__ __forceinline__ bool take(const PromptArgs& a, int tiles)
     {
-        const int block = a.blocks - 1 - (int)blockIdx.x;                                        // the longest rows first
+        const int block = a.blocks - 1 - (int)blockIdx.x / (kParts ? a.ranks : 1);                              // the longest rows first
         kvh = blockIdx.y;
         b = blockIdx.z;
         pos = a.pos[b];
@@ -174,7 +181,25 @@ struct Task {
         last_i = (int)(min(row0 + tiles * kRows, rows) - 1) / a.share;
         last = pos + last_i;
         steps = last / kTokens + 1;
+        rank = kParts ? (int)blockIdx.x % a.ranks : 0;
+        parts = 1;
+        if (kParts && a.ranks > 1) parts = min(a.ranks, max(1, steps / share_of_steps(a)));
+        from = (int)((long long)steps * rank / parts);
+        to = rank < parts ? (int)((long long)steps * (rank + 1) / parts) : from;
         return true;
+    }
+    // The steps that a CTA should have if all of the call were dealt evenly over the GPU, by every warp.
+    __device__ __forceinline__ static int share_of_steps(const PromptArgs& a)
+    {
+        long long all = 0;
+        for (int r = threadIdx.x & 31; r < a.batch; r += 32) {
+            const int at = a.pos[r], n = a.counts ? min(a.counts[r], a.seq) : a.seq;
+            const long long end = min((long long)at + n, (long long)a.c.capacity());
+            if (at >= 0 && n > 0) all += (end + kTokens - 1) / kTokens * (((long long)n * a.share + kRows - 1) / kRows);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        return (int)min(max(all * a.c.kv_heads / a.slots, (long long)kLeastSteps), 1ll << 30);
     }
 };
 
@@ -185,11 +210,11 @@ struct Lookup {
     const unsigned char* head;
     long long page_bytes;
     int tshift, last, pages, id, warp;            // id: of the step that was looked up
-    __device__ __forceinline__ Lookup(const PromptArgs& a, const Task& w, int warp_)
+    __device__ __forceinline__ Lookup(const PromptArgs& a, const Task& w, int warp_, int from)
         : ids(a.c.table + (size_t)w.b * a.c.width), head(a.c.pool + ((size_t)w.kvh << (a.c.page_shift - 4)) * F::kBytes), page_bytes(a.page_bytes),
           tshift(a.c.page_shift - 4), last(w.last >> 4), pages(a.c.pages), warp(warp_)
     {
-        look(0);
+        look(from);
     }
     __device__ __forceinline__ void look(int step)
     {
@@ -429,6 +454,9 @@ __device__ __forceinline__ void issue_pv(uint32_t s, uint64_t v_desc, bool first
     __syncwarp();
 }
 
+// floats of a row of a part's O: columns 32 p .. from 40 p on, so that the lanes of either access touch different banks
+__host__ __device__ constexpr int part_pitch(int dims) { return dims + dims / 4 + 4; }
+
 // A thread's row in the softmax, and its half of the columns.
 template <class F, int D>
 struct Row {
@@ -456,7 +484,7 @@ struct Row {
         sum2 = pair(0.f, 0.f);
     }
     // S of a step becomes P; 16 scores at a time, the next ones on their way
-    __device__ __forceinline__ void softmax(int step, uint64_t pages)
+    __device__ __forceinline__ void softmax(int step, bool first_step, uint64_t pages)
     {
         const bool masked = (step + 1) * kTokens - 1 > first || pages != 0x0101010101010101ull;
         const int seen = sees - step * kTokens - 64 * half;                                      // the last of the thread's tokens that the row sees
@@ -500,7 +528,7 @@ struct Row {
             ref = to;
             const float2 f = unpair(sum2);
             sum2 = pair(f.x * keep, f.y * keep);
-            if (step > 0) {
+            if (!first_step) {
                 uint32_t o[16];
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
@@ -542,8 +570,8 @@ struct Row {
         for (int i = 64 * half; i < 64 * half + 64; ++i)
             if (step * kTokens + i <= sees && (pages >> (8 * (i >> 4)) & 1)) nan_groups |= bad[i];
     }
-    // out = O / sum; swap_bad [rows of the CTA]
-    __device__ __forceinline__ void finish(const PromptArgs& a, const Task& w, int* swap_bad)
+    // what both threads of the row know; swap_bad [rows of the CTA]
+    __device__ __forceinline__ float total(int* swap_bad)
     {
         const float2 sums = unpair(sum2);
         float sum = sums.x + sums.y;
@@ -558,6 +586,30 @@ struct Row {
         }
         meet(barrier, 64);
         nan_groups = swap_bad[slot];
+        return sum;
+    }
+    // the part's reference, sum and O for the cluster's CTAs to join: o [rows][part_pitch]
+    __device__ __forceinline__ void leave(float* o, int* swap_bad)
+    {
+        const float sum = total(swap_bad);
+        if (!half) {
+            swap[slot] = ref;
+            swap[swap_rows + slot] = sum;
+        }
+        float* to = o + slot * part_pitch(D) + half * (D / 64) * 40;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(at_o + 32 * c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + 40 * c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+    }
+    // out = O / sum
+    __device__ __forceinline__ void finish(const PromptArgs& a, const Task& w, int* swap_bad)
+    {
+        const float sum = total(swap_bad);
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const long long f = w.row0 + slot;
         __half* to = a.out + ((long long)w.b * a.seq + (int)(f / a.share)) * a.heads * D + (w.kvh * a.share + (int)(f % a.share)) * D;
@@ -602,6 +654,64 @@ struct SingleSmem {
     int swap_bad[kRows];
 };
 
+__device__ __forceinline__ void cluster_meet()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(const void* here, int rank)
+{
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(here)), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ float load_there(uint32_t at)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+// The parts of a row tile become its output, each CTA an equal number of rows: by all threads of the CTAs that have parts.
+// sum_r 2^(ref_r - M) O_r / sum_r 2^(ref_r - M) sum_r, M the largest reference.
+template <class F, int D, class S>
+__device__ __forceinline__ void join_parts(const PromptArgs& a, const Task& w, S& sm, int tid)
+{
+    constexpr int J = F::J, kWords = D / 4, kAtOnce = kGroup / kWords;
+    static_assert(kRows * part_pitch(D) * sizeof(float) <= sizeof(sm.q) + sizeof(sm.k) + sizeof(sm.v), "O fits the operands");
+    cluster_meet();
+    if (tid < kGroup) {
+        const int used = (int)min(w.rows - w.row0, (long long)kRows), each = (used + w.parts - 1) / w.parts, end = min(used, (w.rank + 1) * each);
+        // word `tid % kWords` of the cache's order: four dims, in columns 8 apart
+        const int word = tid % kWords, at_col = 40 * (word / 8) + word % 8, dim = 32 * (word % J) + 4 * (word / J);
+        for (int row = w.rank * each + tid / kWords; row < end; row += kAtOnce) {
+            float refs[kMostRanks], sums[kMostRanks], top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            int bad = 0;
+#pragma unroll
+            for (int p = 0; p < kMostRanks; ++p)
+                if (p < w.parts) {
+                    refs[p] = load_there(in_cta(&sm.swap[row], p));
+                    sums[p] = load_there(in_cta(&sm.swap[kRows + row], p));
+                    bad |= __float_as_int(load_there(in_cta(&sm.swap_bad[row], p)));
+                    top = fmaxf(top, refs[p]);
+                }
+#pragma unroll
+            for (int p = 0; p < kMostRanks; ++p)
+                if (p < w.parts) {
+                    const float weight = refs[p] == -INFINITY ? 0.f : ex2(refs[p] - top);        // (of nothing seen; NaN scores still reach the sum)
+                    sum = fmaf(weight, sums[p], sum);
+                    const uint32_t o = in_cta(reinterpret_cast<const float*>(sm.q) + row * part_pitch(D) + at_col, p);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) v[n] = fmaf(weight, load_there(o + 32 * n), v[n]);
+                }
+            const float mul = bad >> (dim * F::NG / D) & 1 ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : 1.f / sum;
+            const long long f = w.row0 + row;
+            *reinterpret_cast<uint2*>(a.out + ((long long)w.b * a.seq + (int)(f / a.share)) * a.heads * D + (w.kvh * a.share + (int)(f % a.share)) * D + dim) =
+                make_uint2(h2_bits(__floats2half2_rn(v[0] * mul, v[1] * mul)), h2_bits(__floats2half2_rn(v[2] * mul, v[3] * mul)));
+        }
+    }
+    cluster_meet();                                                                              // (nobody leaves while its part is read)
+}
+
 template <class F, int D>
 __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs a)
 {
@@ -612,7 +722,8 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
     S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Task w;
-    if (!w.take(a, 1)) return;
+    if (!w.take<true>(a, 1)) return;
+    if (w.rank >= w.parts) return;                // (a cluster's barrier waits for the threads that have not left)
     if (warp == 8) {
         tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
         tmem_relinquish();
@@ -628,28 +739,29 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
     mbar_fence_init();
     for (int i = tid; i < 4 * kTokens; i += kGroup + 32) sm.marks.bad[0][i] = 0;
     if (tid < 4 * 8) sm.marks.any[0][tid] = 0;
-    Lookup<F> lookup(a, w, warp);
+    Lookup<F> lookup(a, w, warp, w.from);
     __syncthreads();
     const uint32_t tmem = sm.tmem, s_bar = smem_u32(&sm.s_done), pv_bar = smem_u32(&sm.pv_done), k_bar = smem_u32(&sm.k_ready),
                    v_bar = smem_u32(&sm.v_ready), p_bar = smem_u32(&sm.p_ready);
     bool ok = true;
-    auto wait = [&](uint32_t bar, int step) { ok = ok && mbar_wait(bar, step & 1, &sm.abort_flag, kWaitNs); };
+    auto wait = [&](uint32_t bar, int step) { ok = ok && mbar_wait(bar, (step - w.from) & 1, &sm.abort_flag, kWaitNs); };
 
     if (warp == 8) {
         // ---- the products.  P stands where S stood: S of a step is issued when P V of the step before is over
         const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q)), k_desc = smem_desc_sw128(smem_u32(sm.k)), v_desc = smem_desc_sw128(smem_u32(sm.v));
-        for (int step = 0; step < w.steps; ++step) {
+        for (int step = w.from; step < w.to; ++step) {
             wait(k_bar, step);
-            if (step > 0) wait(pv_bar, step - 1);
+            if (step > w.from) wait(pv_bar, step - 1);
             issue_s<D>(tmem, q_desc, k_desc, s_bar);
             wait(v_bar, step);
             wait(p_bar, step);
-            issue_pv<D>(tmem, v_desc, step == 0, pv_bar);
+            issue_pv<D>(tmem, v_desc, step == w.from, pv_bar);
         }
-        wait(pv_bar, w.steps - 1);
+        wait(pv_bar, w.to - 1);
         if (!ok && lane == 0) atomicExch(a.error, 1);
         __syncthreads();                                                                         // the workers have read O
         tmem_dealloc(tmem, kTmemCols);
+        if (w.parts > 1) join_parts<F, D>(a, w, sm, tid);
         return;
     }
 
@@ -674,34 +786,36 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
         written(k_bar, lane);
         load_codes<F, D>(codes, tile, true, lane, a.c.pool);
     };
-    fetch(0);
+    fetch(w.from);
     put_queries<D>(a, w, sm.q, w.row0, tid);
     unpack_keys();
     Row<F, D> row(a, w, sm.swap, kRows, 0, warp, lane, tmem);
-    for (int step = 0; step < w.steps; ++step) {
+    for (int step = w.from; step < w.to; ++step) {
         copies_landed();
         __syncwarp();
         put_values_of<F, D>(sm.marks, sm.v, codes, w, step, warp, lane);                         // (P V of the step before is over)
         written(v_bar, lane);
-        if (step + 1 < w.steps) fetch(step + 1);
+        if (step + 1 < w.to) fetch(step + 1);
         wait(s_bar, step);
         tc_fence_after_sync();
-        row.softmax(step, sm.marks.pages(step));
+        row.softmax(step, step == w.from, sm.marks.pages(step));
         written(p_bar, lane);
-        if (step + 1 < w.steps) {
+        if (step + 1 < w.to) {
             unpack_keys();                                                                       // (S of this step is over)
             wait(pv_bar, step);
             tc_fence_after_sync();
             row.mind(sm.marks, step);
         }
     }
-    wait(pv_bar, w.steps - 1);
+    wait(pv_bar, w.to - 1);
     tc_fence_after_sync();
     if (!ok && lane == 0) atomicExch(a.error, 1);
-    row.mind(sm.marks, w.steps - 1);
-    row.finish(a, w, sm.swap_bad);
+    row.mind(sm.marks, w.to - 1);
+    if (w.parts == 1) row.finish(a, w, sm.swap_bad);
+    else row.leave(reinterpret_cast<float*>(sm.q), sm.swap_bad);
     tc_fence_before_sync();
     __syncthreads();
+    if (w.parts > 1) join_parts<F, D>(a, w, sm, tid);
 }
 
 // ---- two row tiles that take turns ---------------------------------------------------------------------------------------------------
@@ -729,7 +843,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
     S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Task w;
-    if (!w.take(a, 2)) return;
+    if (!w.take<false>(a, 2)) return;
     if (warp == 16) {
         tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
         tmem_relinquish();
@@ -749,7 +863,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
     for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 128) sm.marks.bad[0][i] = 0;
     if (threadIdx.x < 4 * 8) sm.marks.any[0][threadIdx.x] = 0;
     const int mine = warp >> 3, tid = threadIdx.x & (kGroup - 1), gwarp = warp & 7;              // the worker's row tile, its place in the group
-    Lookup<F> lookup(a, w, gwarp);
+    Lookup<F> lookup(a, w, gwarp, 0);
     __syncthreads();
     const uint32_t tmem = sm.tmem;
     bool ok = true;
@@ -827,7 +941,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
         wait(sm.s_done[mine], step);
         tc_fence_after_sync();
         if (step > 0) row.mind(sm.marks, step - 1);
-        row.softmax(step, sm.marks.pages(step));
+        row.softmax(step, step == 0, sm.marks.pages(step));
         // the first group unpacks afterwards: the values of the next step, whose buffer P V of the step before has left.  (Waited for before
         // this step's P is announced: behind it the barrier could be two phases on.)
         if (mine == 0 && step > 0) wait(sm.pv_done[1], step - 1);
@@ -844,7 +958,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
 }
 
 template <class K>
-int launch_prompt_as(K kernel, int (&configured)[64], int smem, int tiles, int threads, PromptArgs& a, long long rows, int batch, cudaStream_t st)
+int launch_prompt_as(K kernel, int (&configured)[64], int smem, int threads, const PromptArgs& a, cudaStream_t st)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -854,30 +968,52 @@ int launch_prompt_as(K kernel, int (&configured)[64], int smem, int tiles, int t
         if (e != cudaSuccess) return record_cuda_error(e);
         if (dev < 64) configured[dev] = 1;
     }
-    a.blocks = (int)((rows + tiles * kRows - 1) / (tiles * kRows));
-    kernel<<<dim3(a.blocks, a.c.kv_heads, batch), threads, smem, st>>>(a);
+    cudaLaunchAttribute cluster[1];
+    cluster[0].id = cudaLaunchAttributeClusterDimension;
+    cluster[0].val.clusterDim.x = a.ranks;
+    cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.blocks * a.ranks, a.c.kv_heads, a.batch);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = cluster;
+    cfg.numAttrs = a.ranks > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return record_cuda_error(e); }
     count_launch();
-    e = cudaGetLastError();
-    return e == cudaSuccess ? W4A16_OK : record_cuda_error(e);
+    return W4A16_OK;
 }
 
+// Two row tiles a CTA (128 dims; at 64 a step of K and V costs half as much to unpack, and two CTAs that wait for each other's products did
+// better, 243 / 265 us for 2 x 2048 queries behind 1000 tokens) as soon as there are more row tiles than SMs: for 32 heads on 8, 800 queries
+// behind 4096 tokens take 127 us so and 172 one by one, 640 take 122 and 159; with 512 every row tile has an SM, and two CTAs that share its
+// steps: 122 and 95.  One by one, clusters share row tiles as long as two CTAs an SM hold all of them - an idle CTA keeps its place until its
+// cluster is done: 32 x 8 queries behind 1030 tokens took 90 us with two to a cluster, 48 with none; where they fit, 8 queries behind 8000
+// tokens take 35 us and 193 without.
 template <class F, int D>
-int launch_prompt(PromptArgs& a, long long rows, int batch, cudaStream_t st)
+int launch_prompt(PromptArgs& a, long long rows, cudaStream_t st)
 {
-    // (at 64 dims a step of K and V costs half as much, and two CTAs that wait for each other's products do better: 243 / 265 us for
-    // 2 x 2048 queries behind 1000 tokens, 32 heads on 8, before the row tiles took turns)
+    const int sms = device_sm_count();
+    const long long tiles = (rows + kRows - 1) / kRows, all = tiles * a.c.kv_heads * a.batch;
+    a.ranks = 1;
     if constexpr (D == 128) {
-        if (rows > kRows) {
+        if (rows > kRows && all > sms) {
             using S = PairSmem<D, F::kBytes / 2>;
             static_assert(sizeof(S) + 1024 <= 232448, "fits the SM");
             static int configured[64] = {0};
-            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, 2, 2 * kGroup + 128, a, rows, batch, st);
+            a.blocks = (int)((tiles + 1) / 2);
+            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, 2 * kGroup + 128, a, st);
         }
     }
     using S = SingleSmem<D, F::kBytes / 2>;
     static_assert(sizeof(S) + 1024 <= 115712, "two fit the SM");
     static int configured[64] = {0};
-    return launch_prompt_as(single_kernel<F, D>, configured, (int)sizeof(S) + 1024, 1, kGroup + 32, a, rows, batch, st);
+    a.slots = 2 * sms;
+    a.blocks = (int)tiles;
+    const long long steps = ((long long)a.c.width << a.c.page_shift) / kTokens;
+    while (a.ranks < kMostRanks && 2 * a.ranks * kLeastSteps <= steps && 2 * a.ranks * all <= a.slots) a.ranks *= 2;
+    return launch_prompt_as(single_kernel<F, D>, configured, (int)sizeof(S) + 1024, kGroup + 32, a, st);
 }
 
 }  // namespace
@@ -908,13 +1044,13 @@ extern "C" int w4a16_kv4_attention(const void* qkv, const void* pool, const void
     if (batch == 0 || seq == 0) return W4A16_OK;
     a.qkv = (const __half*)qkv; a.out = (__half*)out; a.pos = (const int*)pos; a.counts = (const int*)counts;
     a.cos = (const __half*)rope_cos; a.sin = (const __half*)rope_sin;
-    a.seq = seq; a.heads = heads; a.rope_rows = rope_rows; a.stride = qkv_stride;
+    a.batch = batch; a.seq = seq; a.heads = heads; a.rope_rows = rope_rows; a.stride = qkv_stride;
     a.page_bytes = (long long)kv_heads * (page_size / kTile) * tile_bytes(head_dim, group);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.error = device_error_word();
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        return launch_prompt<F, F::NW * 8>(a, rows, batch, (cudaStream_t)stream);
+        return launch_prompt<F, F::NW * 8>(a, rows, (cudaStream_t)stream);
     });
 }

@@ -400,6 +400,87 @@ def test_chunk_attention_long(heads, kv, S, ctx, counts):
         assert not out[b, n:].any()
 
 
+def _chunk_against_torch(heads, kv, D, G, P, S, ctx, counts=None, spoil=(), hidden=()):
+    """kv4_attention of S queries behind ctx[b] tokens (negative: no sequence) against torch in float64 on what the cache reads back to.  spoil: (row,
+    token, kv head, group, 'k' or 'v') of the cache that are made not finite; hidden: (row, page of the row) whose table entry is none of the pool."""
+    import quant
+    B = len(ctx)
+    g = torch.Generator(device="cuda").manual_seed(S + sum(ctx))
+    width = (max(ctx) + S) // P + 3
+    pool = quant.kv4_pool(1, B * width, kv, D, P, G)
+    table = torch.randperm(B * width, device="cuda", generator=g).int().view(B, -1)
+    n = [0 if c < 0 else c + (S if counts is None else counts[b]) for b, c in enumerate(ctx)]
+    x = torch.randn(B, max(n), (heads + 2 * kv) * D, device="cuda", generator=g).half()
+    for b, t, h, gr, what in spoil:
+        x[b, t, (heads + (kv if what == "v" else 0) + h) * D + gr * G + 1] = float("inf")
+    zero = torch.zeros(B, dtype=torch.int32, device="cuda")
+    total = torch.tensor(n, dtype=torch.int32, device="cuda")
+    quant.kv4_append(x, pool[0], table, zero, heads, counts=total)
+    k, v = quant.kv4_read(pool[0], table, zero, max(n), counts=total)
+    for b, p in hidden:
+        table[b, p] = B * width + 5
+    pos = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    q = torch.zeros(B, S, heads * D, dtype=torch.float16, device="cuda")
+    for b, c in enumerate(ctx):
+        if c >= 0:
+            q[b, :n[b] - c] = x[b, c:n[b], :heads * D]
+    cnt = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda")
+    out = quant.kv4_attention(q, pool[0], table, pos, heads, counts=cnt).view(B, S, heads, D)
+    for b, c in enumerate(ctx):
+        m = n[b] - max(c, 0)
+        assert not out[b, m:].any()
+        if m <= 0:
+            continue
+        qq = q[b, :m].view(m, heads, D).transpose(0, 1).double()
+        kk, vv = (t[b, :, :n[b]].double().repeat_interleave(heads // kv, 0) for t in (k, v))
+        sees = torch.arange(n[b], device="cuda") <= torch.arange(c, n[b], device="cuda").unsqueeze(1)
+        for hb, p in hidden:
+            if hb == b:
+                sees[:, p * P:(p + 1) * P] = False
+        bad_k = (~kk.isfinite()).any(-1).unsqueeze(1) & sees                    # [heads, 1 or m, tokens]
+        bad_v = (sees.double() @ (~vv.isfinite()).double()) > 0                 # [heads, m, D]
+        want_nan = (bad_v | bad_k.any(-1, keepdim=True)).transpose(0, 1)
+        kk, vv = kk.nan_to_num(0, 0, 0), vv.nan_to_num(0, 0, 0)
+        sc = (qq @ kk.transpose(1, 2)) * D ** -0.5
+        sc.masked_fill_(~sees, -float("inf"))
+        ref = (torch.softmax(sc, -1) @ vv).transpose(0, 1)
+        got = out[b, :m].double()
+        assert torch.equal(got.isnan(), want_nan)
+        got, ref = got.masked_fill(want_nan, 0), ref.masked_fill(want_nan, 0)
+        # as at the head of this file; keys and values as the kernel rounds them, read back
+        X = float((qq.abs() @ kk.abs().transpose(1, 2)).max()) * D ** -0.5
+        tol = float(vv.abs().max()) * (2 * X * (D * 2.0 ** -23 + 2.0 ** -11) + 4 * 2.0 ** -11 + n[b] * 2.0 ** -24) + 2.0 ** -11 * ref.abs()
+        assert ((got - ref).abs() <= tol).all(), float((got - ref).abs().max())
+        assert float((got - ref).norm()) <= 2e-3 * float(ref.norm())            # and far closer on average: rounding errors of both signs
+
+
+@pytest.mark.parametrize("D,G", kv4.formats())
+@pytest.mark.parametrize("heads,kv,S,ctx,counts", [
+    (4, 4, 3, [1500], None), (8, 1, 20, [2100, 40, -1, 700], [20, 5, 0, 1]), (3, 1, 2, [511, 512, 513], None), (6, 2, 50, [0, 1100], None),
+])
+def test_chunk_attention_of_few_rows_over_many_tokens(D, G, heads, kv, S, ctx, counts):
+    """The steps of a row tile are shared between CTAs, as many as its length asks for."""
+    _chunk_against_torch(heads, kv, D, G, 64, S, ctx, counts)
+
+
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("ctx,counts", [([0, 300, 129], None), ([127, -1, 1000], [1100, 0, 250])])
+def test_chunk_attention_of_many_rows(G, ctx, counts):
+    """Two row tiles a CTA, whole and partly filled ones."""
+    _chunk_against_torch(10, 2, 128, G, 32, 1100, ctx, counts)
+
+
+@pytest.mark.parametrize("heads,kv,S,ctx", [(4, 2, 5, [1300, 900]), (10, 2, 1100, [300, 0, 140])])
+def test_chunk_attention_bad_values_and_pages_far_apart(heads, kv, S, ctx):
+    """Values and keys that are not finite and pages that are none of the pool, in several steps of the same row; the rest stays as it is."""
+    n = [c + S for c in ctx]
+    spoil = [(0, 5, 0, 1, "v"), (0, 133, 1, 0, "v"), (0, n[0] - 2, 0, 0, "v"), (0, n[0] - 3, 1, 1, "k"), (1, 700, 1, 1, "v"), (1, 701, 1, 1, "v")]
+    _chunk_against_torch(heads, kv, 128, 64, 32, S, ctx, spoil=spoil)
+    assert _take_error() == 0
+    _chunk_against_torch(heads, kv, 128, 64, 32, S, ctx, spoil=spoil[:1], hidden=[(0, 1), (0, 8), (1, 20)])
+    assert _take_error() == 4
+
+
 def test_chunk_attention_takes_queries_alone():
     """Rows of heads * head_dim elements: the queries without keys and values behind them."""
     import quant
