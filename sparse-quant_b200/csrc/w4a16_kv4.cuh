@@ -68,10 +68,49 @@ struct Cache {
     }
 };
 
+// two fp32 numbers in a register pair, for the instructions that take two at once
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_of(__half2 h)
+{
+    const float2 f = __half22float2(h);
+    return pair(f.x, f.y);
+}
+
 // Eight dims of a row (fp16, packed) from a quantisation group spread over `lanes` adjacent lanes: (s, m) of the group and the eight
-// codes.  Minimum and maximum travel as one pair (lo, -hi).  A code is d = x - m over s rounded to the nearest integer, ties to even:
-// d times the rounded reciprocal, rounded by adding 1.5 2^23 in the same operation, is right except next to the half-way points, where
-// the remainder d - n s (exact: it has few bits) tells.  Eight IEEE divisions and conversions took 60 % of the append kernel's time.
+// codes.  Minimum and maximum travel as one pair (lo, -hi).  A code is d = x - m over s rounded to the nearest integer, ties to even.  d times
+// an approximate reciprocal is within 15.5 (2^-23 + 2^-23) < 2^-18 of the quotient, so that rounding it (by adding 1.5 2^23 in the same
+// operation) is right unless it falls within 2^-16 of a half-way point; there the remainder d - n s (exact: it has few bits) tells.  (A code
+// above 15 can only come from a step below fp16's normal numbers, whose own rounding is coarse: those go the same way.)  A division a value,
+// in single precision instructions for one number, took more than twice as long.
 __device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half2& par)
 {
     const __half2* x = reinterpret_cast<const __half2*>(&x8);
@@ -86,31 +125,39 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half
     const float s = __half2float(sh);
     if (!(s > 0.f)) return 0;                                                   // all values m, or not finite
     constexpr float kMagic = 12582912.f;                                        // 1.5 * 2^23: an integer's last bits are the float's
-    const float r = __frcp_rn(s);
-    float d[8], t[8];
-    bool near = false;
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+    const uint64_t r2 = pair(r, r), lo_2 = pair(-lo, -lo), magic2 = pair(kMagic, kMagic), minus2 = pair(-kMagic, -kMagic), neg2 = pair(-1.f, -1.f);
+    uint64_t d[4], t[4];
+    float off = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float2 f = __half22float2(x[e]);
-        d[2 * e] = f.x - lo;
-        d[2 * e + 1] = f.y - lo;
+        d[e] = add2(pair_of(x[e]), lo_2);
+        t[e] = fma2(d[e], r2, magic2);
+        const float2 f = unpair(fma2(d[e], r2, mul2(add2(t[e], minus2), neg2)));
+        off = fmaxf(off, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
+    if (off > 0.5f - 0x1p-16f || s < 0x1p-14f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        t[i] = fminf(fmaf(d[i], r, kMagic), kMagic + 15.f);
-        near |= 2.f * fabsf(fmaf(kMagic - t[i], s, d[i])) >= s;
-    }
-    if (near) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float rem = fmaf(kMagic - t[i], s, d[i]), two = 2.f * fabsf(rem);
-            if (two > s || (two == s && (__float_as_int(t[i]) & 1))) t[i] += rem > 0.f ? 1.f : -1.f;
-            t[i] = fminf(t[i], kMagic + 15.f);
+        for (int e = 0; e < 4; ++e) {
+            float2 u = unpair(t[e]), v = unpair(d[e]);
+            auto settle = [&](float& n, float x) {
+                n = fminf(n, kMagic + 15.f);
+                const float rem = fmaf(kMagic - n, s, x), two = 2.f * fabsf(rem);
+                if (two > s || (two == s && (__float_as_int(n) & 1))) n += rem > 0.f ? 1.f : -1.f;
+                n = fminf(n, kMagic + 15.f);
+            };
+            settle(u.x, v.x);
+            settle(u.y, v.y);
+            t[e] = pair(u.x, u.y);
         }
     }
     uint32_t word = 0;                                                          // (modulo 2^32: the float's other bits come off at the end)
 #pragma unroll
-    for (int i = 7; i >= 0; --i) word = word * 16u + __float_as_uint(t[i]);
+    for (int e = 3; e >= 0; --e) {
+        const float2 n = unpair(t[e]);
+        word = (word * 16u + __float_as_uint(n.y)) * 16u + __float_as_uint(n.x);
+    }
     return word - 0x4b400000u * 0x11111111u;
 }
 
@@ -126,20 +173,21 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
 }
 
 // A word (8 dims) of a head row with the rotary embedding ("rotate half"), rounded to fp16 as the fp16 cache holds keys; fp32 products
-// and sum, each rounded.  y: the word half a row away; sign: -1 in the row's first half.
-__device__ __forceinline__ uint4 rotate(const uint4& x8, const uint4& y8, const uint4& cos8, const uint4& sin8, float sign)
+// and sum, each rounded.  y: the word half a row away, which comes negative in
+// the row's first half.
+__device__ __forceinline__ uint4 rotate(const uint4& x8, const uint4& y8, const uint4& cos8, const uint4& sin8, bool first)
 {
     uint4 out;
-    float x[8], y[8], c[8], s[8];
-    unpack8(x8, x);
-    unpack8(y8, y);
-    unpack8(cos8, c);
-    unpack8(sin8, s);
+    const uint32_t sign = first ? 0x80008000u : 0u;
+    const uint32_t x[4] = {x8.x, x8.y, x8.z, x8.w}, y[4] = {y8.x ^ sign, y8.y ^ sign, y8.z ^ sign, y8.w ^ sign};
+    const __half2 *c = reinterpret_cast<const __half2*>(&cos8), *s = reinterpret_cast<const __half2*>(&sin8);
     __half2* o = reinterpret_cast<__half2*>(&out);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        o[e] = __floats2half2_rn(__fadd_rn(__fmul_rn(x[2 * e], c[2 * e]), __fmul_rn(sign * y[2 * e], s[2 * e])),
-                                 __fadd_rn(__fmul_rn(x[2 * e + 1], c[2 * e + 1]), __fmul_rn(sign * y[2 * e + 1], s[2 * e + 1])));
+    for (int e = 0; e < 4; ++e) {
+        const __half2 xe = *reinterpret_cast<const __half2*>(&x[e]), ye = *reinterpret_cast<const __half2*>(&y[e]);
+        const float2 f = unpair(add2(mul2(pair_of(xe), pair_of(c[e])), mul2(pair_of(ye), pair_of(s[e]))));
+        o[e] = __floats2half2_rn(f.x, f.y);
+    }
     return out;
 }
 // Word w (dims 8w .. 8w+7) of a head row at `src`, rotated for position t where there are tables.
@@ -149,7 +197,7 @@ __device__ __forceinline__ uint4 load_rotated(const __half* src, int w, const __
     const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * w);
     if (!cos) return x;
     return rotate(x, *reinterpret_cast<const uint4*>(src + 8 * (w ^ (D / 16))), *reinterpret_cast<const uint4*>(cos + (size_t)t * D + 8 * w),
-                  *reinterpret_cast<const uint4*>(sin + (size_t)t * D + 8 * w), w < D / 16 ? -1.f : 1.f);
+                  *reinterpret_cast<const uint4*>(sin + (size_t)t * D + 8 * w), w < D / 16);
 }
 template <int D>
 __device__ __forceinline__ void load_rotated(const __half* src, int w, const __half* cos, const __half* sin, int t, float (&x)[8])

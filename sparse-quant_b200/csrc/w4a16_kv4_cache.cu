@@ -33,7 +33,6 @@ struct AppendArgs {
     int* error;
     int seq, rope_rows;
     int key_at, val_at;           // first element of the keys and of the values in a token's row
-    int runs;                     // blocks of a (batch row, head)
     long long stride;
 };
 
@@ -54,7 +53,7 @@ template <class F, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
 {
     using B = Block<F, D>;
-    const int run = blockIdx.x % a.runs, bh = blockIdx.x / a.runs, head = bh % a.c.kv_heads, b = bh / a.c.kv_heads;
+    const int run = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
     const int p = a.pos[b], count = p < 0 ? 0 : min(a.counts ? a.counts[b] : a.seq, a.seq);
     const int room = min(a.c.capacity(), a.cos ? a.rope_rows : 0x7fffffff);
     const int s_first = run * kTile - (p & 15);                                 // of the tile's first position
@@ -63,22 +62,26 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
         if (threadIdx.x == 0) atomicExch(a.error, kErrPosition);
         return;
     }
+    const int w = threadIdx.x % F::NW, r = B::token(), s = s_first + r;
+    const bool mine = s >= 0 && s < count && s < room - p;
+    if (s >= room - p && s < count) atomicExch(a.error, kErrPosition);
+    // (the words are on their way while the page is looked up)
+    uint4 x[B::kEach], y, cs, sn;
+    const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + head * D + 8 * w;
+    const bool rotated = a.cos && mine && !B::value(0);
+#pragma unroll
+    for (int k = 0; k < B::kEach; ++k) x[k] = mine ? *reinterpret_cast<const uint4*>(row + (B::value(k) ? a.val_at : a.key_at)) : make_uint4(0, 0, 0, 0);
+    if (rotated) {
+        y = *reinterpret_cast<const uint4*>(row + a.key_at + (w < D / 16 ? D / 2 : -D / 2));
+        cs = *reinterpret_cast<const uint4*>(a.cos + (size_t)(p + s) * D + 8 * w);
+        sn = *reinterpret_cast<const uint4*>(a.sin + (size_t)(p + s) * D + 8 * w);
+    }
     unsigned char* tile = a.c.tile(b, head, p + max(s_first, 0), F::kBytes);
     if (!tile) {
         if (threadIdx.x == 0) atomicExch(a.error, kErrPage);
         return;
     }
-    const int w = threadIdx.x % F::NW, r = B::token(), s = s_first + r;
-    const bool mine = s >= 0 && s < count && s < room - p;
-    if (s >= room - p && s < count) atomicExch(a.error, kErrPosition);
-    uint4 x[B::kEach];
-    const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + head * D;
-#pragma unroll
-    for (int k = 0; k < B::kEach; ++k) {
-        const bool value = B::value(k);
-        x[k] = make_uint4(0, 0, 0, 0);
-        if (mine) x[k] = load_rotated<D>(row + (value ? a.val_at : a.key_at), w, value ? nullptr : a.cos, a.sin, p + s);
-    }
+    if (rotated) x[0] = rotate(x[0], y, cs, sn, w < D / 16);
     constexpr int kLanes = D / F::NG / 8;                                       // lanes of a group
 #pragma unroll
     for (int k = 0; k < B::kEach; ++k) {
@@ -102,7 +105,7 @@ struct ReadArgs {
     __half* k;
     __half* v;
     int* error;
-    int seq, runs;
+    int seq;
 };
 
 // The same blocks; out [batch][kv heads][seq][D], zeros where a row has no such token.  (A row without a sequence is walked as if it stood
@@ -111,7 +114,7 @@ template <class F, int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a)
 {
     using B = Block<F, D>;
-    const int run = blockIdx.x % a.runs, bh = blockIdx.x / a.runs, head = bh % a.c.kv_heads, b = bh / a.c.kv_heads;
+    const int run = blockIdx.x, head = blockIdx.y, b = blockIdx.z, bh = b * a.c.kv_heads + head;
     const int p = max(a.pos[b], 0), count = a.pos[b] < 0 ? 0 : min(a.counts ? a.counts[b] : a.seq, a.seq), room = a.c.capacity();
     const int s_first = run * kTile - (p & 15);
     if (s_first >= a.seq) return;
@@ -493,9 +496,8 @@ extern "C" int w4a16_kv4_append(const void* qkv, void* pool, const void* table, 
     if (((uintptr_t)qkv | (uintptr_t)rope_cos | (uintptr_t)rope_sin) & 15 || ((uintptr_t)pos | (uintptr_t)counts) & 3) return W4A16_ERR_MISALIGNED;
     if ((heads + 2ll * kv_heads) * head_dim >= (1ll << 30) || seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
     if (batch == 0 || seq == 0) return W4A16_OK;
-    a.runs = runs_of(seq);
-    const long long blocks = (long long)batch * kv_heads * a.runs;
-    if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
+    if (batch > 65535 || kv_heads > 65535) return W4A16_ERR_TOO_LARGE;
+    const dim3 blocks(runs_of(seq), kv_heads, batch);
     a.qkv = (const __half*)qkv; a.pos = (const int*)pos; a.counts = (const int*)counts;
     a.cos = (const __half*)rope_cos; a.sin = (const __half*)rope_sin;
     a.seq = seq; a.rope_rows = rope_rows; a.stride = qkv_stride;
@@ -504,7 +506,7 @@ extern "C" int w4a16_kv4_append(const void* qkv, void* pool, const void* table, 
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        append_kernel<F, F::NW * 8><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+        append_kernel<F, F::NW * 8><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
         return last_launch();
     });
 }
@@ -520,15 +522,14 @@ extern "C" int w4a16_kv4_read(const void* pool, const void* table, const void* p
     if (((uintptr_t)k | (uintptr_t)v) & 15 || ((uintptr_t)pos | (uintptr_t)counts) & 3) return W4A16_ERR_MISALIGNED;
     if (seq >= (1 << 30)) return W4A16_ERR_TOO_LARGE;
     if (batch == 0 || seq == 0) return W4A16_OK;
-    a.runs = runs_of(seq);
-    const long long blocks = (long long)batch * kv_heads * a.runs;
-    if (blocks >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;
+    if (batch > 65535 || kv_heads > 65535) return W4A16_ERR_TOO_LARGE;
+    const dim3 blocks(runs_of(seq), kv_heads, batch);
     a.pos = (const int*)pos; a.counts = (const int*)counts; a.k = (__half*)k; a.v = (__half*)v; a.seq = seq;
     a.error = device_error_word();
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        read_kernel<F, F::NW * 8><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+        read_kernel<F, F::NW * 8><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
         return last_launch();
     });
 }

@@ -67,30 +67,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 // two fp32 operations in one instruction
-__device__ __forceinline__ uint64_t pair(float a, float b)
-{
-    uint64_t p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
-    return p;
-}
-__device__ __forceinline__ float2 unpair(uint64_t p)
-{
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-    return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 h2_of(uint32_t b) { return *reinterpret_cast<const __half2*>(&b); }
 
@@ -408,8 +384,8 @@ __device__ __forceinline__ void put_queries(const PromptArgs& a, const Task& w, 
                 }
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
-                put(r0 + u * kApart, rotate(x[u][0], x[u][1], c[u][0], s[u][0], -1.f), 0);
-                put(r0 + u * kApart, rotate(x[u][1], x[u][0], c[u][1], s[u][1], 1.f), 1);
+                put(r0 + u * kApart, rotate(x[u][0], x[u][1], c[u][0], s[u][0], true), 0);
+                put(r0 + u * kApart, rotate(x[u][1], x[u][0], c[u][1], s[u][1], false), 1);
             }
         } else {
 #pragma unroll
