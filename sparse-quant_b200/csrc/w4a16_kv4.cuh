@@ -105,17 +105,36 @@ __device__ __forceinline__ uint64_t pair_of(__half2 h)
     return pair(f.x, f.y);
 }
 
-// Eight dims of a row (fp16, packed) from a quantisation group spread over `lanes` adjacent lanes: (s, m) of the group and the eight
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 h2_of(uint32_t b) { return *reinterpret_cast<const __half2*>(&b); }
+
+// Codes of a word as half2: dims (0,4), (1,5), (2,6), (3,7).
+__device__ __forceinline__ void codes8(uint32_t w, __half2 (&n)[4])
+{
+    const uint32_t top = w >> 8;
+    const __half2 k1024 = h2_of(0x64006400u), k16th = h2_of(0x2c002c00u), k64 = h2_of(0xd400d400u);   // 1024, 1/16, -64
+    n[0] = __hsub2(h2_of(lop3_and_or(w, 0x000f000fu, 0x64006400u)), k1024);
+    n[1] = __hfma2(h2_of(lop3_and_or(w, 0x00f000f0u, 0x64006400u)), k16th, k64);
+    n[2] = __hsub2(h2_of(lop3_and_or(top, 0x000f000fu, 0x64006400u)), k1024);
+    n[3] = __hfma2(h2_of(lop3_and_or(top, 0x00f000f0u, 0x64006400u)), k16th, k64);
+}
+
+// N words of 8 dims of a row (fp16, packed) from a quantisation group spread over `lanes` adjacent lanes: (s, m) of the group and the words'
 // codes.  Minimum and maximum travel as one pair (lo, -hi).  A code is d = x - m over s rounded to the nearest integer, ties to even.  d times
 // an approximate reciprocal is within 15.5 (2^-23 + 2^-23) < 2^-18 of the quotient, so that rounding it (by adding 1.5 2^23 in the same
 // operation) is right unless it falls within 2^-16 of a half-way point; there the remainder d - n s (exact: it has few bits) tells.  (A code
 // above 15 can only come from a step below fp16's normal numbers, whose own rounding is coarse: those go the same way.)  A division a value,
 // in single precision instructions for one number, took more than twice as long.
-__device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half2& par)
+template <int N>
+__device__ __forceinline__ void quantize(const uint4 (&words)[N], int lanes, __half2& par, uint32_t (&codes)[N])
 {
-    const __half2* x = reinterpret_cast<const __half2*>(&x8);
-    const __half2 lo2 = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
-    const __half2 hi2 = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+    const __half2* x = reinterpret_cast<const __half2*>(words);
+    __half2 lo2 = x[0], hi2 = x[0];
+#pragma unroll
+    for (int e = 1; e < 4 * N; ++e) {
+        lo2 = __hmin2_nan(lo2, x[e]);
+        hi2 = __hmax2_nan(hi2, x[e]);
+    }
     __half2 ends = __halves2half2(__hmin_nan(__low2half(lo2), __high2half(lo2)), __hneg(__hmax_nan(__low2half(hi2), __high2half(hi2))));
     for (int o = 1; o < lanes; o <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, o));
     const float lo = __low2float(ends), hi = -__high2float(ends);
@@ -123,15 +142,17 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half
     const __half sh = finite ? __float2half_rn(__fdiv_rn(hi - lo, 15.f)) : __ushort_as_half(0x7fff);
     par = __halves2half2(sh, __low2half(ends));
     const float s = __half2float(sh);
-    if (!(s > 0.f)) return 0;                                                   // all values m, or not finite
+#pragma unroll
+    for (int k = 0; k < N; ++k) codes[k] = 0;
+    if (!(s > 0.f)) return;                                                     // all values m, or not finite
     constexpr float kMagic = 12582912.f;                                        // 1.5 * 2^23: an integer's last bits are the float's
     float r;
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
     const uint64_t r2 = pair(r, r), lo_2 = pair(-lo, -lo), magic2 = pair(kMagic, kMagic), minus2 = pair(-kMagic, -kMagic), neg2 = pair(-1.f, -1.f);
-    uint64_t d[4], t[4];
+    uint64_t d[4 * N], t[4 * N];
     float off = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4 * N; ++e) {
         d[e] = add2(pair_of(x[e]), lo_2);
         t[e] = fma2(d[e], r2, magic2);
         const float2 f = unpair(fma2(d[e], r2, mul2(add2(t[e], minus2), neg2)));
@@ -139,7 +160,7 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half
     }
     if (off > 0.5f - 0x1p-16f || s < 0x1p-14f) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4 * N; ++e) {
             float2 u = unpair(t[e]), v = unpair(d[e]);
             auto settle = [&](float& n, float x) {
                 n = fminf(n, kMagic + 15.f);
@@ -152,13 +173,15 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& x8, int lanes, __half
             t[e] = pair(u.x, u.y);
         }
     }
-    uint32_t word = 0;                                                          // (modulo 2^32: the float's other bits come off at the end)
 #pragma unroll
-    for (int e = 3; e >= 0; --e) {
-        const float2 n = unpair(t[e]);
-        word = (word * 16u + __float_as_uint(n.y)) * 16u + __float_as_uint(n.x);
+    for (int k = 0; k < N; ++k) {                                               // (modulo 2^32: the floats' other bits come off at the end)
+#pragma unroll
+        for (int e = 3; e >= 0; --e) {
+            const float2 n = unpair(t[4 * k + e]);
+            codes[k] = (codes[k] * 16u + __float_as_uint(n.y)) * 16u + __float_as_uint(n.x);
+        }
+        codes[k] -= 0x4b400000u * 0x11111111u;
     }
-    return word - 0x4b400000u * 0x11111111u;
 }
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])

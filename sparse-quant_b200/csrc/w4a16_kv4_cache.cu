@@ -36,21 +36,23 @@ struct AppendArgs {
     long long stride;
 };
 
-// A block takes one tile: the 16 positions 16 (p/16 + run) .. of one (batch row, head), of which those of the call are written.  D/8
-// adjacent lanes take a row's words of 8 dims; at D = 128 a thread takes a key row's word, then the value row's, at D = 64 half of the
-// warps take keys: no warp has both, since only keys are rotated.  One look at the page table a block.
+// A block takes one tile: the 16 positions 16 (p/16 + run) .. of one (batch row, head), of which those of the call are written.  A thread has
+// two adjacent words (16 dims) of a key or a value row, the first half of the block keys: no warp has both, since only keys are rotated, and
+// what a group costs besides its values (ends, step) is shared by 16 of them - with one word of each a thread, 8 x 2048 tokens took 35 us.
+// One look at the page table a block.
 template <class F, int D>
 struct Block {
-    static constexpr int kEach = D / 64;                                        // rows' words of a thread
-    __device__ static __forceinline__ bool value(int k) { return kEach == 2 ? k == 1 : threadIdx.x >= 128; }
-    __device__ static __forceinline__ int token() { return threadIdx.x / F::NW % kTile; }
+    static constexpr int kPieces = D / 16, kThreads = 2 * kTile * kPieces;      // of a row
+    __device__ static __forceinline__ bool value() { return threadIdx.x >= kThreads / 2; }
+    __device__ static __forceinline__ int token() { return threadIdx.x / kPieces % kTile; }
+    __device__ static __forceinline__ int word() { return 2 * (threadIdx.x % kPieces); }
 };
 int runs_of(int seq) { return (seq + 2 * kTile - 2) / kTile; }                  // tiles that seq positions can touch
 
 // Bound: memory (reads 4 D bytes, writes tile bytes / 16 for a token and head).  8 x 2048 tokens, 8 heads of 128 in groups of 32, rotated:
 // 96 us with a division a value, 64-bit index arithmetic a thread, and keys and values in one warp.
 template <class F, int D>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
+__global__ void __launch_bounds__(Block<F, D>::kThreads) append_kernel(const AppendArgs a)
 {
     using B = Block<F, D>;
     const int run = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
@@ -62,40 +64,49 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
         if (threadIdx.x == 0) atomicExch(a.error, kErrPosition);
         return;
     }
-    const int w = threadIdx.x % F::NW, r = B::token(), s = s_first + r;
-    const bool mine = s >= 0 && s < count && s < room - p;
+    const int w = B::word(), r = B::token(), s = s_first + r;
+    const bool value = B::value(), mine = s >= 0 && s < count && s < room - p;
     if (s >= room - p && s < count) atomicExch(a.error, kErrPosition);
     // (the words are on their way while the page is looked up)
-    uint4 x[B::kEach], y, cs, sn;
-    const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + head * D + 8 * w;
-    const bool rotated = a.cos && mine && !B::value(0);
+    uint4 x[2], y[2], cs[2], sn[2];
+    const __half* row = a.qkv + ((long long)b * a.seq + s) * a.stride + head * D + (value ? a.val_at : a.key_at) + 8 * w;
+    const bool rotated = a.cos && mine && !value;
+    const int other = w < D / 16 ? D / 2 : -D / 2;
+    const size_t at = (size_t)(p + s) * D + 8 * w;
 #pragma unroll
-    for (int k = 0; k < B::kEach; ++k) x[k] = mine ? *reinterpret_cast<const uint4*>(row + (B::value(k) ? a.val_at : a.key_at)) : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < 2; ++k) x[k] = mine ? *reinterpret_cast<const uint4*>(row + 8 * k) : make_uint4(0, 0, 0, 0);
     if (rotated) {
-        y = *reinterpret_cast<const uint4*>(row + a.key_at + (w < D / 16 ? D / 2 : -D / 2));
-        cs = *reinterpret_cast<const uint4*>(a.cos + (size_t)(p + s) * D + 8 * w);
-        sn = *reinterpret_cast<const uint4*>(a.sin + (size_t)(p + s) * D + 8 * w);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            y[k] = *reinterpret_cast<const uint4*>(row + other + 8 * k);
+            cs[k] = *reinterpret_cast<const uint4*>(a.cos + at + 8 * k);
+            sn[k] = *reinterpret_cast<const uint4*>(a.sin + at + 8 * k);
+        }
     }
     unsigned char* tile = a.c.tile(b, head, p + max(s_first, 0), F::kBytes);
     if (!tile) {
         if (threadIdx.x == 0) atomicExch(a.error, kErrPage);
         return;
     }
-    if (rotated) x[0] = rotate(x[0], y, cs, sn, w < D / 16);
-    constexpr int kLanes = D / F::NG / 8;                                       // lanes of a group
+    if (rotated) {
 #pragma unroll
-    for (int k = 0; k < B::kEach; ++k) {
-        __half2 par;
-        const uint32_t word = quantize8(x[k], kLanes, par);                     // (all lanes: shuffles)
-        if (!mine) continue;
-        if (!B::value(k)) {
-            *reinterpret_cast<uint32_t*>(tile + F::key_word(r, w)) = word;
-        } else {
-            *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w)) = (uint16_t)word;
-            *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * w + 1)) = (uint16_t)(word >> 16);
-        }
-        if (w % kLanes == 0) *reinterpret_cast<__half2*>(tile + (B::value(k) ? F::val_par(r, w / kLanes) : F::key_par(r, w / kLanes))) = par;
+        for (int k = 0; k < 2; ++k) x[k] = rotate(x[k], y[k], cs[k], sn[k], w < D / 16);
     }
+    constexpr int kLanes = D / F::NG / 16;                                      // lanes of a group
+    __half2 par;
+    uint32_t codes[2];
+    quantize(x, kLanes, par, codes);                                            // (all lanes: shuffles)
+    if (!mine) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (!value) {
+            *reinterpret_cast<uint32_t*>(tile + F::key_word(r, w + k)) = codes[k];
+        } else {
+            *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * (w + k))) = (uint16_t)codes[k];
+            *reinterpret_cast<uint16_t*>(tile + F::val_half(r, 2 * (w + k) + 1)) = (uint16_t)(codes[k] >> 16);
+        }
+    }
+    if (w % (2 * kLanes) == 0) *reinterpret_cast<__half2*>(tile + (value ? F::val_par(r, w / (2 * kLanes)) : F::key_par(r, w / (2 * kLanes)))) = par;
 }
 
 struct ReadArgs {
@@ -111,7 +122,7 @@ struct ReadArgs {
 // The same blocks; out [batch][kv heads][seq][D], zeros where a row has no such token.  (A row without a sequence is walked as if it stood
 // at position 0.)
 template <class F, int D>
-__global__ void __launch_bounds__(256) read_kernel(const ReadArgs a)
+__global__ void __launch_bounds__(Block<F, D>::kThreads) read_kernel(const ReadArgs a)
 {
     using B = Block<F, D>;
     const int run = blockIdx.x, head = blockIdx.y, b = blockIdx.z, bh = b * a.c.kv_heads + head;
@@ -127,35 +138,32 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a)
             if (!tile && threadIdx.x == 0) atomicExch(a.error, kErrPage);
         }
     }
-    const int w = threadIdx.x % F::NW, r = B::token(), s = s_first + r, g = w * 8 * F::NG / D;
+    const int w = B::word(), r = B::token(), s = s_first + r, g = w * 8 * F::NG / D;
+    const bool value = B::value();
     if (s < 0 || s >= a.seq) return;
     const bool mine = tile && s < count && s < room - p;
     if (tile && s < count && s >= room - p) atomicExch(a.error, kErrPosition);
-    uint32_t word[B::kEach];
-    __half2 par[B::kEach];
+    uint32_t word[2] = {0, 0};
+    __half2 par = h2_of(0);
+    if (mine) {
+        par = *reinterpret_cast<const __half2*>(tile + (value ? F::val_par(r, g) : F::key_par(r, g)));
 #pragma unroll
-    for (int k = 0; k < B::kEach; ++k) {
-        word[k] = 0;
-        par[k] = __half2half2(__ushort_as_half(0));
-        if (!mine) continue;
-        if (!B::value(k)) {
-            word[k] = *reinterpret_cast<const uint32_t*>(tile + F::key_word(r, w));
-            par[k] = *reinterpret_cast<const __half2*>(tile + F::key_par(r, g));
-        } else {
-            word[k] = *reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w)) |
-                      (uint32_t)*reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * w + 1)) << 16;
-            par[k] = *reinterpret_cast<const __half2*>(tile + F::val_par(r, g));
-        }
+        for (int k = 0; k < 2; ++k)
+            word[k] = !value ? *reinterpret_cast<const uint32_t*>(tile + F::key_word(r, w + k))
+                             : *reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * (w + k))) |
+                                   (uint32_t)*reinterpret_cast<const uint16_t*>(tile + F::val_half(r, 2 * (w + k) + 1)) << 16;
     }
+    const __half2 step = __low2half2(par), least = __high2half2(par);
+    __half* to = (value ? a.v : a.k) + ((long long)bh * a.seq + s) * D + 8 * w;
 #pragma unroll
-    for (int k = 0; k < B::kEach; ++k) {
-        const float2 f = __half22float2(par[k]);
-        uint4 out;
-        __half2* o = reinterpret_cast<__half2*>(&out);
+    for (int k = 0; k < 2; ++k) {
+        __half2 n[4];                                                           // dims (0,4), (1,5), (2,6), (3,7): m + n s, rounded once
+        codes8(word[k], n);
+        uint32_t h[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            o[e] = __floats2half2_rn(fmaf((float)((word[k] >> (8 * e)) & 15), f.x, f.y), fmaf((float)((word[k] >> (8 * e + 4)) & 15), f.x, f.y));
-        *reinterpret_cast<uint4*>((B::value(k) ? a.v : a.k) + ((long long)bh * a.seq + s) * D + 8 * w) = out;
+        for (int e = 0; e < 4; ++e) h[e] = h2_bits(__hfma2(n[e], step, least));
+        *reinterpret_cast<uint4*>(to + 8 * k) =
+            make_uint4(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410), __byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632));
     }
 }
 
@@ -506,7 +514,7 @@ extern "C" int w4a16_kv4_append(const void* qkv, void* pool, const void* table, 
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        append_kernel<F, F::NW * 8><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
+        append_kernel<F, F::NW * 8><<<blocks, Block<F, F::NW * 8>::kThreads, 0, (cudaStream_t)stream>>>(a);
         return last_launch();
     });
 }
@@ -529,7 +537,7 @@ extern "C" int w4a16_kv4_read(const void* pool, const void* table, const void* p
     if (!a.error) return W4A16_ERR_CUDA;
     return with_format(head_dim, group, [&](auto f) {
         using F = decltype(f);
-        read_kernel<F, F::NW * 8><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
+        read_kernel<F, F::NW * 8><<<blocks, Block<F, F::NW * 8>::kThreads, 0, (cudaStream_t)stream>>>(a);
         return last_launch();
     });
 }

@@ -386,10 +386,12 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                     const bool value = (lane / F::NW) & 1;
                     const int w = lane % F::NW, r = pos & 15;
                     constexpr int kLanes = D / NG / 8;
-                    const uint4 x = load_rotated<D>(a.qkv + b * a.stride + (a.heads + (value ? a.c.kv_heads : 0) + kvh) * D, w,
-                                                    value ? nullptr : a.cos, a.sin, pos);
+                    const uint4 x[1] = {load_rotated<D>(a.qkv + b * a.stride + (a.heads + (value ? a.c.kv_heads : 0) + kvh) * D, w,
+                                                    value ? nullptr : a.cos, a.sin, pos)};
                     __half2 par;
-                    const uint32_t word = quantize8(x, kLanes, par);
+                    uint32_t codes[1];
+                    quantize(x, kLanes, par, codes);
+                    const uint32_t word = codes[0];
                     auto put = [&](unsigned char* to) {
                         if (!value) {
                             *reinterpret_cast<uint32_t*>(to + F::key_word(r, w)) = word;

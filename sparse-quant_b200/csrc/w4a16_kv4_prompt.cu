@@ -67,19 +67,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 // two fp32 operations in one instruction
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-__device__ __forceinline__ __half2 h2_of(uint32_t b) { return *reinterpret_cast<const __half2*>(&b); }
-
-// Codes of a word as half2: dims (0,4), (1,5), (2,6), (3,7).
-__device__ __forceinline__ void codes8(uint32_t w, __half2 (&n)[4])
-{
-    const uint32_t top = w >> 8;
-    const __half2 k1024 = h2_of(0x64006400u), k16th = h2_of(0x2c002c00u), k64 = h2_of(0xd400d400u);   // 1024, 1/16, -64
-    n[0] = __hsub2(h2_of(lop3_and_or(w, 0x000f000fu, 0x64006400u)), k1024);
-    n[1] = __hfma2(h2_of(lop3_and_or(w, 0x00f000f0u, 0x64006400u)), k16th, k64);
-    n[2] = __hsub2(h2_of(lop3_and_or(top, 0x000f000fu, 0x64006400u)), k1024);
-    n[3] = __hfma2(h2_of(lop3_and_or(top, 0x00f000f0u, 0x64006400u)), k16th, k64);
-}
 __device__ __forceinline__ bool finite2(__half2 p) { return (h2_bits(p) & 0x7c00u) != 0x7c00u && (h2_bits(p) & 0x7c000000u) != 0x7c000000u; }
 template <int N>
 __device__ __forceinline__ void load_params(const unsigned char* at, __half2 (&p)[N])
