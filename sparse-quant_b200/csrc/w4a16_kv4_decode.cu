@@ -97,6 +97,12 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 // that one load instruction touches over the shared-memory banks, for keys (two or four rows at a time) and values (every other).
 __device__ __forceinline__ int token_of(int i) { return i ^ ((i >> 2) & 1); }
 
+// a / b of numbers that hardly ever need 64 bits (whose division takes some hundred instructions)
+__device__ __forceinline__ long long quotient(long long a, long long b)
+{
+    return (unsigned long long)a >> 32 || (unsigned long long)b >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
 // Chunks of batch row b, 0 where it has no sequence or a position that cannot be served.
 __device__ __forceinline__ int chunks_of(const DecodeArgs& a, int b)
 {
@@ -233,14 +239,14 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
             if (me - warp >= warps || total == 0) return;                       // the whole CTA
         }
         long long before;
-        const long long from = total * min(me, warps - 1) / warps, to = me < warps ? total * (me + 1) / warps : from;
+        const long long from = quotient(total * min(me, warps - 1), warps), to = me < warps ? quotient(total * (me + 1), warps) : from;
         line.b = rows.row_of(a, from, before);
         line.n = chunks_of(a, line.b);
         const int len = line.n + kStart;
-        line.unit = (int)((from - before) / len);
+        line.unit = (int)quotient(from - before, len);
         line.left = to - from;
         // does the CTA's stretch end in the unit that it starts in?
-        const long long cta_from = total * (me - warp) / warps, cta_to = total * min(me - warp + kWarps, warps) / warps;
+        const long long cta_from = quotient(total * (me - warp), warps), cta_to = quotient(total * min(me - warp + kWarps, warps), warps);
         const long long unit_at = before + (long long)line.unit * len;
         together = cta_from >= unit_at && cta_to <= unit_at + len;
         together = __syncthreads_and(together);
@@ -648,8 +654,8 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
         const bool starts = line.lo == 0 && line.hi > 0, whole = starts && line.hi == line.n;
         // the warps that a unit starting here is dealt to, this one first: its last chunk stands n - hi behind the segment's end
         auto dealt = [&]() {
-            const long long end = total * (me + 1) / warps - line.left + line.n - line.hi;
-            return make_int4(b, line.unit, (int)((end * warps - 1) / total - me) + 1, 0);
+            const long long end = quotient(total * (me + 1), warps) - line.left + line.n - line.hi;
+            return make_int4(b, line.unit, (int)(quotient(end * warps - 1, total) - me) + 1, 0);
         };
         if (!together) {
             if (line.lo < line.hi) {
@@ -834,16 +840,18 @@ int g_force_ctas = 0;
 
 }  // namespace
 
-// CTAs of a call that share the line, 0 where each takes a whole unit.  The line costs about 8 us more (finding the place, the second
-// launch); a CTA with a unit of its own takes a round of its four warps for every four chunks.  The host knows how long rows can be
-// from the table's width alone.  Measured, by units / by the line: 1 row of 77 tokens 6.3 / 12.9 us, 8 rows of 520 tokens, 32 heads
-// 14 / 20 us, 32 rows of 1030 51 / 50 us, 24 rows of 1 to 6000 tokens, 8 heads of 64 50 / 21 us.
+// CTAs of a call that share the line, 0 where each takes a whole unit.  The line costs 5 to 8 us more (finding the place, the second
+// launch); a CTA with a unit of its own takes a round of its four warps for every four chunks, and a long row alone may keep the call waiting.
+// The host knows how long rows can be from the table's width alone.  Measured, by units / by the line, heads of 128 unless said: 1 row of 77
+// tokens, 32 heads 5.3 / 11.1 us; 1 row, 8 heads of 800 tokens 12.3 / 15.6, of 2000 19 / 16; 16 rows of 2000, 8 heads 20 / 24, of 4000 34 / 32;
+// 64 rows of 2000, 8 heads of 64 29 / 37, of 1 to 2000 18 / 19; 24 rows of 1 to 2000, 32 heads 31 / 24; 24 rows of 1 to 6000, 8 heads of 64 41 / 19.
+// Three CTAs an SM take the line in 40 us for 1 row of 100000 tokens (four 44, two 38), 24 ragged rows up to 32000 in 57 (57, 69).
 int decode_ctas(int batch, int units, int page_size, int width)
 {
     if (g_force_ctas) return g_force_ctas < 0 ? 0 : g_force_ctas;
-    const long long slots = 4ll * device_sm_count(), longest = (long long)width * page_size / kChunk;
-    const long long waves = ((long long)batch * units + slots - 1) / slots;
-    return longest * waves <= 40 ? 0 : (int)slots;
+    const long long slots = 4ll * device_sm_count(), longest = (long long)width * page_size / kChunk, all = (long long)batch * units;
+    const long long waves = (all + slots - 1) / slots;
+    return longest * waves <= 40 || (waves == 1 && 5 * all >= slots && longest <= 64) ? 0 : (int)(slots / 4 * 3);
 }
 
 // Query heads of a unit: as many as have columns for all their groups, where that takes no more passes than 8 heads a pass.
