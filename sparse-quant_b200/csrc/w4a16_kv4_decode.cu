@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a, int warps
     constexpr int kDims = D / 4, kSub = 256 / kDims, kFew = 16;
     __shared__ int4 many[8];
     __shared__ float4 num_s[kSub][kDims];
-    __shared__ float top_s[8], den_s[kSub];
+    __shared__ float2 den_s[kSub];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int me = blockIdx.x * 8 + warp;
@@ -791,44 +791,49 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a, int warps
     for (int k = 0; k < 8; ++k) {
         const int4 w = many[k];
         if (w.z == 0) continue;                                                 // (uniform)
-        float m = -INFINITY;
-        for (int i = threadIdx.x; i < w.z; i += 256) m = fmaxf(m, part(w.w, i)[D]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) top_s[warp] = m;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, top_s[i]);
         const int sub = threadIdx.x / kDims, d4 = threadIdx.x % kDims;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-        // (whole groups of 8 parts in flight; their references first, so that parts that hold nothing are not fetched)
+        float l = 0.f, m = -INFINITY;
+        // eight parts in flight, whether they hold anything or not: waiting for their references first took longer than what it saved
         for (int i0 = sub; i0 < w.z; i0 += 8 * kSub) {
             float2 ml[8];
             float4 x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                ml[i] = i0 + i * kSub < w.z ? *reinterpret_cast<const float2*>(part(w.w, i0 + i * kSub) + D) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (ml[i].x != -INFINITY) x[i] = *reinterpret_cast<const float4*>(part(w.w, i0 + i * kSub) + 4 * d4);
+            float top = m;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (ml[i].x == -INFINITY) continue;
-                const float f = ex2(ml[i].x - m);
+                const float* from = part(w.w, min(i0 + i * kSub, w.z - 1));
+                ml[i] = *reinterpret_cast<const float2*>(from + D);
+                x[i] = *reinterpret_cast<const float4*>(from + 4 * d4);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i0 + i * kSub >= w.z) ml[i].x = -INFINITY;
+                top = fmaxf(top, ml[i].x);
+            }
+            const float keep = m == -INFINITY ? 0.f : ex2(m - top);
+            l *= keep;
+            v = make_float4(v.x * keep, v.y * keep, v.z * keep, v.w * keep);
+            m = top;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (ml[i].x == -INFINITY) continue;                             // (what stands there is nobody's)
+                const float f = ex2(ml[i].x - m);                               // (NaN stays)
                 l = fmaf(ml[i].y, f, l);
                 v = make_float4(fmaf(x[i].x, f, v.x), fmaf(x[i].y, f, v.y), fmaf(x[i].z, f, v.z), fmaf(x[i].w, f, v.w));
             }
         }
         num_s[sub][d4] = v;
-        if (d4 == 0) den_s[sub] = l;
+        if (d4 == 0) den_s[sub] = make_float2(m, l);
         __syncthreads();
         if (threadIdx.x < D) {
-            float x = 0.f, den = 0.f;
+            float x = 0.f, den = 0.f, top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kSub; ++i) top = fmaxf(top, den_s[i].x);
 #pragma unroll
             for (int i = 0; i < kSub; ++i) {
-                x += reinterpret_cast<const float*>(num_s[i])[threadIdx.x];
-                den += den_s[i];
+                const float f = den_s[i].x == -INFINITY ? 0.f : ex2(den_s[i].x - top);
+                x = fmaf(reinterpret_cast<const float*>(num_s[i])[threadIdx.x], f, x);
+                den = fmaf(den_s[i].y, f, den);
             }
             out(w)[threadIdx.x] = __float2half_rn(den == 0.f ? 0.f : x / den);
         }
@@ -844,14 +849,15 @@ int g_force_ctas = 0;
 // launch); a CTA with a unit of its own takes a round of its four warps for every four chunks, and a long row alone may keep the call waiting.
 // The host knows how long rows can be from the table's width alone.  Measured, by units / by the line, heads of 128 unless said: 1 row of 77
 // tokens, 32 heads 5.3 / 11.1 us; 1 row, 8 heads of 800 tokens 12.3 / 15.6, of 2000 19 / 16; 16 rows of 2000, 8 heads 20 / 24, of 4000 34 / 32;
-// 64 rows of 2000, 8 heads of 64 29 / 37, of 1 to 2000 18 / 19; 24 rows of 1 to 2000, 32 heads 31 / 24; 24 rows of 1 to 6000, 8 heads of 64 41 / 19.
+// 64 rows of 2000, 8 heads of 64 29 / 37, of 1 to 2000 18 / 19; 32 rows of 1030, 32 heads 38 / 40; 24 rows of 1 to 2000, 32 heads 31 / 24; 24 rows of 1 to 6000, 8 heads of 64 41 / 19.
 // Three CTAs an SM take the line in 40 us for 1 row of 100000 tokens (four 44, two 38), 24 ragged rows up to 32000 in 57 (57, 69).
 int decode_ctas(int batch, int units, int page_size, int width)
 {
     if (g_force_ctas) return g_force_ctas < 0 ? 0 : g_force_ctas;
     const long long slots = 4ll * device_sm_count(), longest = (long long)width * page_size / kChunk, all = (long long)batch * units;
     const long long waves = (all + slots - 1) / slots;
-    return longest * waves <= 40 || (waves == 1 && 5 * all >= slots && longest <= 64) ? 0 : (int)(slots / 4 * 3);
+    const long long most = waves > 1 ? 70 : 5 * all >= slots ? 64 : 40;
+    return longest * waves <= most ? 0 : (int)(slots / 4 * 3);
 }
 
 // Query heads of a unit: as many as have columns for all their groups, where that takes no more passes than 8 heads a pass.
