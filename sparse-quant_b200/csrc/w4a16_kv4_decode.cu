@@ -8,7 +8,11 @@
 // (q 2^-24 or q 2^-20) that the tensor core multiplies exactly, and is never rounded.  What is rounded to fp16: the rotated query
 // (as the cache's own keys are), scaled by a power of two of its head's largest element, which is exact; and the weight p s of a
 // (token, group), 2^-11 of it, scaled by a power of two that follows the largest step seen, so that values near fp16's smallest keep
-// their precision.  Scores, maxima, sums and the minima's part of the output are fp32.
+// their precision.  That error counts with the code n it meets, up to 15; with w the weight as rounded,
+//     sum_t p_t v_t[d] = sum_t w_t (n_t - 7.5) + sum_t p_t (m_t + 7.5 s_t) = sum_t w_t n_t + sum_t p_t (m_t + 7.5 s_t) - 7.5 sum_t w_t
+// up to errors that count with n - 7.5: half as much, for one more product a group (with ones), 1 to 5 % of the time (32 x 1030 tokens 37.8 /
+// 39.5 us; the output is off by 0.00057 / 0.00038 of it).  More than two heads in groups of 32 of 128 dims have no registers for it (54 / 92 us).
+// Scores, maxima, sums and the middles' part of the output are fp32.
 //
 // Work is dealt in chunks of 32 tokens of one (row, key/value head, 8 query heads) - a unit.  All units of all rows stand in one line,
 // and every warp of the GPU takes an equal stretch of it (four CTAs of four warps an SM), so that rows of any lengths fill the
@@ -199,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
     constexpr int NC = split_columns(NG);         // kSplit: columns of a head
     constexpr int KC = kSplit ? 1 : 2;            // heads of a lane
     constexpr int OG = kSplit ? 1 : NG;           // groups of dims whose weights are separate operands
+    constexpr bool kCentred = kSplit || NG < 4;   // codes count from their middle in what the weights' rounding leaves: see above
     constexpr int kAtOnce = kSplit && NG < 4 ? 2 : 1;   // tiles side by side: two fill the waits of each other's chains, where registers allow
     extern __shared__ __align__(128) unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c4 = lane & 3;
@@ -358,7 +363,11 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
             for (int g = 0; g < NG; ++g) qsum[g][k] = qsum_s[n * NG + g];
         }
         float acc[J][2][4];                                                     // [32 dims][pair of dims of a half-word][fragment]
-        float off[OG][2];                                                       // the minima's part: by group and head, or (kSplit) the lane's columns
+        float off[OG][2];                                                       // weights times the groups' middles: by group and head, or (kSplit) the lane's columns
+        float rounded[OG][4];                                                   // sums of the weights as the product takes them
+        constexpr uint32_t kOnes = 0x3c003c00u;
+        const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
+        auto middle = [](const float2& par) { return kCentred ? fmaf(7.5f, par.x, par.y) : par.y; };
         float ref[KC], sum[KC];
         int elog = -24;                                                         // steps are below 2^(elog + 5)
 #pragma unroll
@@ -368,7 +377,11 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[j][e][i] = 0.f;
 #pragma unroll
-        for (int g = 0; g < OG; ++g) off[g][0] = off[g][1] = 0.f;
+        for (int g = 0; g < OG; ++g) {
+            off[g][0] = off[g][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rounded[g][i] = 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
             ref[k] = -INFINITY;
@@ -525,7 +538,10 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                             keep[k] = keep[0];
                         }
 #pragma unroll
-                        for (int g = 0; g < OG; ++g) off[g][k] *= keep[k];
+                        for (int g = 0; g < OG; ++g) {
+                            off[g][k] *= keep[k];
+                            rounded[g][k] *= keep[k];
+                        }
 #pragma unroll
                         for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -553,8 +569,9 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                             gb1 = __half22float2(NC == 4 && ga ? vb[u][3 % NG] : vb[u][1]);
                         }
                         const uint32_t w0 = transpose8x8(pack2(p[0] * fa.x, p[0] * ga1.x)), w1 = transpose8x8(pack2(p[1] * fb.x, p[1] * gb1.x));
-                        off[0][0] = fmaf(p[0], fa.y, fmaf(p[1], fb.y, off[0][0]));
-                        if constexpr (NG > 1) off[0][1] = fmaf(p[0], ga1.y, fmaf(p[1], gb1.y, off[0][1]));
+                        off[0][0] = fmaf(p[0], middle(fa), fmaf(p[1], middle(fb), off[0][0]));
+                        if constexpr (NG > 1) off[0][1] = fmaf(p[0], middle(ga1), fmaf(p[1], middle(gb1), off[0][1]));
+                        if constexpr (kCentred) mma_m16n8k16(rounded[0], ones, w0, w1);
                         // output: fragment rows are dims 4 h + 2 e and the next one of half-word h = 8 j + row of the cache's order
                         uint32_t v[2][J];
                         if constexpr (J == 4) {
@@ -585,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
                             wf[g][0] = transpose8x8(pack2(p[0] * fa.x, p[KC - 1] * fa.x));
                             wf[g][1] = transpose8x8(pack2(p[KC] * fb.x, p[2 * KC - 1] * fb.x));
 #pragma unroll
-                            for (int k = 0; k < KC; ++k) off[g][k] = fmaf(p[k], fa.y, fmaf(p[KC + k], fb.y, off[g][k]));
+                            for (int k = 0; k < KC; ++k) off[g][k] = fmaf(p[k], middle(fa), fmaf(p[KC + k], middle(fb), off[g][k]));
+                            if constexpr (kCentred) mma_m16n8k16(rounded[g], ones, wf[g][0], wf[g][1]);
                         }
                         // output: fragment rows are dims 32 j + 4 row + 2 e and the next one
                         uint32_t v[4][J / 2];
@@ -634,7 +652,8 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float o = off[kSplit ? 0 : 32 * j * NG / D][k];
+                const int g = kSplit ? 0 : 32 * j * NG / D;
+                const float o = kCentred ? fmaf(-7.5f, rounded[g][k], off[g][k]) : off[g][k];
                 acc[j][0][k] = fmaf(acc[j][0][k], kDenormScaleLo, o);
                 acc[j][0][2 + k] = fmaf(acc[j][0][2 + k], kDenormScaleHi, o);
                 acc[j][1][k] = fmaf(acc[j][1][k], kDenormScaleLo, o);
