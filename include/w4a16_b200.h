@@ -331,7 +331,7 @@ int w4a16_gemm_prenorm(const void* x, const void* row_stats, const void* norm_we
  *           and its outputs stay as they were
  *   counts  int32 [batch] or NULL: new tokens of the row, at most `seq` (NULL: seq); outputs of the others stay as they were
  * head_dim 64 or 128, g 32, 64 or 128 and at most head_dim, page_size a power of two from 16 to 1024, heads a multiple of kv_heads
- * (query head h reads key/value head h / (heads / kv_heads)), width * page_size < 2^30.  Positions, page and row numbers are read
+ * (query head h reads key/value head h / (heads / kv_heads)), width * page_size < 2^30, batch and kv_heads at most 65535.  Positions, page and row numbers are read
  * on the device, so that a captured graph can be replayed: one out of range raises the device error word and is left out - 3: a
  * position outside the table or the rotary tables (that token or query is skipped), 4: a page number outside the pool (its tokens
  * are neither written nor attended to), 5: fewer free pages than asked for, 6: a row number outside the table, a fork into a row
@@ -410,8 +410,8 @@ int w4a16_static_scratch_error_flag(int* flag);
  * Both GEMM kernels bound every barrier wait; if one ever times out the kernel sets a
  * per-device error word, releases what it holds (tensor memory) and returns.  This reads that
  * word (*flag = 0: no kernel on the current device ever gave up; 1: a barrier wait inside a GEMM kernel timed out;
- * 2: a wait for a peer in the exchange gave up; 3: w4a16_decode_attention was given a position outside the
- * cache).  Synchronises the device; the first call on a device allocates the word, so make it outside stream capture.  The
+ * 2: a wait for a peer in the exchange gave up; 3: w4a16_decode_attention or a w4a16_kv4 call was given a position
+ * outside the cache; 4 to 6: what the w4a16_kv4 calls find in their tables, see there).  Synchronises the device; the first call on a device allocates the word, so make it outside stream capture.  The
  * reference has no counterpart (it checks no CUDA error at all, gemm_s4_f16_kernel.h:136-145).
  */
 int w4a16_device_error_flag(int* flag);

@@ -547,7 +547,7 @@ int check_pages(const void* table, const void* refs, int rows, int width, int pa
 {
     if (!table || !refs) return W4A16_ERR_NULL_POINTER;
     if (rows <= 0 || width <= 0 || pages <= 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return W4A16_ERR_BAD_SHAPE;
-    if ((long long)width * page_size >= (1ll << 30)) return W4A16_ERR_TOO_LARGE;
+    if ((long long)width * page_size >= (1ll << 30) || (long long)rows * width >= (1ll << 31)) return W4A16_ERR_TOO_LARGE;   // (demands are summed in 32 bits)
     if (((uintptr_t)table | (uintptr_t)refs) & 3) return W4A16_ERR_MISALIGNED;
     return W4A16_OK;
 }

@@ -112,7 +112,7 @@ def _call_shape(x, x_dims, pool, table, pos, counts, rope, heads, row_parts):
 
 def _output(out, shape, like):
     if out is None:
-        return torch.zeros(shape, dtype=torch.float16, device=like.device)
+        return like.new_zeros(shape)
     if not (isinstance(out, torch.Tensor) and _is(out, _F16, len(shape), like.get_device()) and out.shape == shape):
         _check_tensor(out, "out", dtype=torch.float16)
         _need(tuple(out.shape) == shape and out.device == like.device, f"Tensor out must have shape {list(shape)}")
@@ -147,7 +147,8 @@ def kv4_read(pool, table, pos, count: int, counts=None):
     B, _, _, dev, pages, kv, page, D, g, _, width, _, _, _ = _call_shape(None, 0, pool, table, pos, counts, None, 0, 0)
     count = int(count)
     _need(count >= 0, "count must not be negative")
-    k, v = torch.empty((2, B, kv, count, D), dtype=torch.float16, device=pool.device).unbind()
+    k = pool.new_empty((B, kv, count, D), dtype=_F16)
+    v = torch.empty_like(k)
     if B == 0 or count == 0:
         return k, v
     st = _guarded(dev, load_library().w4a16_kv4_read, pool.data_ptr(), table.data_ptr(), pos.data_ptr(), None if counts is None else counts.data_ptr(),
@@ -168,7 +169,7 @@ def kv4_decode_attention(qkv, pool, table, pos, heads: int, rope=None, scale=Non
     lib = load_library()
     ws, ws_bytes = None, lib.w4a16_kv4_decode_workspace(B, heads, kv, D, g, page, width)
     if ws_bytes:
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
+        ws = pool.new_empty(ws_bytes)
     st = _guarded(dev, lib.w4a16_kv4_decode_attention, qkv.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(), cos, sin, out.data_ptr(),
                   None if ws is None else ws.data_ptr(), ws_bytes, B, heads, kv, D, g, page, pages, width, N, rope_rows,
                   D ** -0.5 if scale is None else float(scale))
@@ -256,7 +257,7 @@ def kv4_fork(pool, table, lens, refs, src, dst):
     _need(dst.shape[0] == n, f"Tensor dst must have {n} elements")
     if n == 0:
         return
-    ws = torch.empty(4 * (4 * n + rows), dtype=torch.uint8, device=pool.device)          # w4a16_kv4_fork_workspace
+    ws = pool.new_empty(4 * (4 * n + rows))                                              # w4a16_kv4_fork_workspace
     st = _guarded(dev, load_library().w4a16_kv4_fork, pool.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(),
                   dst.data_ptr(), ws.data_ptr(), ws.shape[0], n, rows, width, layers, pages, kv, D, g, 16 * per)
     if st:
@@ -268,7 +269,7 @@ def kv4_compact(pool, table, refs):
     dev = _book_device(table, None, refs, (), pool)
     layers, pages, kv, per, tile = pool.shape
     D, g = _FORMATS[tile]
-    ws = torch.empty(4 * (3 * pages + 2), dtype=torch.uint8, device=pool.device)         # w4a16_kv4_compact_workspace
+    ws = pool.new_empty(4 * (3 * pages + 2))                                             # w4a16_kv4_compact_workspace
     st = _guarded(dev, load_library().w4a16_kv4_compact, pool.data_ptr(), table.data_ptr(), refs.data_ptr(), ws.data_ptr(), ws.shape[0],
                   table.shape[0], table.shape[1], layers, pages, kv, D, g, 16 * per)
     if st:

@@ -67,6 +67,8 @@ def test_status_codes_of_cache_calls():
     assert decode(width=10000) == 5 and decode(width=10000, ws=p, ws_bytes=need - 1) == 5 and decode(width=10000, ws=p + 2, ws_bytes=need) == 4
     assert append(seq=0) == 0 and read(seq=0) == 0 and chunk(seq=0) == 0
     assert append(seq=-1) == 2 and read(seq=-1) == 2 and chunk(seq=-1) == 2
+    for call in (append, read, decode, chunk):
+        assert call(batch=65536) == 9
     del keep
 
 
@@ -93,7 +95,7 @@ def test_status_codes_of_page_calls():
         assert call(table=p + 2) == 4 and call(refs=p + 2) == 4
         assert call(width=2 ** 27) == 9
     assert reserve(lens=None) == 1 and reserve(counts=None) == 1 and reserve(pos=None) == 1 and reserve(page=24) == 2
-    assert reserve(rows=8193) == 9
+    assert reserve(rows=8193) == 9 and free(rows=2 ** 20, width=2 ** 11) == 9
     assert free(lens=None) == 1 and free(which=None) == 1 and free(n=-1) == 2 and free(n=0, which=None) == 0
     assert fork(pool=None) == 1 and fork(lens=None) == 1 and fork(src=None) == 1 and fork(dst=None) == 1 and fork(layers=0) == 2
     assert fork(n=-1) == 2 and fork(n=8193) == 9 and fork(g=48) == 3 and fork(pool=p + 4) == 4
