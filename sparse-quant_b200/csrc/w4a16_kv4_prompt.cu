@@ -384,9 +384,9 @@ __device__ __forceinline__ void put_queries(const PromptArgs& a, const Task& w, 
     }
 }
 
-// The two products of a step, by one warp.
+// The two products of a step, by one warp, and the barriers that are told of their end.
 template <int D>
-__device__ __forceinline__ void issue_s(uint32_t s, uint64_t q_desc, uint64_t k_desc, uint32_t done)
+__device__ __forceinline__ void issue_s(uint32_t s, uint64_t q_desc, uint64_t k_desc, uint32_t done, uint32_t free = 0)
 {
     tc_fence_after_sync();
     __syncwarp();
@@ -397,11 +397,12 @@ __device__ __forceinline__ void issue_s(uint32_t s, uint64_t q_desc, uint64_t k_
             mma_f16_ss(s, q_desc + at, k_desc + at, idesc_f16_m128(kTokens), kk > 0);
         }
         tc_commit(done);
+        if (free) tc_commit(free);
     }
     __syncwarp();
 }
 template <int D>
-__device__ __forceinline__ void issue_pv(uint32_t s, uint64_t v_desc, bool first, uint32_t done)
+__device__ __forceinline__ void issue_pv(uint32_t s, uint64_t v_desc, bool first, uint32_t done, uint32_t free = 0)
 {
     tc_fence_after_sync();
     __syncwarp();
@@ -413,6 +414,7 @@ __device__ __forceinline__ void issue_pv(uint32_t s, uint64_t v_desc, bool first
             mma_f16_ts(s + kTokens, s + (kk >> 2) * 64 + (kk & 3) * 8, v_desc + at, idesc_f16_m128(D), !first || kk > 0);
         }
         tc_commit(done);
+        if (free) tc_commit(free);
     }
     __syncwarp();
 }
@@ -790,6 +792,7 @@ struct PairSmem {
     uint64_t s_done[2], pv_done[2];               // products over, by row tile
     uint64_t p_ready[2];                          // ... P written
     uint64_t k_ready[2], v_ready[2];              // operands written, by step modulo 2
+    uint64_t k_free[2], v_free[2];                // ... and both row tiles' products that read them over
     uint32_t tmem;
     int abort_flag;
     float swap[2 * 2 * kRows];
@@ -818,6 +821,8 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
             mbar_init(smem_u32(&sm.pv_done[t]), 1);
             mbar_init(smem_u32(&sm.p_ready[t]), 8);
             mbar_init(smem_u32(&sm.k_ready[t]), 8);
+            mbar_init(smem_u32(&sm.k_free[t]), 2);
+            mbar_init(smem_u32(&sm.v_free[t]), 2);
             mbar_init(smem_u32(&sm.v_ready[t]), 8);
         }
         sm.abort_flag = 0;
@@ -834,40 +839,32 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
 
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp > 16) {
+        if (warp > 17) {
             __syncthreads();
             return;
         }
-        // ---- the products, in the order in which the groups take turns: P V of the first row tile, its next S, then the second's.  P stands
-        // where S stood: S of a step is issued when P V of the step before is over
+        // ---- the products, of a row tile by a warp each, so that neither waits for what the other waits for (one warp for both, in turn:
+        // TURN us for 4096 queries behind 4096 tokens).  P stands where S stood: S of a step is issued when P V of the step before is over
         constexpr int kOperand = kRows * D * 2 / 16;                                             // q, k and v of two buffers each, one behind the other
+        const int t = warp - 16;
         const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q[0]));
-        wait(sm.k_ready[0], 0);
-        wait(sm.v_ready[0], 0);                                                                  // (with it the first group's queries)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) issue_s<D>(tmem + 256 * t, q_desc + t * kOperand, q_desc + 2 * kOperand, smem_u32(&sm.s_done[t]));
+        const uint32_t s = tmem + 256 * t;
+        wait(sm.v_ready[0], 0);                                                                  // (with it the first group's queries; the second's with the keys)
         for (int step = 0; step < w.steps; ++step) {
-            const int now = step & 1, next = now ^ 1;
-            if (step > 0) wait(sm.v_ready[now], step >> 1);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                wait(sm.p_ready[t], step);
-                issue_pv<D>(tmem + 256 * t, q_desc + (4 + now) * kOperand, step == 0, smem_u32(&sm.pv_done[t]));
-                if (step + 1 < w.steps) {
-                    if (t == 0) wait(sm.k_ready[next], (step + 1) >> 1);
-                    wait(sm.pv_done[t], step);
-                    issue_s<D>(tmem + 256 * t, q_desc + t * kOperand, q_desc + (2 + next) * kOperand, smem_u32(&sm.s_done[t]));
-                }
-            }
+            const int now = step & 1;
+            wait(sm.k_ready[now], step >> 1);
+            if (step > 0) wait(sm.pv_done[t], step - 1);
+            issue_s<D>(s, q_desc + t * kOperand, q_desc + (2 + now) * kOperand, smem_u32(&sm.s_done[t]), smem_u32(&sm.k_free[now]));
+            wait(sm.v_ready[now], step >> 1);
+            wait(sm.p_ready[t], step);
+            issue_pv<D>(s, q_desc + (4 + now) * kOperand, step == 0, smem_u32(&sm.pv_done[t]), smem_u32(&sm.v_free[now]));
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) wait(sm.pv_done[t], w.steps - 1);
+        wait(sm.pv_done[t], w.steps - 1);
         if (!ok && lane == 0) atomicExch(a.error, 1);
         __syncthreads();                                                                         // the workers have read O
-        tmem_dealloc(tmem, kTmemCols);
+        if (t == 0) tmem_dealloc(tmem, kTmemCols);
         return;
     }
-
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");  // the workers take what the products' warps leave: 16 x 104 + 4 x 56 of 20 x 96
     // ---- the groups: the first unpacks values, the second keys, each warp a tile of the step
     unsigned char* codes = sm.codes[mine] + gwarp * kHalf;
@@ -899,17 +896,21 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
     unpack(0);
     Row<F, D> row(a, w, sm.swap, 2 * kRows, mine, gwarp, lane, tmem);
     for (int step = 0; step < w.steps; ++step) {
-        // the second group unpacks first: the keys of the next step, whose buffer S of the step before has left
-        if (mine == 1 && step + 1 < w.steps) unpack(step + 1);                                   // (products are over in the order of their issue)
+        // the second group unpacks first: the keys of the next step, once S of the step before has left their buffer
+        if (mine == 1 && step + 1 < w.steps) {
+            if (step > 0) wait(sm.k_free[(step + 1) & 1], (step - 1) >> 1);
+            unpack(step + 1);
+        }
         wait(sm.s_done[mine], step);
         tc_fence_after_sync();
         if (step > 0) row.mind(sm.marks, step - 1);
         row.softmax(step, step == 0, sm.marks.pages(step));
-        // the first group unpacks afterwards: the values of the next step, whose buffer P V of the step before has left.  (Waited for before
-        // this step's P is announced: behind it the barrier could be two phases on.)
-        if (mine == 0 && step > 0) wait(sm.pv_done[1], step - 1);
         written(smem_u32(&sm.p_ready[mine]), lane);
-        if (mine == 0 && step + 1 < w.steps) unpack(step + 1);
+        // the first group afterwards: the values of the next step, once P V of the step before has left theirs
+        if (mine == 0 && step + 1 < w.steps) {
+            if (step > 0) wait(sm.v_free[(step + 1) & 1], (step - 1) >> 1);
+            unpack(step + 1);
+        }
     }
     wait(sm.pv_done[mine], w.steps - 1);
     tc_fence_after_sync();
