@@ -93,7 +93,7 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
           "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }      // this thread's
-// barriers of `threads` worker threads: 1 to 8 are the pairs of warps that share rows
+// barriers of `threads` worker threads: 1 to 8 are the pairs of warps that share rows, 9 and 10 the row tiles' turns
 __device__ __forceinline__ void meet(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t at, const uint32_t (&r)[8])
 {
@@ -107,6 +107,8 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&s)[16])
                  : "+r"(s[0]), "+r"(s[1]), "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7]), "+r"(s[8]), "+r"(s[9]), "+r"(s[10]),
                    "+r"(s[11]), "+r"(s[12]), "+r"(s[13]), "+r"(s[14]), "+r"(s[15])::"memory");
 }
+// ... and an arrival at one of them that does not wait
+__device__ __forceinline__ void let_meet(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // the warp's operand writes of either kind, made visible to the products, and its arrival
 __device__ __forceinline__ void written(uint32_t bar, int lane)
 {
@@ -263,6 +265,7 @@ template <class F, int D>
 __device__ __forceinline__ bool put_values(unsigned char* v, const unsigned char* tile, int* bad, int left, int warp, int lane)
 {
     constexpr int J = F::J;
+    asm volatile("" : "+r"(lane));              // (addresses are worked out anew each step: kept over the softmax they were spilled)
     const int vh = lane >> 2, vp2 = 2 * (lane & 3), vgroup = 32 * (vh % J) * F::NG / D;
     uint32_t w[2][J];
     __half2 par[2][2];
@@ -299,13 +302,15 @@ __device__ __forceinline__ bool put_values(unsigned char* v, const unsigned char
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const __half2 s = __lows2half2(par[i][0], par[i][1]), m = __highs2half2(par[i][0], par[i][1]);
+        // dim d of the half-words of a piece are a matrix of 8 rows, one behind the other: lane l gives the address of row l of the four
+        const uint32_t to = smem_u32(v) + operand_at(D, lane, 2 * warp + i);
 #pragma unroll
         for (int q = 0; q < J; ++q) {
             __half2 n[4];
             codes8(w[i][q], n);
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-                *reinterpret_cast<__half2*>(v + operand_at(D, 32 * q + 8 * d + vh, 2 * warp + i) + 2 * vp2) = __hfma2(n[d], s, m);
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};"
+                         ::"r"(to + q * 32 * 128), "r"(h2_bits(__hfma2(n[0], s, m))), "r"(h2_bits(__hfma2(n[1], s, m))), "r"(h2_bits(__hfma2(n[2], s, m))),
+                           "r"(h2_bits(__hfma2(n[3], s, m))) : "memory");
         }
     }
     return found;
@@ -448,8 +453,9 @@ struct Row {
         sign = a.scale_log2 == 0.f ? 0.f : a.scale_log2 < 0.f ? -1.f : 1.f;
         sum2 = pair(0.f, 0.f);
     }
-    // S of a step becomes P; 16 scores at a time, the next ones on their way
-    __device__ __forceinline__ void softmax(int step, bool first_step, uint64_t pages)
+    // S of a step becomes P; 16 scores at a time, the next ones on their way.  begin, end: around the exponentials
+    template <class Begin, class End>
+    __device__ __forceinline__ void softmax(int step, bool first_step, uint64_t pages, Begin begin, End end)
     {
         const bool masked = (step + 1) * kTokens - 1 > first || pages != 0x0101010101010101ull;
         const int seen = sees - step * kTokens - 64 * half;                                      // the last of the thread's tokens that the row sees
@@ -505,6 +511,7 @@ struct Row {
                 }
             }
         }
+        begin();
         const float shift = ref == -INFINITY ? 0.f : -ref;                                       // nothing seen yet: weights 0
         const uint64_t unit2 = pair(unit, unit), shift2 = pair(shift, shift);
 #pragma unroll
@@ -523,6 +530,7 @@ struct Row {
             }
             tmem_st_32x32b_x8(at_s + 64 * half + 8 * c, p);                                      // over columns that this thread has read
         }
+        end();
         tmem_wait_st();
     }
     // the values of a step that are not finite
@@ -763,7 +771,7 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
         if (step + 1 < w.to) fetch(step + 1);
         wait(s_bar, step);
         tc_fence_after_sync();
-        row.softmax(step, step == w.from, sm.marks.pages(step));
+        row.softmax(step, step == w.from, sm.marks.pages(step), []() {}, []() {});
         written(p_bar, lane);
         if (step + 1 < w.to) {
             unpack_keys();                                                                       // (S of this step is over)
@@ -844,7 +852,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
             return;
         }
         // ---- the products, of a row tile by a warp each, so that neither waits for what the other waits for (one warp for both, in turn:
-        // TURN us for 4096 queries behind 4096 tokens).  P stands where S stood: S of a step is issued when P V of the step before is over
+        // 600 us instead of 591 for 4096 queries behind 4096 tokens).  P stands where S stood: S of a step is issued when P V of the step before is over
         constexpr int kOperand = kRows * D * 2 / 16;                                             // q, k and v of two buffers each, one behind the other
         const int t = warp - 16;
         const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q[0]));
@@ -895,6 +903,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
     put_queries<D>(a, w, sm.q[mine], w.row0 + mine * kRows, tid);
     unpack(0);
     Row<F, D> row(a, w, sm.swap, 2 * kRows, mine, gwarp, lane, tmem);
+    if (mine == 1) let_meet(9, 2 * kGroup);                                                      // the first row tile begins
     for (int step = 0; step < w.steps; ++step) {
         // the second group unpacks first: the keys of the next step, once S of the step before has left their buffer
         if (mine == 1 && step + 1 < w.steps) {
@@ -904,7 +913,8 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
         wait(sm.s_done[mine], step);
         tc_fence_after_sync();
         if (step > 0) row.mind(sm.marks, step - 1);
-        row.softmax(step, step == 0, sm.marks.pages(step));
+        row.softmax(step, step == 0, sm.marks.pages(step), [&]() { meet(9 + mine, 2 * kGroup); },
+                    [&]() { if (mine == 0 || step + 1 < w.steps) let_meet(10 - mine, 2 * kGroup); });
         written(smem_u32(&sm.p_ready[mine]), lane);
         // the first group afterwards: the values of the next step, once P V of the step before has left theirs
         if (mine == 0 && step + 1 < w.steps) {
