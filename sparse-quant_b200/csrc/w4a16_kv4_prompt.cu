@@ -795,10 +795,10 @@ __global__ void __launch_bounds__(kGroup + 32, 2) single_kernel(const PromptArgs
 template <int D, int half_tile>
 struct PairSmem {
     alignas(1024) unsigned char q[2][kRows * D * 2], k[2][kTokens * D * 2], v[2][kTokens * D * 2];   // k, v: by step modulo 2
-    alignas(16) unsigned char codes[2][kTilesOf * half_tile];                                    // of the values (first group), of the keys
+    alignas(16) unsigned char codes[2][kTilesOf * half_tile];                                    // of the keys, of the values
     Marks marks;
     uint64_t s_done[2], pv_done[2];               // products over, by row tile
-    uint64_t p_ready[2];                          // ... P written
+    uint64_t p_ready[2], q_ready[2];              // ... P written; queries written
     uint64_t k_ready[2], v_ready[2];              // operands written, by step modulo 2
     uint64_t k_free[2], v_free[2];                // ... and both row tiles' products that read them over
     uint32_t tmem;
@@ -806,9 +806,10 @@ struct PairSmem {
     float swap[2 * 2 * kRows];
     int swap_bad[2 * kRows];
 };
+constexpr int kPairThreads = 2 * kGroup + kGroup + 128;      // the row tiles' groups, the unpackers, the products' warps
 
 template <class F, int D>
-__global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptArgs a)
+__global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const PromptArgs a)
 {
     constexpr int kHalf = F::kBytes / 2;
     constexpr uint32_t kTmemCols = 512;           // a row tile's S (then P) in 128 columns, O in the 128 behind them
@@ -818,7 +819,7 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Task w;
     if (!w.take<false>(a, 2)) return;
-    if (warp == 16) {
+    if (warp == 24) {
         tmem_alloc(smem_u32(&sm.tmem), kTmemCols);
         tmem_relinquish();
     }
@@ -828,36 +829,36 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
             mbar_init(smem_u32(&sm.s_done[t]), 1);
             mbar_init(smem_u32(&sm.pv_done[t]), 1);
             mbar_init(smem_u32(&sm.p_ready[t]), 8);
+            mbar_init(smem_u32(&sm.q_ready[t]), 8);
             mbar_init(smem_u32(&sm.k_ready[t]), 8);
+            mbar_init(smem_u32(&sm.v_ready[t]), 8);
             mbar_init(smem_u32(&sm.k_free[t]), 2);
             mbar_init(smem_u32(&sm.v_free[t]), 2);
-            mbar_init(smem_u32(&sm.v_ready[t]), 8);
         }
         sm.abort_flag = 0;
     }
     mbar_fence_init();
-    for (int i = threadIdx.x; i < 4 * kTokens; i += 2 * kGroup + 128) sm.marks.bad[0][i] = 0;
+    for (int i = threadIdx.x; i < 4 * kTokens; i += kPairThreads) sm.marks.bad[0][i] = 0;
     if (threadIdx.x < 4 * 8) sm.marks.any[0][threadIdx.x] = 0;
-    const int mine = warp >> 3, tid = threadIdx.x & (kGroup - 1), gwarp = warp & 7;              // the worker's row tile, its place in the group
-    Lookup<F> lookup(a, w, gwarp, 0);
     __syncthreads();
     const uint32_t tmem = sm.tmem;
     bool ok = true;
     auto wait = [&](uint64_t& bar, int phase) { ok = ok && mbar_wait(smem_u32(&bar), phase & 1, &sm.abort_flag, kWaitNs); };
 
-    if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp > 17) {
+    // registers of the launch: 28 warps of 72 = 16 of 88, 8 of 56, 4 of 40
+    if (warp >= 24) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp > 25) {
             __syncthreads();
             return;
         }
-        // ---- the products, of a row tile by a warp each, so that neither waits for what the other waits for (one warp for both, in turn:
-        // 600 us instead of 591 for 4096 queries behind 4096 tokens).  P stands where S stood: S of a step is issued when P V of the step before is over
+        // ---- the products, of a row tile by a warp each, so that neither waits for what the other waits for.  P stands where S stood: S of
+        // a step is issued when P V of the step before is over
         constexpr int kOperand = kRows * D * 2 / 16;                                             // q, k and v of two buffers each, one behind the other
-        const int t = warp - 16;
+        const int t = warp - 24;
         const uint64_t q_desc = smem_desc_sw128(smem_u32(sm.q[0]));
         const uint32_t s = tmem + 256 * t;
-        wait(sm.v_ready[0], 0);                                                                  // (with it the first group's queries; the second's with the keys)
+        wait(sm.q_ready[t], 0);
         for (int step = 0; step < w.steps; ++step) {
             const int now = step & 1;
             wait(sm.k_ready[now], step >> 1);
@@ -873,54 +874,59 @@ __global__ void __launch_bounds__(2 * kGroup + 128, 1) pair_kernel(const PromptA
         if (t == 0) tmem_dealloc(tmem, kTmemCols);
         return;
     }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");  // the workers take what the products' warps leave: 16 x 104 + 4 x 56 of 20 x 96
-    // ---- the groups: the first unpacks values, the second keys, each warp a tile of the step
-    unsigned char* codes = sm.codes[mine] + gwarp * kHalf;
-    bool page_fails = false;
-    auto fetch = [&](int step) {                                                                 // the step's codes, and the page of the one behind it
-        const unsigned char* tile = lookup.tile(step);
-        page_fails = lookup.fails(tile, step);
-        load_codes<F, D>(codes, tile, mine == 0, lane, a.c.pool);
-        lookup.look(step + 1);
-    };
-    auto unpack = [&](int step) {                                                                // what was fetched, into the buffer of step modulo 2
-        copies_landed();
-        __syncwarp();
-        if (mine == 0) {
-            put_values_of<F, D>(sm.marks, sm.v[step & 1], codes, w, step, gwarp, lane);
-            written(smem_u32(&sm.v_ready[step & 1]), lane);
-        } else {
-            put_keys<F, D>(sm.k[step & 1], codes, gwarp, lane);
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        // ---- the unpackers, each warp a tile of the step: its keys, its values; the codes of the step behind on their way meanwhile
+        const int gwarp = warp - 16;
+        unsigned char *k_codes = sm.codes[0] + gwarp * kHalf, *v_codes = sm.codes[1] + gwarp * kHalf;
+        Lookup<F> lookup(a, w, gwarp, 0);
+        const unsigned char* tile = lookup.tile(0);
+        bool fails = lookup.fails(tile, 0);
+        load_codes<F, D>(k_codes, tile, false, lane, a.c.pool);
+        load_codes<F, D>(v_codes, tile, true, lane, a.c.pool);
+        lookup.look(1);
+        for (int step = 0; step < w.steps; ++step) {
+            const int now = step & 1;
+            const bool more = step + 1 < w.steps;
+            copies_landed();
+            __syncwarp();
+            if (step > 1) wait(sm.k_free[now], (step - 2) >> 1);
+            put_keys<F, D>(sm.k[now], k_codes, gwarp, lane);
             if (lane == 0) {
-                sm.marks.page_ok[step & 3][gwarp] = !page_fails;
-                if (page_fails) atomicExch(a.error, kErrPage);
+                sm.marks.page_ok[step & 3][gwarp] = !fails;
+                if (fails) atomicExch(a.error, kErrPage);
             }
-            written(smem_u32(&sm.k_ready[step & 1]), lane);
+            written(smem_u32(&sm.k_ready[now]), lane);
+            if (more) {
+                tile = lookup.tile(step + 1);
+                fails = lookup.fails(tile, step + 1);
+                load_codes<F, D>(k_codes, tile, false, lane, a.c.pool);
+                lookup.look(step + 2);
+            }
+            if (step > 1) wait(sm.v_free[now], (step - 2) >> 1);
+            put_values_of<F, D>(sm.marks, sm.v[now], v_codes, w, step, gwarp, lane);
+            written(smem_u32(&sm.v_ready[now]), lane);
+            if (more) load_codes<F, D>(v_codes, tile, true, lane, a.c.pool);
         }
-        if (step + 1 < w.steps) fetch(step + 1);
-    };
-    fetch(0);
+        if (!ok && lane == 0) atomicExch(a.error, 1);
+        __syncthreads();
+        return;
+    }
+
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    // ---- the row tiles' groups
+    const int mine = warp >> 3, tid = threadIdx.x & (kGroup - 1);
     put_queries<D>(a, w, sm.q[mine], w.row0 + mine * kRows, tid);
-    unpack(0);
-    Row<F, D> row(a, w, sm.swap, 2 * kRows, mine, gwarp, lane, tmem);
+    written(smem_u32(&sm.q_ready[mine]), lane);
+    Row<F, D> row(a, w, sm.swap, 2 * kRows, mine, warp & 7, lane, tmem);
     if (mine == 1) let_meet(9, 2 * kGroup);                                                      // the first row tile begins
     for (int step = 0; step < w.steps; ++step) {
-        // the second group unpacks first: the keys of the next step, once S of the step before has left their buffer
-        if (mine == 1 && step + 1 < w.steps) {
-            if (step > 0) wait(sm.k_free[(step + 1) & 1], (step - 1) >> 1);
-            unpack(step + 1);
-        }
         wait(sm.s_done[mine], step);
         tc_fence_after_sync();
         if (step > 0) row.mind(sm.marks, step - 1);
         row.softmax(step, step == 0, sm.marks.pages(step), [&]() { meet(9 + mine, 2 * kGroup); },
                     [&]() { if (mine == 0 || step + 1 < w.steps) let_meet(10 - mine, 2 * kGroup); });
         written(smem_u32(&sm.p_ready[mine]), lane);
-        // the first group afterwards: the values of the next step, once P V of the step before has left theirs
-        if (mine == 0 && step + 1 < w.steps) {
-            if (step > 0) wait(sm.v_free[(step + 1) & 1], (step - 1) >> 1);
-            unpack(step + 1);
-        }
     }
     wait(sm.pv_done[mine], w.steps - 1);
     tc_fence_after_sync();
@@ -977,7 +983,7 @@ int launch_prompt(PromptArgs& a, long long rows, cudaStream_t st)
             static_assert(sizeof(S) + 1024 <= 232448, "fits the SM");
             static int configured[64] = {0};
             a.blocks = (int)((tiles + 1) / 2);
-            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, 2 * kGroup + 128, a, st);
+            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, kPairThreads, a, st);
         }
     }
     using S = SingleSmem<D, F::kBytes / 2>;
