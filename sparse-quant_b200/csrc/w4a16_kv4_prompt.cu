@@ -1,23 +1,29 @@
 // Attention of a chunk of queries over the paged 4-bit cache, on the 5th-generation tensor cores.
 //
-// Row f of the chunk's S x R is query f / R of head f % R of the R that share the key/value head.  128 rows are a row tile; for each of its
-// row tiles a CTA walks over steps of 128 cached tokens, up to its last query's position:
+// Row f of the chunk's S x R is query f / R of head f % R of the R that share the key/value head.  128 rows are a row tile; a CTA walks
+// over steps of 128 cached tokens, up to its last query's position, and for each of its row tiles:
 //     S = Q K^T     128 x 128, Q and K in shared memory, S in tensor memory
-//     P = 2^(S scale - ref), rounded to fp16, over S's place in tensor memory; ref follows the row's maximum by steps of 2^8 and more
+//     P = 2^(S scale - ref), over S's place in tensor memory; ref follows the row's maximum by steps of 2^8 and more
 //     O += P V      P in tensor memory, V^T in shared memory, O in tensor memory
-// K and V come as codes: worker warps turn m + n s into fp16 (one rounding, 2^-11 of the value) while the products run, and write the
-// 128-byte swizzled layouts the products read - keys by tokens (dims of a word of 8 in the order 0 4 1 5 2 6 3 7 that the codes unpack
-// in; the queries are stored in the same order), values by dims: a transposing matrix load gives a lane the same four dims of two tokens,
-// which unpack side by side.  The rows of V^T, and with them the columns of O, stand in the order 8 n + h + 32 p of dim n of the half-word
-// 8 p + h that the cache stores, which puts the eight rows that one store instruction touches on different banks.  The codes of the next
-// step are on their way to shared memory meanwhile, and where its tiles stand is looked up two steps ahead.  Two threads a row in the
-// softmax, eight warps a row tile, and one warp that issues the products (issuing eight takes as long as they run).
+// The products take fp16: queries are rounded to it once rotated (as the cache's own keys were), m + n s once (2^-11 of the value, a hundred
+// times less than the codes' own coarseness), P once.  S, O, maxima and sums are fp32.
 //
-// What bounds it is what the workers can issue, and the exponentials (16 a clock): a step of K and V costs as much to unpack as a row tile's
-// softmax.  Where there are many row tiles of 128 dims a CTA has two (pair_kernel, one CTA an SM), whose warps take turns: while one
-// row tile is in its softmax the other's warps unpack - the first row tile's the values, the second's the keys, into two buffers each -, and
-// the tensor cores run the products of whichever is ready.  Otherwise (single_kernel) one row tile, two CTAs an SM; where there are few, the
-// CTAs of a cluster share the steps of a row tile and join their (reference, sum, O) through each other's shared memory.
+// K and V come as codes, which warps unpack while the products run, into the 128-byte swizzled layouts the products read - keys by
+// tokens (dims of a word of 8 in the order 0 4 1 5 2 6 3 7 that the codes unpack in; the queries are stored in the same order), values by
+// dims: a transposing matrix load gives a lane the same four dims of two tokens, which unpack side by side and are stored as matrices.  The
+// rows of V^T, and with them the columns of O, stand in the order 8 n + h + 32 p of dim n of the half-word 8 p + h that the cache stores.
+// A warp fetches and unpacks a 16-token tile of the step by itself; the codes of the next step are on their way to shared memory meanwhile,
+// and its page is looked up a step ahead.  Two threads a row in the softmax, eight warps a row tile; the products are issued by a warp that
+// does nothing else (issuing eight takes as long as they run).
+//
+// Where there are many row tiles a CTA has two (pair_kernel, one CTA an SM, 28 warps): eight warps each for their softmax, which
+// take turns at the exponentials (without turns 650 us instead of 545 for 4096 queries behind 4096 tokens, 32 heads on 8), and eight that
+// unpack for both, into two buffers of K and V.  That is 750 TFLOP/s.  It is bound by the chain of a row tile: P V, the next S (1900 cycles
+// until its scores are there), their maximum (900) and exponentials (1500); two row tiles fill tensor memory.  Before: the groups unpacked
+// between their softmaxes 571, one row tile's warps after the other 776.
+// Otherwise (single_kernel) one row tile, two CTAs an SM, whose eight warps do everything in turn: 8 x 77 queries behind 1000 tokens 50 us.
+// Where there are few row tiles, the CTAs of a cluster share the steps of each and join their (reference, sum, O) through each other's
+// shared memory: 8 queries behind 8000 tokens 35 us.
 //
 // A value whose group is not finite is multiplied as 0, so that rows that must not see its token stay clean, and the rows that do see it
 // get NaN for that group's dims at the end.
@@ -965,26 +971,24 @@ int launch_prompt_as(K kernel, int (&configured)[64], int smem, int threads, con
     return W4A16_OK;
 }
 
-// Two row tiles a CTA (128 dims; at 64 a step of K and V costs half as much to unpack, and two CTAs that wait for each other's products did
-// better, 243 / 265 us for 2 x 2048 queries behind 1000 tokens) as soon as there are more row tiles than SMs: for 32 heads on 8, 800 queries
-// behind 4096 tokens take 127 us so and 172 one by one, 640 take 122 and 159; with 512 every row tile has an SM, and two CTAs that share its
-// steps: 122 and 95.  One by one, clusters share row tiles as long as two CTAs an SM hold all of them - an idle CTA keeps its place until its
-// cluster is done: 32 x 8 queries behind 1030 tokens took 90 us with two to a cluster, 48 with none; where they fit, 8 queries behind 8000
-// tokens take 35 us and 193 without.
+// Two row tiles a CTA as soon as there are more row tiles than clusters of two CTAs can take at once, which is not one for every SM (128 row
+// tiles in clusters of two take 91 us, 136 143): for 32 heads on 8 of 128 dims, 544 queries behind 4096 tokens take 113 us so and 143 one
+// by one, 800 115 and 160, 2048 262 and 347, 4096 of 64 dims 472 and 569; with 512 queries every row tile has two CTAs that share its steps:
+// 110 and 91.  One by one, clusters share row tiles as long as all of them are resident - an idle CTA keeps its place until its cluster is
+// done: 32 x 8 queries behind 1030 tokens took 90 us with two to a cluster, 48 with none; where they fit, 8 queries behind 8000 tokens take
+// 35 us and 193 without.
 template <class F, int D>
 int launch_prompt(PromptArgs& a, long long rows, cudaStream_t st)
 {
     const int sms = device_sm_count();
     const long long tiles = (rows + kRows - 1) / kRows, all = tiles * a.c.kv_heads * a.batch;
     a.ranks = 1;
-    if constexpr (D == 128) {
-        if (rows > kRows && all > sms) {
-            using S = PairSmem<D, F::kBytes / 2>;
-            static_assert(sizeof(S) + 1024 <= 232448, "fits the SM");
-            static int configured[64] = {0};
-            a.blocks = (int)((tiles + 1) / 2);
-            return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, kPairThreads, a, st);
-        }
+    if (rows > kRows && 8 * all > 7 * sms) {
+        using S = PairSmem<D, F::kBytes / 2>;
+        static_assert(sizeof(S) + 1024 <= 232448, "fits the SM");
+        static int configured[64] = {0};
+        a.blocks = (int)((tiles + 1) / 2);
+        return launch_prompt_as(pair_kernel<F, D>, configured, (int)sizeof(S) + 1024, kPairThreads, a, st);
     }
     using S = SingleSmem<D, F::kBytes / 2>;
     static_assert(sizeof(S) + 1024 <= 115712, "two fit the SM");
@@ -992,7 +996,7 @@ int launch_prompt(PromptArgs& a, long long rows, cudaStream_t st)
     a.slots = 2 * sms;
     a.blocks = (int)tiles;
     const long long steps = ((long long)a.c.width << a.c.page_shift) / kTokens;
-    while (a.ranks < kMostRanks && 2 * a.ranks * kLeastSteps <= steps && 2 * a.ranks * all <= a.slots) a.ranks *= 2;
+    while (a.ranks < kMostRanks && 2 * a.ranks * kLeastSteps <= steps && 2 * a.ranks * 8 * all <= 7 * a.slots) a.ranks *= 2;
     return launch_prompt_as(single_kernel<F, D>, configured, (int)sizeof(S) + 1024, kGroup + 32, a, st);
 }
 

@@ -463,11 +463,11 @@ def test_chunk_attention_of_few_rows_over_many_tokens(D, G, heads, kv, S, ctx, c
     _chunk_against_torch(heads, kv, D, G, 64, S, ctx, counts)
 
 
-@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("D,G", kv4.formats())
 @pytest.mark.parametrize("ctx,counts", [([0, 300, 129], None), ([127, -1, 1000], [1100, 0, 250])])
-def test_chunk_attention_of_many_rows(G, ctx, counts):
+def test_chunk_attention_of_many_rows(D, G, ctx, counts):
     """Two row tiles a CTA, whole and partly filled ones."""
-    _chunk_against_torch(10, 2, 128, G, 32, 1100, ctx, counts)
+    _chunk_against_torch(10, 2, D, G, 32, 1100, ctx, counts)
 
 
 @pytest.mark.parametrize("heads,kv,S,ctx", [(4, 2, 5, [1300, 900]), (10, 2, 1100, [300, 0, 140])])
