@@ -1,4 +1,4 @@
-"""Checker of the paged 4-bit key/value cache: the format in numpy (fp32 arithmetic step by step, as the definition has it), attention in
+"""Oracle of the paged 4-bit key/value cache: the format in numpy (fp32 arithmetic step by step, as the definition has it), attention in
 float64, the page operations as plain loops over Python lists.  Nothing here is imported by the product."""
 import numpy as np
 

@@ -27,8 +27,8 @@
 // and the accumulator of the first is the layout the second needs after an 8x8 transpose (movmatrix).  A weight p s depends on the group
 // of the dim.  Where the eight columns hold all (head, group) pairs (kSplit: up to 4 heads, 2 in groups of 32 of 128 dims) one product
 // runs with all of them and each dim takes the column of its group at the end: values then come transposed from a matrix load, whatever
-// groups its rows mix, and a lane has one score a token instead of two.  Otherwise the columns are 8 heads and a group of dims has its
-// own weights.  Weights are 2^(score - ref)
+// groups its rows mix, and a lane has one score a token instead of two (32 rows of 1030 tokens, 32 heads, 39.3 us, as below 43.0; 1 row of
+// 100000, 32 heads on 8, groups of 64, 40.4 and 44.2).  Otherwise the columns are 8 heads and a group of dims has its own weights.  Weights are 2^(score - ref)
 // with ref = maximum + log2 of the largest step, moved only when a score exceeds the maximum by 2^8 or a step the largest by 2^5.
 #include "w4a16_kv4.cuh"
 
@@ -204,7 +204,9 @@ __global__ void __launch_bounds__(kThreads, 4) decode_kernel(const DecodeArgs a)
     constexpr int KC = kSplit ? 1 : 2;            // heads of a lane
     constexpr int OG = kSplit ? 1 : NG;           // groups of dims whose weights are separate operands
     constexpr bool kCentred = kSplit || NG < 4;   // codes count from their middle in what the weights' rounding leaves: see above
-    constexpr int kAtOnce = kSplit && NG < 4 ? 2 : 1;   // tiles side by side: two fill the waits of each other's chains, where registers allow
+    // tiles side by side: two fill the waits of each other's chains, where registers allow.  One / two at a time: 32 rows of 1030 tokens, 32 heads,
+    // groups of 64, 40.6 / 39.3 us; 16 rows of 2000, 40 heads on 8, 25.9 / 22.9; 1 row of 100000, 32 heads on 8, groups of 32, 54 / 82
+    constexpr int kAtOnce = NG < 4 ? 2 : 1;
     extern __shared__ __align__(128) unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c4 = lane & 3;
     unsigned char* ring = raw + warp * L::warp_bytes(a.cols);

@@ -1,4 +1,4 @@
-"""The paged 4-bit key/value cache on the GPU against the checker (oracle/kv4.py).
+"""The paged 4-bit key/value cache on the GPU against the oracle (oracle/kv4.py).
 
 Append is compared byte for byte: quantisation and rotation are single fp32 operations in a fixed order.  Reading back rounds m + n s to
 fp16 once: half a step, 2^-11 of the value (2^-25 below fp16's normal numbers), and the same again for the fp32 step in between.
@@ -45,7 +45,7 @@ def _rope(n, D, seed):
 
 
 class Case:
-    """A cache of random rows with shuffled pages, in numpy (what the checker holds) and on the device."""
+    """A cache of random rows with shuffled pages, in numpy (what the oracle holds) and on the device."""
 
     def __init__(self, lens, kv, heads, D, G, P, seed=0, new=1, rope=False, pad=0, scale_v=1.0, dead=()):
         rng = np.random.default_rng(seed)
@@ -116,7 +116,7 @@ def _bytes(t):
 
 @pytest.mark.parametrize("D,G", kv4.formats())
 @pytest.mark.parametrize("rope", [False, True])
-def test_append_writes_the_checkers_bytes(D, G, rope):
+def test_append_writes_the_oracles_bytes(D, G, rope):
     import quant
     for P, lens, new, kv, pad, counts in ((16, [0, 5, 15, 16], 19, 2, 0, None), (64, [3, 0, 60], 9, 1, 8, [9, 0, 5]), (32, [0], 1, 3, 64, None)):
         c = Case(lens, kv, 2 * kv, D, G, P, seed=D + G + P, new=new, rope=rope, pad=pad, dead=(1,) if P == 64 else ())
@@ -139,7 +139,7 @@ def test_append_writes_the_checkers_bytes(D, G, rope):
 
 
 def test_append_edges_of_the_quantiser():
-    """Constant groups, the widest and the smallest ranges, infinities and NaN: the checker's bytes (NaN scales compare as bytes too)."""
+    """Constant groups, the widest and the smallest ranges, infinities and NaN: the oracle's bytes (NaN scales compare as bytes too)."""
     import quant
     D, G = 128, 64
     c = Case([0], 1, 1, D, G, 16, new=7)

@@ -1,5 +1,5 @@
 """The paged 4-bit key/value cache without a GPU: argument errors come back as status codes or RuntimeError before anything is
-launched, and the checker that the GPU tests use agrees with itself."""
+launched, and the oracle that the GPU tests use agrees with itself."""
 import ctypes
 
 import numpy as np
