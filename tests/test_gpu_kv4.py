@@ -420,7 +420,7 @@ def _chunk_against_torch(heads, kv, D, G, P, S, ctx, counts=None, spoil=(), hidd
     for b, p in hidden:
         table[b, p] = B * width + 5
     pos = torch.tensor(ctx, dtype=torch.int32, device="cuda")
-    q = torch.zeros(B, S, heads * D, dtype=torch.float16, device="cuda")
+    q = torch.full((B, S, heads * D), float("nan"), dtype=torch.float16, device="cuda")      # (padding is not read)
     for b, c in enumerate(ctx):
         if c >= 0:
             q[b, :n[b] - c] = x[b, c:n[b], :heads * D]
@@ -688,6 +688,56 @@ def test_on_another_stream_and_captured():
     torch.cuda.synchronize()
     for g, s, ref in graphs:
         assert torch.equal(s["out"], ref)
+
+
+def test_calls_at_once_on_two_streams_and_from_two_graphs():
+    """Token steps dealt over the whole GPU, chunks of few and of many rows: two programs at once, eager and captured, each with its own
+    workspaces, give bit by bit what they give alone."""
+    import quant
+    programs = []
+    for seed, heads, kv, D, G, n in ((1, 32, 8, 128, 64, 9000), (2, 16, 16, 64, 32, 7000)):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        width = n // 64 + 2
+        pool = quant.kv4_pool(1, 2 * width, kv, D, 64, G)
+        table = torch.randperm(2 * width, device="cuda", generator=g).int().view(2, -1)
+        N = (heads + 2 * kv) * D
+        x = torch.randn(2, n, N, device="cuda", generator=g).half()
+        quant.kv4_append(x, pool[0], table, torch.zeros(2, dtype=torch.int32, device="cuda"), heads)
+        pos = torch.tensor([n, n // 3], dtype=torch.int32, device="cuda")
+        few, many = x[:, :9].contiguous(), x[:, :1500].contiguous()
+
+        def run(pool=pool[0], table=table, pos=pos, heads=heads, one=x[:, 0].contiguous(), few=few, many=many):
+            early = torch.clamp(pos - 2000, min=0)
+            return (quant.kv4_decode_attention(one, pool, table, pos, heads), quant.kv4_attention(few, pool, table, pos - 10, heads),
+                    quant.kv4_attention(many, pool, table, early, heads))
+        programs.append(run)
+    alone = [tuple(t.clone() for t in run()) for run in programs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in programs]
+    for _ in range(3):
+        got = []
+        for st, run in zip(streams, programs):
+            with torch.cuda.stream(st):
+                got.append(run())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(alone, got) for a, b in zip(x, y))
+    graphs, outs = [], []
+    for st, run in zip(streams, programs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(run())
+        graphs.append(graph)
+    for _ in range(3):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(alone, outs) for a, b in zip(x, y))
+    assert _take_error() == 0
 
 
 def test_offsets_beyond_32_bits():
