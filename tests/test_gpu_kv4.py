@@ -463,6 +463,14 @@ def test_chunk_attention_of_few_rows_over_many_tokens(D, G, heads, kv, S, ctx, c
     _chunk_against_torch(heads, kv, D, G, 64, S, ctx, counts)
 
 
+@pytest.mark.parametrize("D,G", [(64, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("counts", [None, [3 - i % 4 for i in range(41)]])
+def test_chunk_attention_of_ragged_batches(D, G, counts):
+    """Rows much longer than the others, rows without a sequence, a wide table."""
+    ctx = [3000 if i == 7 else 1700 if i == 30 else -1 if i % 11 == 5 else (37 * i) % 260 for i in range(41)]
+    _chunk_against_torch(8, 4, D, G, 32, 3, ctx, counts)
+
+
 @pytest.mark.parametrize("D,G", kv4.formats())
 @pytest.mark.parametrize("ctx,counts", [([0, 300, 129], None), ([127, -1, 1000], [1100, 0, 250])])
 def test_chunk_attention_of_many_rows(D, G, ctx, counts):
