@@ -1,4 +1,4 @@
-// Decode attention over the paged 4-bit cache: one new token per row, appended and attended to in one launch.
+// Decode attention over the paged 4-bit cache: one new token per row, appended and attended to in one call.
 //
 // Mathematics.  With codes n, steps s and minima m per group g of a head row, a score is
 //     k . q = sum_g  s_g (sum_{d in g} n_d q_d) + m_g (sum_{d in g} q_d)
@@ -9,18 +9,22 @@
 // (as the cache's own keys are), scaled by a power of two of its head's largest element, which is exact; and the weight p s of a
 // (token, group), 2^-11 of it, scaled by a power of two that follows the largest step seen, so that values near fp16's smallest keep
 // their precision.  That error counts with the code n it meets, up to 15; with w the weight as rounded,
-//     sum_t p_t v_t[d] = sum_t w_t (n_t - 7.5) + sum_t p_t (m_t + 7.5 s_t) = sum_t w_t n_t + sum_t p_t (m_t + 7.5 s_t) - 7.5 sum_t w_t
-// up to errors that count with n - 7.5: half as much, for one more product a group (with ones), 1 to 5 % of the time (32 x 1030 tokens 37.8 /
+//     sum_t w_t (n_t - 7.5) + sum_t p_t (m_t + 7.5 s_t) = sum_t w_t n_t + sum_t p_t (m_t + 7.5 s_t) - 7.5 sum_t w_t
+// is the output up to errors that count with n - 7.5: half as much, for one more product a group (with ones), 1 to 5 % of the time (32 x 1030 tokens 37.8 /
 // 39.5 us; the output is off by 0.00057 / 0.00038 of it).  More than two heads in groups of 32 of 128 dims have no registers for it (54 / 92 us).
 // Scores, maxima, sums and the middles' part of the output are fp32.
 //
 // Work is dealt in chunks of 32 tokens of one (row, key/value head, 8 query heads) - a unit.  All units of all rows stand in one line,
-// and every warp of the GPU takes an equal stretch of it (four CTAs of four warps an SM), so that rows of any lengths fill the
+// and every warp of the GPU takes an equal stretch of it (three CTAs of four warps an SM), so that rows of any lengths fill the
 // machine.  A stretch is cut into segments at the ends of units; a segment that is not a whole unit leaves (reference, sum, output) in a
 // workspace, which join_kernel puts together.  Where a CTA's four stretches lie in one unit its warps meet in shared memory first.  Short
 // rows are dealt by units instead, a CTA each, and need no second launch.  A warp streams its chunks through a ring
 // of its own in shared memory (16-byte asynchronous copies; two adjacent tiles are one run, from pages of 32 tokens on), across segments.
-// (Copies by one lane in bulk cost three times the instructions here: the loop is bound by what the warps can issue.)
+// (Copies by one lane in bulk cost three times the instructions here.)
+//
+// What bounds it: 225 instructions for a tile of 16 tokens, issued at 0.5 a cycle and scheduler by the 12 to 16 warps an SM that 128 registers
+// allow; without its copies it was 16 % faster.  32 rows of 1030 tokens, 32 heads of 128 in groups of 64: 39.3 us, 3.9 TB/s; 1 row of 100000, 32
+// heads on 8, groups of 128: 38.5 us, 2.8 TB/s.  Before: a warp per 16 tokens and floats throughout 188, queries as columns of one group 48.
 //
 // Queries that share the key/value head are columns of mma.m16n8k16:
 //     scores  A = keys (16 tokens x 16 dims), B = queries;   output  A = values^T (16 dims x 16 tokens), B = weights
