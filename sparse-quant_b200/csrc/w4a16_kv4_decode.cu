@@ -24,7 +24,7 @@
 //
 // What bounds it: 225 instructions for a tile of 16 tokens, issued at 0.5 a cycle and scheduler by the 12 to 16 warps an SM that 128 registers
 // allow; without its copies it was 16 % faster.  32 rows of 1030 tokens, 32 heads of 128 in groups of 64: 39.3 us, 3.9 TB/s; 1 row of 100000, 32
-// heads on 8, groups of 128: 38.5 us, 2.8 TB/s.  Before: a warp per 16 tokens and floats throughout 188, queries as columns of one group 48.
+// heads on 8, groups of 128: 38.5 us, 2.8 TB/s.  The first simple kernel took 188 for the former.
 //
 // Queries that share the key/value head are columns of mma.m16n8k16:
 //     scores  A = keys (16 tokens x 16 dims), B = queries;   output  A = values^T (16 dims x 16 tokens), B = weights
